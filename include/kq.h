@@ -319,6 +319,81 @@ kq_status_t kq_fa_decode_q8_0_ragged(const void* q_f16, const void* k, const voi
                                      int B, int Hq, int Hkv, int D, int max_seqlen, int total_rows, float scale,
                                      void* out_f16, kq_stream_t stream);
 
+/* ---- 3. Paged serving ------------------------------------------------------ */
+
+/* 16-bit types of activations, queries and outputs below. */
+#define KQ_F16 0
+#define KQ_BF16 1
+
+/* A paged q8_0 cache: k_cache and v_cache are [num_pages, page_size, Hkv,
+ * D/32] q8_0 blocks (34 B). Slot page * page_size + i is token row i of a
+ * page; block_tables int32 [B, max_blocks] gives the page of each run of
+ * page_size tokens of a sequence. The reference has no paged cache; the
+ * block format is its q8_0 (quantize_to_q8_0, quantize.py:105-162).
+ *
+ * kq_page_plan: tables and slot map of one serving step, from the lengths.
+ * cached_lens, new_lens int32 [B]: tokens of request b already in the cache
+ * and tokens it adds now (negative counts as 0). Request b's new pages are
+ * appended to its table row at column ceil(cached / page_size), taken from
+ * free_pages int32 [num_free] in request order (-1 where the list is too
+ * short). Outputs: slots int64 [total_new], one per new token in packed
+ * request order (-1 for a token without a page, past max_blocks, or past the
+ * new tokens); seq_lens int32 [B] = cached + new; cu_new, cu_seqlens int32
+ * [B+1], prefix sums of new_lens and seq_lens; counts int32 [2]: pages the
+ * step needs (more than num_free: the list was too short) and new tokens that
+ * got no slot. Lengths sum to less than 2^31. A shared prefix is whole pages
+ * already in the tables and counted in cached_lens. No device value is read
+ * back. */
+kq_status_t kq_page_plan(const int32_t* cached_lens, const int32_t* new_lens, int B, int32_t* block_tables,
+                         int max_blocks, const int32_t* free_pages, int num_free, int page_size, int64_t total_new,
+                         int64_t* slots, int32_t* seq_lens, int32_t* cu_new, int32_t* cu_seqlens, int32_t* counts,
+                         kq_stream_t stream);
+
+/* Rows k, v [T, Hkv, D] (dtype KQ_F16 or KQ_BF16; row and head strides in
+ * elements, last dimension contiguous) quantised to q8_0 into the cache rows
+ * slots[t] (int64; below 0 or >= num_slots: the row is skipped). The bytes
+ * are those of kq_quantize_rows on the same values. Slots of one call must
+ * differ. */
+kq_status_t kq_page_write_q8_0(int dtype, const void* k, const void* v, int64_t k_row_stride, int64_t k_head_stride,
+                               int64_t v_row_stride, int64_t v_head_stride, const int64_t* slots, int64_t T, int Hkv,
+                               int D, void* k_cache, void* v_cache, int64_t num_slots, kq_stream_t stream);
+
+/* The sequences' cache rows in packed order: row cu_seqlens[b] + i of k and v
+ * [total_rows, Hkv, D] is token i of sequence b, d * code rounded to dtype.
+ * Rows of pages outside the cache, and rows past cu_seqlens[B], are zero. */
+kq_status_t kq_page_read_q8_0(int dtype, const void* k_cache, const void* v_cache, int64_t num_pages, int page_size,
+                              int Hkv, int D, const int32_t* block_tables, int max_blocks, const int32_t* cu_seqlens,
+                              int B, int64_t total_rows, void* k, void* v, kq_stream_t stream);
+
+/* Attention of packed prompts: q [Tq, Hq, D], k and v [Tk, Hkv, D] (row and
+ * head strides in elements, last dimension contiguous), out [Tq, Hq, D]
+ * contiguous, all of dtype. Sequence b owns q rows cu_seqlens_q[b] ..
+ * cu_seqlens_q[b+1]-1 and k / v rows cu_seqlens_k[b] .. (int32 [B+1],
+ * device); query head h reads KV head h / (Hq / Hkv); causal: row i sees keys
+ * j <= i + (len_k - len_q). A row without keys is zero. D % 8 == 0, D <= 256.
+ * workspace: kq_fa_prompt_workspace() bytes of device memory, 16-byte
+ * aligned, used by this call only until it has run. */
+size_t kq_fa_prompt_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int D);
+kq_status_t kq_fa_prompt(int dtype, const void* q, const void* k, const void* v, int64_t q_row_stride,
+                         int64_t q_head_stride, int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+                         int64_t v_head_stride, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int B, int Tq,
+                         int Tk, int Hq, int Hkv, int D, int causal, float scale, void* out, void* workspace,
+                         size_t workspace_bytes, kq_stream_t stream);
+
+/* Decode over the paged q8_0 cache, one query token per sequence: q and out
+ * [B, Hq, D] contiguous, of dtype; seq_lens int32 [B] (device), 0 for a
+ * padding row (its output is zero). The first prefix_len tokens are the same
+ * pages for every sequence: they are read once for the whole batch, through
+ * row 0 of block_tables; a sequence shorter than that sees its first
+ * seq_lens[b] of them. max_seqlen bounds the lengths (it
+ * sizes the work split; longer sequences are cut to it). Tokens in pages
+ * outside the cache are hidden. D % 32 == 0, D <= 256. workspace as above. */
+size_t kq_fa_decode_paged_workspace(int B, int Hq, int Hkv, int D, int prefix_len, int max_seqlen);
+kq_status_t kq_fa_decode_paged(int dtype, const void* q, const void* k_cache, const void* v_cache, int64_t num_pages,
+                               int page_size, const int32_t* block_tables, int max_blocks, const int32_t* seq_lens,
+                               int B, int Hq, int Hkv, int D, int prefix_len, int max_seqlen, float scale, void* out,
+                               void* workspace, size_t workspace_bytes, kq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

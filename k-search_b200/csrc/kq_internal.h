@@ -192,5 +192,45 @@ kq_status_t launch_fa_batch_mha(int kv_format, const float* q, const void* k, co
                                 int S, int H, cudaStream_t s);
 kq_status_t launch_fa_ragged(const void* q, const void* k, const void* v, const int32_t* cu, int B, int Hq, int Hkv,
                              int D, int max_seqlen, int total_rows, float scale, void* out, cudaStream_t s);
+// paged.cu: the paged q8_0 cache
+kq_status_t launch_page_plan(const int32_t* cached, const int32_t* fresh, int B, int32_t* table, int W,
+                             const int32_t* free_pages, int F, int ps, int64_t T, int64_t* slots, int32_t* seq_lens,
+                             int32_t* cu_new, int32_t* cu_seqlens, int32_t* counts, cudaStream_t s);
+// strides: k row, k head, v row, v head (elements)
+kq_status_t launch_page_write_q8_0(int dtype, const void* k, const void* v, const int64_t* strides,
+                                   const int64_t* slots, int64_t T, int H, int D, void* k_cache, void* v_cache,
+                                   int64_t num_slots, cudaStream_t s);
+kq_status_t launch_page_read_q8_0(int dtype, const void* k_cache, const void* v_cache, int64_t num_pages, int ps,
+                                  int H, int D, const int32_t* table, int W, const int32_t* cu, int B, int64_t rows,
+                                  void* k, void* v, cudaStream_t s);
+// fa_prompt.cu: attention of packed prompts. Strides in elements; out is
+// contiguous [Tq, Hq, D]; ws holds fa_prompt_workspace() bytes.
+struct FaPromptArgs {
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const int32_t *cu_q, *cu_k;
+  int B, Tq, Tk, Hq, Hkv, D, causal;
+  float scale;
+  void* out;
+  void* ws;
+};
+size_t fa_prompt_workspace(const FaPromptArgs& a);
+kq_status_t launch_fa_prompt(const FaPromptArgs& a, int dtype, cudaStream_t s);
+// fa_paged.cu: decode over the paged q8_0 cache with a shared prefix
+struct FaPagedArgs {
+  const void* q;  // [B, Hq, D] contiguous, as out
+  const uint8_t *k, *v;
+  int64_t num_pages;
+  int ps;
+  const int32_t* table;
+  int W;
+  const int32_t* seq_lens;
+  int B, Hq, Hkv, D, prefix_len, max_seqlen;
+  float scale;
+  void* out;
+  void* ws;
+};
+size_t fa_paged_workspace(const FaPagedArgs& a);
+kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s);
 
 }  // namespace kq

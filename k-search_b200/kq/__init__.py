@@ -15,3 +15,6 @@ from .ops import (  # noqa: F401
     moe_route, mul_mat_q,
     mul_mat_q8x, quantize_q8_1, quantize_rows, rms_norm, rms_norm_quantize_q8_1,
 )
+from .paged import (  # noqa: F401
+    PagePlan, flash_decode_paged, flash_prompt_ragged, page_plan, page_read, page_write,
+)

@@ -61,6 +61,15 @@ SIGNATURES = {
     "kq_fa_decode_q8_0_mha": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "kq_fa_decode_mha": (_i, [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "kq_fa_decode_q8_0_ragged": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _vp]),
+    "kq_page_plan": (_i, [_vp, _vp, _i, _vp, _i, _vp, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "kq_page_write_q8_0": (_i, [_i, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i, _i, _vp, _vp, _i64, _vp]),
+    "kq_page_read_q8_0": (_i, [_i, _vp, _vp, _i64, _i, _i, _i, _vp, _i, _vp, _i, _i64, _vp, _vp, _vp]),
+    "kq_fa_prompt_workspace": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "kq_fa_prompt": (_i, [_i, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i, _i, _i, _i, _i, _i, _i,
+                          _f, _vp, _vp, _sz, _vp]),
+    "kq_fa_decode_paged_workspace": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "kq_fa_decode_paged": (_i, [_i, _vp, _vp, _vp, _i64, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _vp, _sz,
+                                _vp]),
 }
 
 _lib: ctypes.CDLL | None = None

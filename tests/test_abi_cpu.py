@@ -132,3 +132,35 @@ def test_baseline_lookup_fixups():
     assert harness.baseline_hardware("NVIDIA B200") is None
     assert harness.quant_gemm_baseline_case("block_q4_0", 1, 4096, 14336) == "w4a32c8_q4_0_f32_m4096_n1_k14336"
     assert harness.quant_gemm_baseline_case("block_q8_0", 512, 11008, 4096) == "w8a32c8_q8_0_f32_m11008_n512_k4096"
+
+
+def test_paged_entry_points_refuse_before_any_cuda_call():
+    """Bad arguments of the paged-serving entries are refused on the host; empty calls are no-ops."""
+    from kq import _lib
+    L = _lib.lib()
+    f = ctypes.c_float(1.0)
+    nul = [None] * 8
+
+    def prompt(dtype=0, B=1, Tq=4, Tk=4, Hq=8, Hkv=2, D=128, q=1 << 20, out=1 << 20):
+        return L.kq_fa_prompt(dtype, q, 1 << 20, 1 << 20, 1024, 128, 256, 128, 256, 128, 1 << 20, 1 << 20, B, Tq, Tk, Hq,
+                              Hkv, D, 1, f, out, None, 0, None)
+
+    for bad in ({"dtype": 2}, {"B": -1}, {"Hq": 9}, {"D": 12}, {"D": 264}, {"Hkv": 0}, {"B": 0}, {"q": None}, {"q": 1 << 20 | 1},
+                {"out": 1 << 20 | 2}):
+        assert prompt(**bad) == 1, bad
+    assert prompt(Tq=0) == 0
+
+    def decode(dtype=0, B=2, Hq=8, Hkv=2, D=128, prefix=0, W=4, ps=16, q=1 << 20, kc=1 << 20):
+        return L.kq_fa_decode_paged(dtype, q, kc, 1 << 20, 10, ps, 1 << 20, W, 1 << 20, B, Hq, Hkv, D, prefix, 64, f,
+                                    1 << 20, None, 0, None)
+
+    for bad in ({"dtype": -1}, {"D": 48}, {"Hq": 7}, {"prefix": 65}, {"prefix": -1}, {"ps": 0}, {"q": None}, {"kc": 1 << 20 | 2}):
+        assert decode(**bad) == 1, bad
+    assert decode(B=0) == 0
+    assert L.kq_page_plan(*nul[:2], 1, None, 1, None, 0, 16, 1, *nul[:5], None) == 1
+    assert L.kq_page_plan(*nul[:2], 1, None, 1, None, 0, 0, 1, *nul[:5], None) == 1
+    assert "page_size" in _lib.last_error()
+    assert L.kq_page_write_q8_0(0, None, None, 0, 0, 0, 0, None, 0, 2, 48, None, None, 0, None) == 1
+    assert L.kq_page_write_q8_0(0, None, None, 0, 0, 0, 0, None, 0, 2, 64, None, None, 0, None) == 0
+    assert L.kq_page_read_q8_0(0, None, None, 1, 16, 2, 64, None, 1, None, 0, 5, None, None, None) == 1
+    assert L.kq_page_read_q8_0(0, None, None, 1, 16, 2, 64, None, 1, None, 1, 0, None, None, None) == 0
