@@ -26,6 +26,521 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float
 __device__ __forceinline__ void store_f(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store_f(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// ---- work split ------------------------------------------------------------------
+// Tokens start .. n_b - 1 of every sequence (n_b its length, cut to max_seqlen
+// and the table) are cut into units of 16; a KV head's units of all sequences
+// in a row are divided evenly among C workers, whatever the lengths are.
+// Worker c takes units U c / C .. U (c + 1) / C; the part of it inside
+// sequence b is one segment with its own softmax state, stored at index c + b
+// (unique: c and b only grow along the row).
+constexpr int kUnit = 16;
+constexpr int kCta = 256;
+
+struct Split {
+  const int32_t* seq_lens;
+  int B, start, limit;  // limit: min(max_seqlen, W * ps)
+  int workers;          // upper bound of C
+  __device__ __forceinline__ int len(int b) const { return max(0, min(seq_lens[b], limit)); }
+  __device__ __forceinline__ int units(int b) const { return (max(0, len(b) - start) + kUnit - 1) / kUnit; }
+  // C for U units: at least kMinUnits each
+  __device__ __forceinline__ int active(int U) const { return max(1, min(workers, U / kMinUnits)); }
+  static constexpr int kMinUnits = 2;
+};
+__device__ __forceinline__ int unit_begin(int U, int C, int c) { return (int)((long long)U * c / C); }
+
+// Prefix sums of the units of B sequences, kCta contiguous runs of them (one
+// per thread): scan[i] = units before run i, scan[kCta] = all.
+struct SplitScan {
+  int scan[kCta + 1];
+  int warp_sums[kCta / 32];
+};
+__device__ __forceinline__ int run_len(const Split& sp) { return (sp.B + kCta - 1) / kCta; }
+__device__ __forceinline__ void scan_units(const Split& sp, SplitScan& ss) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = run_len(sp);
+  int v = 0;
+  for (int b = tid * per; b < min(sp.B, (tid + 1) * per); ++b) v += sp.units(b);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += t;
+  }
+  if (lane == 31) ss.warp_sums[warp] = v;
+  __syncthreads();
+  for (int i = 0; i < warp; ++i) v += ss.warp_sums[i];
+  ss.scan[tid + 1] = v;
+  if (tid == 0) ss.scan[0] = 0;
+  __syncthreads();
+}
+// Units before sequence b.
+__device__ __forceinline__ int units_before(const Split& sp, const SplitScan& ss, int b) {
+  const int per = run_len(sp), run = b / per;
+  int u = ss.scan[run];
+  for (int i = run * per; i < b; ++i) u += sp.units(i);
+  return u;
+}
+
+// ---- streaming kernel --------------------------------------------------------------
+// A warp streams one worker's tokens of one KV head (for up to 16 of its query
+// heads): 16-token K and V rows arrive by bulk copies (one row per lane, from
+// the 16-byte boundary below it) in its own ring of stages, so no two warps
+// wait for each other; neighbouring warps hold neighbouring heads of the same
+// tokens. Products on mma.m16n8k16 with the query heads as rows:
+//   S[h, t] = sum_j d_k(t, j) (q_j . codes_j): exact fp16 codes per 32-dim
+//     block j, rescaled in fp32;
+//   O[h, :] += sum_t (p d_v(t, j)) codes: the value block's scale folded into
+//     p in fp32, rounded to fp16 once (the codes are exact), times 2^kPBits so
+//     that small scales stay in fp16's normal range. d_v up to 1023 fits.
+// The head dimension is permuted inside a block so that every operand word is
+// one 32-bit load (a word of 4 codes) per lane.
+constexpr int kStreamWarps = kCta / 32;
+constexpr int kStages = 3;
+constexpr float kPScale = 64.0f;
+
+template <int NB>
+struct Row {
+  static constexpr int BYTES = NB * kQ8;
+  static constexpr int UNITS16 = BYTES & 15;  // heads and tokens move the row start by multiples of this mod 16
+  static constexpr int STEP = UNITS16 == 0 ? 16 : (UNITS16 & 2) ? 2 : (UNITS16 & 4) ? 4 : 8;
+  static constexpr int NEED = (BYTES + 16 - STEP + 15) / 16 * 16;
+  static constexpr int PITCH = (NEED / 16) % 2 ? NEED : NEED + 16;  // odd multiple of 16: 8 rows hit distinct banks
+  static constexpr int STAGE = 2 * kUnit * PITCH;
+  static constexpr int SMEM = kStreamWarps * kStages * STAGE + 16;
+};
+
+struct StreamArgs {
+  const void* q;
+  int q_bf16;
+  const uint8_t *k, *v;
+  long long num_pages;
+  int ps, W, Hq, Hkv, G, QG;  // QG groups of up to 16 query heads per KV head
+  const int32_t* table;
+  int prefix_len;
+  Split split;
+  float sl;     // scale * log2(e)
+  float* part;  // [segment][Hq][NB * 32] accumulators
+  float2* ml;   // [segment][Hq] maximum (log2 units), sum
+  int* err;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// 4 codes (one word) -> two fp16 pairs: 0x64uu is 1024 + uu, uu = code + 128.
+__device__ __forceinline__ void codes_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = w ^ 0x80808080u;
+  lo = hsub2(__byte_perm(u, 0x64646464u, 0x4140), 0x64806480u);
+  hi = hsub2(__byte_perm(u, 0x64646464u, 0x4342), 0x64806480u);
+}
+// The word at byte offset `off` (even) of 4-byte aligned shared memory.
+__device__ __forceinline__ uint32_t word_at(const uint8_t* p, int off) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(p + (off & ~3));
+  return (off & 2) ? __funnelshift_r(w[0], w[1], 16) : w[0];
+}
+__device__ __forceinline__ float scale_at(const uint8_t* p, int off) {
+  return __half2float(*reinterpret_cast<const __half*>(p + off));
+}
+
+// A position in a worker's row of units.
+struct Cursor {
+  int b, tok, n;  // sequence, first token of the tile, the sequence's end
+};
+
+template <int NB, bool WIDE>
+__global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_stream_kernel(const StreamArgs a) {
+  using R = Row<NB>;
+  constexpr int RH = WIDE ? 2 : 1;  // row halves in use: query heads lane / 4 (+ 8)
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ SplitScan ss;
+  __shared__ __align__(8) uint64_t s_bar[kStreamWarps][kStages];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&s_bar[warp][i], 1);
+    fence_mbar_init();
+  }
+  pdl_launch_dependents();
+  scan_units(a.split, ss);
+  const int U = ss.scan[kCta], C = a.split.active(U);
+  const int per_worker = a.Hkv * a.QG;
+  const int gw = blockIdx.x * kStreamWarps + warp;
+  const int wk = gw / per_worker, hw = gw % per_worker, h = hw / a.QG, qg = hw % a.QG;
+  if (wk >= C) return;
+  int u = unit_begin(U, C, wk);
+  const int ue = unit_begin(U, C, wk + 1);
+  if (u >= ue) return;
+
+  uint8_t* ring = smem + warp * kStages * R::STAGE;
+  const long long row_bytes = (long long)a.Hkv * R::BYTES;
+  const int head_off = h * R::BYTES, row15 = (int)(row_bytes & 15);
+
+  // the worker's first tile
+  Cursor f;
+  {
+    int lo = 0, hi = kCta;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (ss.scan[mid] <= u) lo = mid;
+      else hi = mid;
+    }
+    f.b = lo * run_len(a.split);
+    int before = ss.scan[lo], here;
+    while (before + (here = a.split.units(f.b)) <= u) {
+      before += here;
+      ++f.b;
+    }
+    f.n = a.split.len(f.b);
+    f.tok = a.split.start + (u - before) * kUnit;
+  }
+  Cursor cur = f;
+  auto advance = [&](Cursor& x) {  // to the next tile of the row (there is one)
+    x.tok += kUnit;
+    while (x.tok >= x.n) {
+      ++x.b;
+      x.n = a.split.len(x.b);
+      x.tok = a.split.start;
+    }
+  };
+  // the page of this lane's row of tile x (-1: no such token)
+  auto page_of = [&](const Cursor& x) {
+    const int tok = x.tok + (lane & 15);
+    return tok < x.n ? a.table[(long long)(tok < a.prefix_len ? 0 : x.b) * a.W + tok / a.ps] : -1;
+  };
+  // issues the copies of tile x, whose pages are `page`; the lanes with a row
+  auto issue = [&](const Cursor& x, int page, int st) -> uint32_t {
+    const int tok = x.tok + (lane & 15);
+    const bool valid = page >= 0 && page < a.num_pages;
+    const long long at = valid ? ((long long)page * a.ps + tok % a.ps) * row_bytes + head_off : 0;
+    const uint32_t off = (uint32_t)at & 15u;
+    const uint32_t bytes = valid ? (off + R::BYTES + 15u) & ~15u : 0u;
+    const uint32_t mask = __ballot_sync(0xffffffffu, valid);
+    const uint32_t total = __reduce_add_sync(0xffffffffu, bytes);
+    if (lane == 0) mbar_arrive_expect_tx(&s_bar[warp][st], total);
+    __syncwarp();
+    if (valid)
+      bulk_g2s(ring + st * R::STAGE + lane * R::PITCH, (lane < 16 ? a.k : a.v) + (at - off), bytes, &s_bar[warp][st]);
+    return mask & 0xffffu;
+  };
+
+  int left = ue - u;         // tiles not yet consumed
+  int ahead = left;          // tiles not yet issued
+  int page = page_of(f);
+  uint32_t masks[kStages];   // rows present in the tiles in flight, oldest first
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) masks[i] = 0;
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (ahead > 0) {
+      masks[i] = issue(f, page, i);
+      if (--ahead > 0) {
+        advance(f);
+        page = page_of(f);
+      }
+    }
+  }
+
+  bool dead = false;
+  int st = 0;
+  uint32_t phase = 0;
+  while (left > 0) {
+    // ---- a segment: the worker's tiles of sequence cur.b
+    const int b = cur.b;
+    uint32_t qa[2 * NB][2 * RH];
+    float sl[RH];
+#pragma unroll
+    for (int r = 0; r < RH; ++r) {
+      const int hl = qg * 16 + g + 8 * r;  // query head within the KV head's group
+      const bool real = hl < a.G;
+      const uint2* q = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.q) +
+                                                      ((long long)b * a.Hq + h * a.G + (real ? hl : 0)) * (NB * 32));
+      sl[r] = a.sl;
+      uint2 w[2 * NB];
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) w[i] = real ? q[4 * i + c] : make_uint2(0, 0);
+      if (a.q_bf16) {
+        // bf16 -> fp16 after an exact power of two per row that puts the
+        // largest element near 2^14; the factor returns with the scores
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) {
+          top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i].x << 16)), fabsf(__uint_as_float(w[i].x & 0xffff0000u))));
+          top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i].y << 16)), fabsf(__uint_as_float(w[i].y & 0xffff0000u))));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = min(max((int)(__float_as_uint(top) >> 23) - 127 - 14, -100), 100);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        sl[r] *= __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) {
+          w[i].x = pack_h2(__uint_as_float(w[i].x << 16) * down, __uint_as_float(w[i].x & 0xffff0000u) * down);
+          w[i].y = pack_h2(__uint_as_float(w[i].y << 16) * down, __uint_as_float(w[i].y & 0xffff0000u) * down);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) {
+        qa[i][r] = w[i].x;
+        qa[i][RH + r] = w[i].y;
+      }
+    }
+    float acc[NB * 4][2 * RH];
+#pragma unroll
+    for (int i = 0; i < NB * 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 2 * RH; ++r) acc[i][r] = 0.0f;
+    float m[RH], l[RH];
+#pragma unroll
+    for (int r = 0; r < RH; ++r) m[r] = -INFINITY, l[r] = 0.0f;
+
+    int tiles = min(left, (cur.n - cur.tok + kUnit - 1) / kUnit);
+    left -= tiles;
+    int tok = cur.tok;
+    if (left > 0) {
+      cur.tok = cur.n - 1;  // the last tile of this sequence, then the next
+      advance(cur);
+    }
+    for (; tiles > 0; --tiles, tok += kUnit) {
+      // keep the ring full: the stage read in the previous step is free
+      uint32_t fresh = 0;
+      if (ahead > 0) {
+        int s2 = st + kStages - 1;
+        s2 = s2 >= kStages ? s2 - kStages : s2;
+        fresh = issue(f, page, s2);
+        if (--ahead > 0) {
+          advance(f);
+          page = page_of(f);
+        }
+      }
+      const uint32_t mask = masks[0];
+#pragma unroll
+      for (int i = 0; i + 1 < kStages; ++i) masks[i] = masks[i + 1];
+      masks[kStages - 2] = fresh;
+      mbar_wait_or_poison(&s_bar[warp][st], phase, a.err, DEV_TIMEOUT_FULL, dead);
+      __syncwarp();
+      const uint8_t* ks = ring + st * R::STAGE;
+      const uint8_t* vs = ks + kUnit * R::PITCH;
+      // start of a row's blocks within its slot of the stage. Pages hold a
+      // multiple of 8 tokens, so it depends on the token index mod 8 only.
+      auto at = [&](int i) { return i * R::PITCH + ((((tok + i) & 7) * row15 + head_off) & 15); };
+
+      float s[2][2 * RH];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int kr = at(8 * t + g), k0 = at(8 * t + 2 * c), k1 = at(8 * t + 2 * c + 1);
+#pragma unroll
+        for (int r = 0; r < 2 * RH; ++r) s[t][r] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            uint32_t b0, b1;
+            codes_h2(word_at(ks, kr + j * kQ8 + 2 + 16 * x + 4 * c), b0, b1);
+            const uint32_t* q = qa[2 * j + x];
+            mma16816(d, q[0], WIDE ? q[1] : 0u, q[RH], WIDE ? q[2 * RH - 1] : 0u, b0, b1);
+          }
+          const float d0 = scale_at(ks, k0 + j * kQ8), d1 = scale_at(ks, k1 + j * kQ8);
+#pragma unroll
+          for (int r = 0; r < RH; ++r) {
+            s[t][2 * r] = fmaf(d[2 * r], d0, s[t][2 * r]);
+            s[t][2 * r + 1] = fmaf(d[2 * r + 1], d1, s[t][2 * r + 1]);
+          }
+        }
+      }
+      bool on[2][2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) on[t][x] = (mask >> (8 * t + 2 * c + x)) & 1u;
+      float p[2][2 * RH], f_[RH];
+      bool moved = false;
+#pragma unroll
+      for (int r = 0; r < RH; ++r) {
+        float mx = m[r];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            s[t][2 * r + x] = on[t][x] ? s[t][2 * r + x] * sl[r] : -INFINITY;
+            mx = fmaxf(mx, s[t][2 * r + x]);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float base = mx == -INFINITY ? 0.0f : mx;
+        f_[r] = ex2(m[r] - base);
+        moved |= mx != m[r];
+        m[r] = mx;
+        float sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            p[t][2 * r + x] = ex2(s[t][2 * r + x] - base);
+            sum += p[t][2 * r + x];
+          }
+        l[r] = fmaf(l[r], f_[r], sum);
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int i = 0; i < NB * 4; ++i)
+#pragma unroll
+          for (int r = 0; r < 2 * RH; ++r) acc[i][r] *= f_[r >> 1];
+      }
+      int vr[4];
+      bool von[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int ti = 2 * c + (i & 1) + 8 * (i >> 1);
+        vr[i] = at(ti);
+        von[i] = on[i >> 1][i & 1];
+      }
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        float dv[4];
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // an absent row may hold anything: its weight is 0, not 0 x scale
+          dv[i] = von[i] ? scale_at(vs, vr[i] + j * kQ8) * kPScale : 0.0f;
+          w[i] = word_at(vs, vr[i] + j * kQ8 + 2 + 4 * g) ^ 0x80808080u;
+        }
+        uint32_t pa[2 * RH];
+#pragma unroll
+        for (int r = 0; r < RH; ++r) {
+          pa[r] = pack_h2(p[0][2 * r] * dv[0], p[0][2 * r + 1] * dv[1]);
+          pa[RH + r] = pack_h2(p[1][2 * r] * dv[2], p[1][2 * r + 1] * dv[3]);
+        }
+        // byte i of the two tokens of a pair, for the 4 dims of the word
+        const uint32_t x01 = __byte_perm(w[0], w[1], 0x5140), x23 = __byte_perm(w[0], w[1], 0x7362);
+        const uint32_t y01 = __byte_perm(w[2], w[3], 0x5140), y23 = __byte_perm(w[2], w[3], 0x7362);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t sel = (i & 1) ? 0x4342u : 0x4140u;
+          const uint32_t b0 = hsub2(__byte_perm(i < 2 ? x01 : x23, 0x64646464u, sel), 0x64806480u);
+          const uint32_t b1 = hsub2(__byte_perm(i < 2 ? y01 : y23, 0x64646464u, sel), 0x64806480u);
+          float* d = acc[4 * j + i];
+          float t4[4] = {d[0], d[1], WIDE ? d[2 * RH - 2] : 0.0f, WIDE ? d[2 * RH - 1] : 0.0f};
+          mma16816(t4, pa[0], WIDE ? pa[1] : 0u, pa[RH], WIDE ? pa[2 * RH - 1] : 0u, b0, b1);
+          d[0] = t4[0], d[1] = t4[1];
+          if (WIDE) d[2 * RH - 2] = t4[2], d[2 * RH - 1] = t4[3];
+        }
+      }
+      // the stage may be refilled: order these reads before the next copy
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (++st == kStages) st = 0, phase ^= 1;
+    }
+    // ---- the segment's state
+    const long long seg = wk + b;
+#pragma unroll
+    for (int r = 0; r < RH; ++r) {
+      float sum = l[r];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const int hl = qg * 16 + g + 8 * r;
+      if (hl < a.G) {
+        const long long row = seg * a.Hq + h * a.G + hl;
+        float4* o = reinterpret_cast<float4*>(a.part + row * (NB * 32));
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          o[8 * j + 2 * c] = make_float4(acc[4 * j][2 * r], acc[4 * j + 1][2 * r], acc[4 * j + 2][2 * r], acc[4 * j + 3][2 * r]);
+          o[8 * j + 2 * c + 1] = make_float4(acc[4 * j][2 * r + 1], acc[4 * j + 1][2 * r + 1], acc[4 * j + 2][2 * r + 1],
+                                             acc[4 * j + 3][2 * r + 1]);
+        }
+        if (c == 0) a.ml[row] = make_float2(m[r], sum * kPScale);
+      }
+    }
+  }
+}
+
+// ---- combine -------------------------------------------------------------------------
+// One warp per (sequence, query head): the states of its segments, merged with
+// the maximum of their maxima; out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
+struct CombineArgs {
+  Split split;
+  const float* part;
+  const float2* ml;
+  int Hq, D;
+  void* out;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kCta) fa_paged_combine_kernel(const CombineArgs a) {
+  __shared__ SplitScan ss;
+  scan_units(a.split, ss);
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * kStreamWarps + warp;
+  if (row >= (long long)a.split.B * a.Hq) return;
+  const int b = (int)(row / a.Hq), h = (int)(row % a.Hq);
+  const int U = ss.scan[kCta], C = a.split.active(U);
+  const int u0 = units_before(a.split, ss, b), u1 = u0 + a.split.units(b);
+  // workers whose range meets [u0, u1): the last c with begin(c) <= u, for both ends
+  auto worker_of = [&](int u) {
+    int c = (int)((long long)u * C / max(U, 1));
+    while (c + 1 < C && unit_begin(U, C, c + 1) <= u) ++c;
+    while (c > 0 && unit_begin(U, C, c) > u) --c;
+    return c;
+  };
+  const int c0 = u1 > u0 ? worker_of(u0) : 0, n = u1 > u0 ? worker_of(u1 - 1) - c0 + 1 : 0;
+  constexpr int kVec = kMaxNB * 32 / 128;
+  float4 o[kVec];
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float M = -INFINITY, L = 0.0f;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    float2 s = make_float2(-INFINITY, 0.0f);
+    if (i0 + lane < n) s = a.ml[((long long)c0 + b + i0 + lane) * a.Hq + h];
+    const float Mn = fmaxf(M, warp_max(s.x));
+    const float base = Mn == -INFINITY ? 0.0f : Mn;
+    const float f = ex2(M - base), wgt = ex2(s.x - base);
+    float t = wgt * s.y;
+#pragma unroll
+    for (int x = 16; x >= 1; x >>= 1) t += __shfl_xor_sync(0xffffffffu, t, x);
+    L = L * f + t;
+    M = Mn;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) o[i].x *= f, o[i].y *= f, o[i].z *= f, o[i].w *= f;
+    const int cnt = min(32, n - i0);
+#pragma unroll 4
+    for (int k = 0; k < cnt; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, wgt, k);
+      const float4* p = reinterpret_cast<const float4*>(a.part + (((long long)c0 + b + i0 + k) * a.Hq + h) * a.D);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        if (i * 128 + lane * 4 < a.D) {
+          const float4 v = p[i * 32 + lane];
+          o[i].x = fmaf(wk, v.x, o[i].x), o[i].y = fmaf(wk, v.y, o[i].y);
+          o[i].z = fmaf(wk, v.z, o[i].z), o[i].w = fmaf(wk, v.w, o[i].w);
+        }
+    }
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  T* out = static_cast<T*>(a.out) + row * a.D;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i)
+    if (i * 128 + lane * 4 < a.D) {
+      T* p = out + i * 128 + lane * 4;
+      store_f(p, o[i].x * inv), store_f(p + 1, o[i].y * inv), store_f(p + 2, o[i].z * inv), store_f(p + 3, o[i].w * inv);
+    }
+}
+
+// ---- pages of other sizes than a multiple of 8 tokens -----------------------------------
 // One warp per (sequence, query head), 32 tokens per step: a lane per token
 // for q . k, then a lane per dimension for p . v.
 constexpr int kWarps = 4;
@@ -102,16 +617,93 @@ __global__ void __launch_bounds__(kWarps * 32) fa_paged_simple_kernel(const FaPa
     if (t < nb) store_f(out + t * 32 + lane, acc[t] * inv);
 }
 
+// Workers per KV head (and group of 16 of its query heads): two CTAs' warps per SM in all.
+int workers_of(const FaPagedArgs& a) {
+  const int qg = (a.Hq / a.Hkv + 15) / 16;
+  return std::max(1, sm_count() * 2 * kStreamWarps / (a.Hkv * qg));
+}
+struct Workspace {
+  size_t part, ml, total;  // offsets
+};
+Workspace workspace_of(const FaPagedArgs& a) {
+  const size_t rows = ((size_t)workers_of(a) + a.B) * a.Hq;
+  Workspace w;
+  w.part = 0;
+  w.ml = rows * a.D * sizeof(float);
+  w.total = w.ml + rows * sizeof(float2);
+  return w;
+}
+
+template <int NB, bool WIDE>
+kq_status_t launch_stream(const StreamArgs& a, int grid, cudaStream_t s) {
+  auto kernel = fa_paged_stream_kernel<NB, WIDE>;
+  if (kq_status_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), Row<NB>::SMEM, "fa_paged")) return st;
+  kernel<<<grid, kCta, Row<NB>::SMEM, s>>>(a);
+  return check_launch("fa_paged_stream");
+}
+template <int NB>
+kq_status_t launch_stream_nb(const StreamArgs& a, int grid, cudaStream_t s) {
+  return a.G > 8 ? launch_stream<NB, true>(a, grid, s) : launch_stream<NB, false>(a, grid, s);
+}
+
+// Launches `kernel` as a programmatic dependent of the previous kernel on s.
+template <typename... Params, typename Arg>
+kq_status_t launch_pdl(void (*kernel)(Params...), int grid, cudaStream_t s, const Arg& arg, const char* what) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kCta);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, arg), what);
+}
+
 }  // namespace
 
-size_t fa_paged_workspace(const FaPagedArgs&) { return 0; }
+size_t fa_paged_workspace(const FaPagedArgs& a) { return workspace_of(a).total; }
 
 kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s) {
-  const long long items = (long long)a.B * a.Hq;
-  const unsigned grid = (unsigned)((items + kWarps - 1) / kWarps);
-  if (dtype == KQ_F16) fa_paged_simple_kernel<__half><<<grid, kWarps * 32, 0, s>>>(a);
-  else fa_paged_simple_kernel<__nv_bfloat16><<<grid, kWarps * 32, 0, s>>>(a);
-  return check_launch("fa_paged");
+  if (a.ps % 8) {
+    const long long items = (long long)a.B * a.Hq;
+    const unsigned grid = (unsigned)((items + kWarps - 1) / kWarps);
+    if (dtype == KQ_F16) fa_paged_simple_kernel<__half><<<grid, kWarps * 32, 0, s>>>(a);
+    else fa_paged_simple_kernel<__nv_bfloat16><<<grid, kWarps * 32, 0, s>>>(a);
+    return check_launch("fa_paged");
+  }
+  const Workspace w = workspace_of(a);
+  char* ws = static_cast<char*>(a.ws);
+  StreamArgs p{};
+  p.q = a.q, p.q_bf16 = dtype == KQ_BF16;
+  p.k = a.k, p.v = a.v, p.num_pages = a.num_pages;
+  p.ps = a.ps, p.W = a.W, p.Hq = a.Hq, p.Hkv = a.Hkv, p.table = a.table, p.prefix_len = a.prefix_len;
+  p.G = a.Hq / a.Hkv;
+  p.QG = (p.G + 15) / 16;
+  p.split.seq_lens = a.seq_lens, p.split.B = a.B, p.split.start = 0;
+  p.split.limit = (int)std::min<long long>(a.max_seqlen, (long long)a.W * a.ps);
+  p.split.workers = workers_of(a);
+  p.sl = a.scale * 1.44269504088896340736f;
+  p.part = reinterpret_cast<float*>(ws + w.part), p.ml = reinterpret_cast<float2*>(ws + w.ml);
+  p.err = device_error_word();
+  const int grid = (p.split.workers * a.Hkv * p.QG + kStreamWarps - 1) / kStreamWarps;
+  kq_status_t st = KQ_OK;
+  switch (a.D / 32) {
+    case 1: st = launch_stream_nb<1>(p, grid, s); break;
+    case 2: st = launch_stream_nb<2>(p, grid, s); break;
+    case 3: st = launch_stream_nb<3>(p, grid, s); break;
+    case 4: st = launch_stream_nb<4>(p, grid, s); break;
+    case 5: st = launch_stream_nb<5>(p, grid, s); break;
+    case 6: st = launch_stream_nb<6>(p, grid, s); break;
+    case 7: st = launch_stream_nb<7>(p, grid, s); break;
+    default: st = launch_stream_nb<8>(p, grid, s); break;
+  }
+  if (st) return st;
+  CombineArgs ca{p.split, p.part, p.ml, a.Hq, a.D, a.out};
+  const int cgrid = (int)(((long long)a.B * a.Hq + kStreamWarps - 1) / kStreamWarps);
+  return dtype == KQ_F16 ? launch_pdl(fa_paged_combine_kernel<__half>, cgrid, s, ca, "fa_paged_combine")
+                         : launch_pdl(fa_paged_combine_kernel<__nv_bfloat16>, cgrid, s, ca, "fa_paged_combine");
 }
 
 }  // namespace kq
