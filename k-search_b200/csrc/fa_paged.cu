@@ -11,9 +11,11 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "kq_internal.h"
 #include "kq_device.cuh"
+#include "kq_tc.cuh"
 
 namespace kq {
 namespace {
@@ -94,7 +96,7 @@ __device__ __forceinline__ int units_before(const Split& sp, const SplitScan& ss
 // one 32-bit load (a word of 4 codes) per lane.
 constexpr int kStreamWarps = kCta / 32;
 constexpr int kStages = 3;
-constexpr float kPScale = 64.0f;
+constexpr float kPBits = 6.0f, kPScale = 64.0f;
 
 template <int NB>
 struct Row {
@@ -180,10 +182,12 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
   const int per_worker = a.Hkv * a.QG;
   const int gw = blockIdx.x * kStreamWarps + warp;
   const int wk = gw / per_worker, hw = gw % per_worker, h = hw / a.QG, qg = hw % a.QG;
-  if (wk >= C) return;
+  // a programmatic dependent of the prefix kernel, whose results it does not
+  // read: it only may not end before it (the combine waits for this grid)
+  if (wk >= C) return pdl_wait();
   int u = unit_begin(U, C, wk);
   const int ue = unit_begin(U, C, wk + 1);
-  if (u >= ue) return;
+  if (u >= ue) return pdl_wait();
 
   uint8_t* ring = smem + warp * kStages * R::STAGE;
   const long long row_bytes = (long long)a.Hkv * R::BYTES;
@@ -462,10 +466,426 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
           o[8 * j + 2 * c + 1] = make_float4(acc[4 * j][2 * r + 1], acc[4 * j + 1][2 * r + 1], acc[4 * j + 2][2 * r + 1],
                                              acc[4 * j + 3][2 * r + 1]);
         }
-        if (c == 0) a.ml[row] = make_float2(m[r], sum * kPScale);
+        if (c == 0) a.ml[row] = make_float2(m[r] - kPBits, sum * kPScale);  // the sums carry 2^kPBits: as if m were lower
       }
     }
   }
+  pdl_wait();
+}
+
+// ---- shared prefix: one pass of the tensor cores over it for the whole batch -----------
+// The B * G query heads of a KV head are the rows of 128-row tiles; a CTA
+// takes two tiles and a range of 64-token blocks of the prefix, so each block
+// is read and dequantised once for 256 rows. Per block and tile:
+//   S = Q K^T (tcgen05, Q from TMEM), P = 2^(S sl - m + kBias) (a thread per
+//   row), O += P V (tcgen05, P from TMEM)
+// as in the prompt kernel (lazy maximum, two tiles alternating).
+// Operands are fp16. K = d * code has up to 19 significant bits: with fp16
+// queries it enters as an fp16 high part plus the exact remainder (two
+// products into the same accumulator), likewise V, so that P is the only
+// rounded factor. With bf16 queries and outputs (whose own rounding is 8
+// times coarser) the high part alone is used; the queries become fp16 after
+// an exact power of two per row. d above 515 overflows the high part.
+//
+// Warps: 0-3 / 4-7 softmax of tile 0 / 1, 8 MMA issue and TMEM, 9 row copies,
+// 10-17 dequantise (64 tokens x 4 blocks: a block of 32 per thread).
+// 64-token blocks keep S at 64 registers per row, so that 18 warps fit.
+constexpr int kBlk = 64;
+constexpr int kTile = 128;
+constexpr int kPrefixThreads = 576;
+constexpr int kMmaWarp = 8, kCopyWarp = 9, kDeqWarp = 10, kDeqWarps = 8;
+constexpr float kBias = 7.0f, kLazy = 8.0f;
+constexpr int kRaw = 6, kOps = 4;      // raw and operand stages (K and V alternate)
+constexpr int kMasks = 16;             // blocks whose row masks are kept (more than are in flight)
+
+template <int NB, bool LO>
+struct PrefixTraits {
+  static constexpr int DP = NB <= 2 ? 64 : 128;
+  static constexpr int PANELS = DP / 64;
+  static constexpr int PANEL = kBlk * 128;
+  static constexpr int PART = PANELS * PANEL;       // the high (or low) parts of a block
+  static constexpr int OP = PART * (LO ? 2 : 1);
+  static constexpr int RAW = kBlk * Row<NB>::PITCH;
+  static constexpr int OFF_RAW = kOps * OP;
+  static constexpr int OFF_BAR = OFF_RAW + kRaw * RAW;
+  static constexpr int SMEM = OFF_BAR + 512 + 1024;
+  static_assert(SMEM <= 232448, "shared memory budget");
+  static_assert(OFF_RAW % 1024 == 0 && OFF_BAR % 16 == 0, "alignment");
+};
+constexpr uint32_t kColS = 0, kColQ = 128, kColO = 256;  // TMEM: S0 S1 (64 each) | Q0 Q1 (64 each) | O0 O1
+
+struct PrefixArgs {
+  const void* q;
+  int q_bf16;
+  const uint8_t *k, *v;
+  long long num_pages;
+  int ps, B, Hq, Hkv, G, prefix_len, limit, chunks;
+  const int32_t *table, *seq_lens;  // the table's row 0
+  float sl;
+  uint32_t flip;
+  float* part;  // [chunk][B * Hq][NB * 32]
+  float2* ml;
+  int* err;
+};
+
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+// fp16 operands, fp32 D, M = 128; bit 16: B is MN-major (V: dims across, tokens down).
+__host__ __device__ constexpr uint32_t idesc_h(int n, bool b_mn) {
+  return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// V block as B operand: 64-dim panels `panel` bytes apart, 8 tokens per 1024 bytes, SWIZZLE_128B.
+__device__ __forceinline__ uint64_t v_desc(uint32_t saddr, uint32_t panel) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+template <int NB, bool LO>
+__global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(const PrefixArgs a) {
+  using R = PrefixTraits<NB, LO>;
+  constexpr int DP = R::DP;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* raw_full = reinterpret_cast<uint64_t*>(smem + R::OFF_BAR);
+  uint64_t* raw_empty = raw_full + kRaw;
+  uint64_t* op_full = raw_empty + kRaw;
+  uint64_t* op_empty = op_full + kOps;
+  uint64_t* s_full = op_empty + kOps;  // S of a tile is there (and its earlier P V is done)
+  uint64_t* p_full = s_full + 2;       // P of a tile is there, its S is read
+  uint64_t* o_full = p_full + 2;       // the tile's last P V is done
+  uint64_t* q_full = o_full + 2;       // the tiles' queries are in TMEM
+  uint64_t* row_mask = q_full + 1;     // rows present in block j, at j % kMasks
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(row_mask + kMasks);
+  static_assert((2 * kRaw + 2 * kOps + 7 + kMasks) * 8 + 4 <= 512, "barrier area");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_dependents();
+
+  const int chunk = blockIdx.x % a.chunks, hp = blockIdx.x / a.chunks, h = hp % a.Hkv, row0 = hp / a.Hkv * 2 * kTile;
+  const int rows = a.B * a.G;
+  const bool two = row0 + kTile < rows;
+  const int blocks = (a.prefix_len + kBlk - 1) / kBlk;
+  const int j0 = (int)((long long)blocks * chunk / a.chunks), n = (int)((long long)blocks * (chunk + 1) / a.chunks) - j0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRaw; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], kDeqWarps);
+    }
+    for (int i = 0; i < kOps; ++i) {
+      mbar_init(&op_full[i], kDeqWarps);
+      mbar_init(&op_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(q_full, two ? 8 : 4);
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) tc::tmem_alloc(tmem_slot, 512);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const long long row_bytes = (long long)a.Hkv * Row<NB>::BYTES;
+  const int head_off = h * Row<NB>::BYTES, row15 = (int)(row_bytes & 15);
+  bool dead = false;
+
+  if (warp == kCopyWarp) {
+    // ---- raw rows: two per lane, from the 16-byte boundary below them
+    auto pages = [&](int j, int x) {
+      const int tok = (j0 + j) * kBlk + lane + 32 * x;
+      return j < n && tok < a.prefix_len ? a.table[tok / a.ps] : -1;
+    };
+    int page[2] = {pages(0, 0), pages(0, 1)};
+    for (int j = 0; j < n; ++j) {
+      long long at[2];
+      uint32_t bytes[2], mask[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const bool valid = page[x] >= 0 && page[x] < a.num_pages;
+        const int tok = (j0 + j) * kBlk + lane + 32 * x;
+        at[x] = valid ? ((long long)page[x] * a.ps + tok % a.ps) * row_bytes + head_off : 0;
+        bytes[x] = valid ? (((uint32_t)at[x] & 15u) + Row<NB>::BYTES + 15u) & ~15u : 0u;
+        mask[x] = __ballot_sync(0xffffffffu, valid);
+        page[x] = pages(j + 1, x);
+      }
+      const uint32_t total = __reduce_add_sync(0xffffffffu, bytes[0] + bytes[1]);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const int i = 2 * j + kv, st = i % kRaw;
+        if (i >= kRaw) mbar_wait_idle_or_poison(&raw_empty[st], ((i / kRaw) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
+        if (lane == 0) {
+          if (kv == 0) row_mask[j % kMasks] = (uint64_t)mask[1] << 32 | mask[0];
+          mbar_arrive_expect_tx(&raw_full[st], total);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (bytes[x])
+            bulk_g2s(smem + R::OFF_RAW + st * R::RAW + (lane + 32 * x) * Row<NB>::PITCH,
+                     (kv ? a.v : a.k) + (at[x] & ~15ll), bytes[x], &raw_full[st]);
+      }
+    }
+  } else if (warp >= kDeqWarp) {
+    // ---- one block of 32 values per thread: token 8 w + lane % 8, block lane / 8
+    const int tok = (warp - kDeqWarp) * 8 + (lane & 7), blk = lane >> 3;
+    const int off = ((lane & 7) * row15 + head_off & 15) + blk * kQ8;  // blocks start at a multiple of 64 tokens
+    const uint32_t sh = (uint32_t)(off & 2) * 8;
+    const bool used = blk * 32 < DP, real = blk < NB;
+    uint8_t* dst = smem + (blk >> 1) * R::PANEL;
+    for (int i = 0; i < 2 * n; ++i) {
+      const int rs = i % kRaw, os = i % kOps;
+      mbar_wait_or_poison(&raw_full[rs], (i / kRaw) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+      const bool present = real && (row_mask[(i >> 1) % kMasks] >> tok & 1);
+      uint32_t w[9];
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(smem + R::OFF_RAW + rs * R::RAW + tok * Row<NB>::PITCH + (off & ~3));
+#pragma unroll
+      for (int x = 0; x < 9; ++x) w[x] = present && (x < 8 || sh) ? src[x] : 0u;
+      if (present && !sh) w[8] = *reinterpret_cast<const uint16_t*>(src + 8);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_empty[rs]);
+      if (i >= kOps) mbar_wait_or_poison(&op_empty[os], ((i / kOps) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
+      if (used) {
+        // an absent row is zero throughout: whatever its slot held must not meet P = 0
+        const uint32_t d = (w[0] >> sh) & 0xffffu, d2 = present ? d | d << 16 : 0u;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            uint32_t c[2];
+            codes_h2(__funnelshift_rc(w[2 * x + y], w[2 * x + y + 1], sh + 16), c[0], c[1]);
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              hi[2 * y + z] = hmul2(c[z], d2);
+              if (LO) lo[2 * y + z] = hfma2(c[z], d2, hi[2 * y + z] ^ 0x80008000u);
+            }
+          }
+          uint8_t* o = dst + os * R::OP + tc::sw128_off(tok, (blk & 1) * 4 + x);
+          *reinterpret_cast<uint4*>(o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          if (LO) *reinterpret_cast<uint4*>(o + R::PART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&op_full[os]);
+    }
+  } else if (warp == kMmaWarp) {
+    constexpr uint32_t idesc_s = idesc_h(kBlk, false), idesc_o = idesc_h(DP, true);
+    const uint32_t base = smem_u32(smem);
+    const int tiles = two ? 2 : 1;
+    auto score = [&](int t, int j) {
+      const int st = 2 * j % kOps;
+      mbar_wait_or_poison(&op_full[st], (2 * j / kOps) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+      tc::tc_fence_after();
+      if (lane == 0) {
+        const uint64_t kd = tc::sw128_desc(base + st * R::OP);
+#pragma unroll
+        for (int part = 0; part < (LO ? 2 : 1); ++part)
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)
+            mma_ts(tmem + kColS + t * kBlk, tmem + kColQ + t * 64 + 8 * k,
+                   kd + (uint64_t)(part * (R::PART >> 4) + (k >> 2) * (R::PANEL >> 4) + (k & 3) * 2), idesc_s,
+                   (part > 0 || k > 0) ? 1u : 0u);
+        tc::mma_commit(&s_full[t]);
+      }
+      __syncwarp();
+    };
+    mbar_wait_or_poison(q_full, 0, a.err, DEV_TIMEOUT_FULL, dead);
+    tc::tc_fence_after();
+    if (n > 0) {
+      for (int t = 0; t < tiles; ++t) score(t, 0);
+      if (lane == 0) tc::mma_commit(&op_empty[0]);
+    }
+    __syncwarp();
+    for (int j = 0; j < n; ++j) {
+      const int sv = (2 * j + 1) % kOps;
+#pragma unroll 1
+      for (int t = 0; t < tiles; ++t) {
+        mbar_wait_or_poison(&op_full[sv], ((2 * j + 1) / kOps) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        mbar_wait_or_poison(&p_full[t], j & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        tc::tc_fence_after();
+        if (lane == 0) {
+          const uint64_t vd = v_desc(base + sv * R::OP, R::PANEL);
+#pragma unroll
+          for (int part = 0; part < (LO ? 2 : 1); ++part)
+#pragma unroll
+            for (int k = 0; k < kBlk / 16; ++k)
+              mma_ts(tmem + kColO + t * DP, tmem + kColS + t * kBlk + 8 * k,
+                     vd + (uint64_t)(part * (R::PART >> 4) + k * (2048 >> 4)), idesc_o, (j > 0 || part > 0 || k > 0) ? 1u : 0u);
+          if (j + 1 == n) tc::mma_commit(&o_full[t]);
+        }
+        __syncwarp();
+        if (j + 1 < n) score(t, j + 1);
+      }
+      if (lane == 0) {
+        tc::mma_commit(&op_empty[sv]);
+        if (j + 1 < n) tc::mma_commit(&op_empty[(2 * j + 2) % kOps]);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---- softmax, a thread per row
+    const int t = warp >> 2, r = row0 + threadIdx.x, b = r / a.G, gq = r % a.G;
+    if (t == 0 || two) {
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t s_addr = tmem + lanes + kColS + t * kBlk, o_addr = tmem + lanes + kColO + t * DP;
+      const bool mine = r < rows;
+      const int keys = mine ? max(0, min(min(a.seq_lens[b], a.limit), a.prefix_len)) : 0;
+      const long long qrow = (long long)(mine ? b : 0) * a.Hq + h * a.G + (mine ? gq : 0);
+      float sl = a.sl;
+      {
+        // the row's queries to TMEM (two fp16 per column), dims past D zero
+        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + qrow * (NB * 32));
+        float down = 1.0f;
+        if (a.q_bf16 && mine) {
+          float top = 0.0f;
+#pragma unroll 4
+          for (int i = 0; i < NB * 4; ++i) {
+            const uint4 w = q[i];
+            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              top = fmaxf(top, fmaxf(fabsf(__uint_as_float(v[x] << 16)), fabsf(__uint_as_float(v[x] & 0xffff0000u))));
+          }
+          const int e = min(max((int)(__float_as_uint(top) >> 23) - 127 - 14, -100), 100);
+          down = __uint_as_float((uint32_t)(127 - e) << 23);
+          sl *= __uint_as_float((uint32_t)(127 + e) << 23);
+        }
+#pragma unroll 1
+        for (int p = 0; p < R::PANELS; ++p) {
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int at = p * 8 + i;
+            const uint4 v = mine && at < NB * 4 ? q[at] : make_uint4(0, 0, 0, 0);
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+          }
+          if (a.q_bf16) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              w[i] = pack_h2(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down);
+          }
+          __syncwarp();
+          tmem_st32(tmem + lanes + kColQ + t * 64 + p * 32, w);
+        }
+        tc::tmem_st_wait();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+      }
+      float m = -INFINITY, l = 0.0f;
+      for (int j = 0; j < n; ++j) {
+        mbar_wait_or_poison(&s_full[t], j & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        __syncwarp();
+        tc::tc_fence_after();
+        uint32_t s[kBlk];
+        tc::tmem_ld32(s_addr, reinterpret_cast<uint32_t(&)[32]>(s[0]));
+        tc::tmem_ld32(s_addr + 32, reinterpret_cast<uint32_t(&)[32]>(s[32]));
+        tc::tmem_ld_wait();
+        if (a.flip) {
+#pragma unroll
+          for (int i = 0; i < kBlk; ++i) s[i] ^= a.flip;
+        }
+        const int lim = keys - (j0 + j) * kBlk;
+        const uint64_t present = row_mask[j % kMasks];
+        if (__any_sync(0xffffffffu, lim < kBlk) || ~present) {
+#pragma unroll
+          for (int i = 0; i < kBlk; ++i)
+            if (i >= lim || !(present >> i & 1)) s[i] = 0xff800000u;
+        }
+        float mx[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(s[i]);
+#pragma unroll
+        for (int i = 4; i < kBlk; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
+        const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl;
+        float f = 1.0f;
+        if (mn > m + kLazy) {  // also the row's first keys (m = -inf)
+          f = ex2(m - mn);
+          m = mn;
+          l *= f;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
+#pragma unroll 1
+          for (int x = 0; x < DP / 32; ++x) {
+            uint32_t o[32];
+            tc::tmem_ld32(o_addr + 32 * x, o);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st32(o_addr + 32 * x, o);
+          }
+        }
+        const float off = m == -INFINITY ? 0.0f : kBias - m;
+        float sum[2] = {0.0f, 0.0f};
+        uint32_t p[kBlk / 2];
+#pragma unroll
+        for (int i = 0; i < kBlk / 2; ++i) {
+          const float p0 = ex2(fmaf(__uint_as_float(s[2 * i]), sl, off));
+          const float p1 = ex2(fmaf(__uint_as_float(s[2 * i + 1]), sl, off));
+          sum[0] += p0;
+          sum[1] += p1;
+          p[i] = pack_h2(p0, p1);
+        }
+        l += sum[0] + sum[1];
+        __syncwarp();
+        tmem_st32(s_addr, p);
+        tc::tmem_st_wait();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      if (n > 0) mbar_wait_or_poison(&o_full[t], 0, a.err, DEV_TIMEOUT_FULL, dead);
+      __syncwarp();
+      tc::tc_fence_after();
+      const long long at = (long long)chunk * a.B * a.Hq + qrow;
+#pragma unroll 1
+      for (int x = 0; x < DP / 32; ++x) {
+        uint32_t o[32];
+        __syncwarp();
+        tc::tmem_ld32(o_addr + 32 * x, o);
+        tc::tmem_ld_wait();
+        if (mine && x < NB) {
+          uint4* dst = reinterpret_cast<uint4*>(a.part + at * (NB * 32) + 32 * x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            dst[i] = l > 0.0f || l != l ? make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]) : make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (mine) a.ml[at] = make_float2(m - kBias, l);
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
 }
 
 // ---- combine -------------------------------------------------------------------------
@@ -475,6 +895,9 @@ struct CombineArgs {
   Split split;
   const float* part;
   const float2* ml;
+  const float* ppart;  // the prefix chunks' states, [chunk][B * Hq]
+  const float2* pml;
+  int chunks;
   int Hq, D;
   void* out;
 };
@@ -503,9 +926,13 @@ __global__ void __launch_bounds__(kCta) fa_paged_combine_kernel(const CombineArg
 #pragma unroll
   for (int i = 0; i < kVec; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float M = -INFINITY, L = 0.0f;
-  for (int i0 = 0; i0 < n; i0 += 32) {
+  // state i of the row: a prefix chunk, then a segment
+  const long long brows = (long long)a.split.B * a.Hq;
+  const int total = a.chunks + n;
+  auto index = [&](int i) { return i < a.chunks ? i * brows + row : ((long long)c0 + b + i - a.chunks) * a.Hq + h; };
+  for (int i0 = 0; i0 < total; i0 += 32) {
     float2 s = make_float2(-INFINITY, 0.0f);
-    if (i0 + lane < n) s = a.ml[((long long)c0 + b + i0 + lane) * a.Hq + h];
+    if (i0 + lane < total) s = (i0 + lane < a.chunks ? a.pml : a.ml)[index(i0 + lane)];
     const float Mn = fmaxf(M, warp_max(s.x));
     const float base = Mn == -INFINITY ? 0.0f : Mn;
     const float f = ex2(M - base), wgt = ex2(s.x - base);
@@ -516,11 +943,11 @@ __global__ void __launch_bounds__(kCta) fa_paged_combine_kernel(const CombineArg
     M = Mn;
 #pragma unroll
     for (int i = 0; i < kVec; ++i) o[i].x *= f, o[i].y *= f, o[i].z *= f, o[i].w *= f;
-    const int cnt = min(32, n - i0);
+    const int cnt = min(32, total - i0);
 #pragma unroll 4
     for (int k = 0; k < cnt; ++k) {
       const float wk = __shfl_sync(0xffffffffu, wgt, k);
-      const float4* p = reinterpret_cast<const float4*>(a.part + (((long long)c0 + b + i0 + k) * a.Hq + h) * a.D);
+      const float4* p = reinterpret_cast<const float4*>((i0 + k < a.chunks ? a.ppart : a.part) + index(i0 + k) * a.D);
 #pragma unroll
       for (int i = 0; i < kVec; ++i)
         if (i * 128 + lane * 4 < a.D) {
@@ -622,43 +1049,73 @@ int workers_of(const FaPagedArgs& a) {
   const int qg = (a.Hq / a.Hkv + 15) / 16;
   return std::max(1, sm_count() * 2 * kStreamWarps / (a.Hkv * qg));
 }
+// The prefix kernel's pass: head dimensions up to 128, whole groups of 8
+// tokens per page, and a batch (one sequence alone streams its prefix).
+bool use_prefix(const FaPagedArgs& a) { return a.prefix_len > 0 && a.D <= 128 && a.B > 1; }
+// Token chunks of the prefix, so that the grid fills the SMs once.
+int prefix_groups(const FaPagedArgs& a) {  // (KV head, pair of row tiles)
+  const long long rows = (long long)a.B * (a.Hq / a.Hkv);
+  return (int)((rows + 2 * kTile - 1) / (2 * kTile)) * a.Hkv;
+}
+int prefix_chunks(const FaPagedArgs& a) {
+  if (!use_prefix(a)) return 0;
+  const int blocks = (a.prefix_len + kBlk - 1) / kBlk;
+  return std::max(1, std::min(blocks, sm_count() / prefix_groups(a)));
+}
 struct Workspace {
-  size_t part, ml, total;  // offsets
+  size_t part, ml, ppart, pml, total;  // offsets
 };
 Workspace workspace_of(const FaPagedArgs& a) {
-  const size_t rows = ((size_t)workers_of(a) + a.B) * a.Hq;
+  const size_t rows = ((size_t)workers_of(a) + a.B) * a.Hq, prows = (size_t)prefix_chunks(a) * a.B * a.Hq;
   Workspace w;
   w.part = 0;
-  w.ml = rows * a.D * sizeof(float);
-  w.total = w.ml + rows * sizeof(float2);
+  w.ppart = rows * a.D * sizeof(float);
+  w.ml = w.ppart + prows * a.D * sizeof(float);
+  w.pml = w.ml + rows * sizeof(float2);
+  w.total = w.pml + prows * sizeof(float2);
   return w;
 }
 
-template <int NB, bool WIDE>
-kq_status_t launch_stream(const StreamArgs& a, int grid, cudaStream_t s) {
-  auto kernel = fa_paged_stream_kernel<NB, WIDE>;
-  if (kq_status_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), Row<NB>::SMEM, "fa_paged")) return st;
-  kernel<<<grid, kCta, Row<NB>::SMEM, s>>>(a);
-  return check_launch("fa_paged_stream");
+template <int NB, bool LO>
+kq_status_t launch_prefix(const PrefixArgs& a, int grid, cudaStream_t s) {
+  auto kernel = fa_paged_prefix_kernel<NB, LO>;
+  constexpr int smem = PrefixTraits<NB, LO>::SMEM;
+  if (kq_status_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, "fa_paged_prefix")) return st;
+  kernel<<<grid, kPrefixThreads, smem, s>>>(a);
+  return check_launch("fa_paged_prefix");
 }
 template <int NB>
-kq_status_t launch_stream_nb(const StreamArgs& a, int grid, cudaStream_t s) {
-  return a.G > 8 ? launch_stream<NB, true>(a, grid, s) : launch_stream<NB, false>(a, grid, s);
+kq_status_t launch_prefix_nb(const PrefixArgs& a, int grid, cudaStream_t s) {
+  return a.q_bf16 ? launch_prefix<NB, false>(a, grid, s) : launch_prefix<NB, true>(a, grid, s);
 }
 
-// Launches `kernel` as a programmatic dependent of the previous kernel on s.
+// Launches `kernel` as a programmatic dependent of the previous kernel on s
+// (plainly where !pdl).
 template <typename... Params, typename Arg>
-kq_status_t launch_pdl(void (*kernel)(Params...), int grid, cudaStream_t s, const Arg& arg, const char* what) {
+kq_status_t launch_after(void (*kernel)(Params...), int grid, int smem, bool pdl, cudaStream_t s, const Arg& arg,
+                         const char* what) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kCta);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = pdl ? 1 : 0;
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, arg), what);
+}
+
+template <int NB, bool WIDE>
+kq_status_t launch_stream(const StreamArgs& a, int grid, bool pdl, cudaStream_t s) {
+  auto kernel = fa_paged_stream_kernel<NB, WIDE>;
+  if (kq_status_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), Row<NB>::SMEM, "fa_paged")) return st;
+  return launch_after(kernel, grid, Row<NB>::SMEM, pdl, s, a, "fa_paged_stream");
+}
+template <int NB>
+kq_status_t launch_stream_nb(const StreamArgs& a, int grid, bool pdl, cudaStream_t s) {
+  return a.G > 8 ? launch_stream<NB, true>(a, grid, pdl, s) : launch_stream<NB, false>(a, grid, pdl, s);
 }
 
 }  // namespace
@@ -675,35 +1132,57 @@ kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s) {
   }
   const Workspace w = workspace_of(a);
   char* ws = static_cast<char*>(a.ws);
+  const int chunks = prefix_chunks(a);
   StreamArgs p{};
   p.q = a.q, p.q_bf16 = dtype == KQ_BF16;
   p.k = a.k, p.v = a.v, p.num_pages = a.num_pages;
   p.ps = a.ps, p.W = a.W, p.Hq = a.Hq, p.Hkv = a.Hkv, p.table = a.table, p.prefix_len = a.prefix_len;
   p.G = a.Hq / a.Hkv;
   p.QG = (p.G + 15) / 16;
-  p.split.seq_lens = a.seq_lens, p.split.B = a.B, p.split.start = 0;
+  p.split.seq_lens = a.seq_lens, p.split.B = a.B, p.split.start = chunks ? a.prefix_len : 0;
   p.split.limit = (int)std::min<long long>(a.max_seqlen, (long long)a.W * a.ps);
   p.split.workers = workers_of(a);
   p.sl = a.scale * 1.44269504088896340736f;
   p.part = reinterpret_cast<float*>(ws + w.part), p.ml = reinterpret_cast<float2*>(ws + w.ml);
   p.err = device_error_word();
-  const int grid = (p.split.workers * a.Hkv * p.QG + kStreamWarps - 1) / kStreamWarps;
   kq_status_t st = KQ_OK;
+  if (chunks) {
+    PrefixArgs x{};
+    x.q = a.q, x.q_bf16 = p.q_bf16, x.k = a.k, x.v = a.v, x.num_pages = a.num_pages;
+    x.ps = a.ps, x.B = a.B, x.Hq = a.Hq, x.Hkv = a.Hkv, x.G = p.G;
+    x.prefix_len = a.prefix_len, x.limit = p.split.limit, x.chunks = chunks;
+    x.table = a.table, x.seq_lens = a.seq_lens;
+    x.flip = p.sl < 0.0f ? 0x80000000u : 0u;
+    x.sl = fmaxf(fabsf(p.sl), 1e-30f);  // a scale of 0 keeps -inf for hidden keys
+    x.part = reinterpret_cast<float*>(ws + w.ppart), x.ml = reinterpret_cast<float2*>(ws + w.pml);
+    x.err = p.err;
+    const int pgrid = prefix_groups(a) * chunks;
+    switch (a.D / 32) {
+      case 1: st = launch_prefix_nb<1>(x, pgrid, s); break;
+      case 2: st = launch_prefix_nb<2>(x, pgrid, s); break;
+      case 3: st = launch_prefix_nb<3>(x, pgrid, s); break;
+      default: st = launch_prefix_nb<4>(x, pgrid, s); break;
+    }
+    if (st) return st;
+  }
+  const bool pdl = chunks > 0;
+  const int grid = (p.split.workers * a.Hkv * p.QG + kStreamWarps - 1) / kStreamWarps;
   switch (a.D / 32) {
-    case 1: st = launch_stream_nb<1>(p, grid, s); break;
-    case 2: st = launch_stream_nb<2>(p, grid, s); break;
-    case 3: st = launch_stream_nb<3>(p, grid, s); break;
-    case 4: st = launch_stream_nb<4>(p, grid, s); break;
-    case 5: st = launch_stream_nb<5>(p, grid, s); break;
-    case 6: st = launch_stream_nb<6>(p, grid, s); break;
-    case 7: st = launch_stream_nb<7>(p, grid, s); break;
-    default: st = launch_stream_nb<8>(p, grid, s); break;
+    case 1: st = launch_stream_nb<1>(p, grid, pdl, s); break;
+    case 2: st = launch_stream_nb<2>(p, grid, pdl, s); break;
+    case 3: st = launch_stream_nb<3>(p, grid, pdl, s); break;
+    case 4: st = launch_stream_nb<4>(p, grid, pdl, s); break;
+    case 5: st = launch_stream_nb<5>(p, grid, pdl, s); break;
+    case 6: st = launch_stream_nb<6>(p, grid, pdl, s); break;
+    case 7: st = launch_stream_nb<7>(p, grid, pdl, s); break;
+    default: st = launch_stream_nb<8>(p, grid, pdl, s); break;
   }
   if (st) return st;
-  CombineArgs ca{p.split, p.part, p.ml, a.Hq, a.D, a.out};
+  CombineArgs ca{p.split, p.part, p.ml, reinterpret_cast<float*>(ws + w.ppart), reinterpret_cast<float2*>(ws + w.pml),
+                 chunks, a.Hq, a.D, a.out};
   const int cgrid = (int)(((long long)a.B * a.Hq + kStreamWarps - 1) / kStreamWarps);
-  return dtype == KQ_F16 ? launch_pdl(fa_paged_combine_kernel<__half>, cgrid, s, ca, "fa_paged_combine")
-                         : launch_pdl(fa_paged_combine_kernel<__nv_bfloat16>, cgrid, s, ca, "fa_paged_combine");
+  return dtype == KQ_F16 ? launch_after(fa_paged_combine_kernel<__half>, cgrid, 0, true, s, ca, "fa_paged_combine")
+                         : launch_after(fa_paged_combine_kernel<__nv_bfloat16>, cgrid, 0, true, s, ca, "fa_paged_combine");
 }
 
 }  // namespace kq
