@@ -30,7 +30,8 @@ __device__ __forceinline__ void store_f(__nv_bfloat16* p, float v) { *p = __floa
 
 // ---- work split ------------------------------------------------------------------
 // Tokens start .. n_b - 1 of every sequence (n_b its length, cut to max_seqlen
-// and the table) are cut into units of 16; a KV head's units of all sequences
+// and the table) are cut into units of 16 at multiples of 16 (so that 8 rows
+// of a unit are neighbours in one page); a KV head's units of all sequences
 // in a row are divided evenly among C workers, whatever the lengths are.
 // Worker c takes units U c / C .. U (c + 1) / C; the part of it inside
 // sequence b is one segment with its own softmax state, stored at index c + b
@@ -43,7 +44,11 @@ struct Split {
   int B, start, limit;  // limit: min(max_seqlen, W * ps)
   int workers;          // upper bound of C
   __device__ __forceinline__ int len(int b) const { return max(0, min(seq_lens[b], limit)); }
-  __device__ __forceinline__ int units(int b) const { return (max(0, len(b) - start) + kUnit - 1) / kUnit; }
+  __device__ __forceinline__ int first() const { return start & ~(kUnit - 1); }
+  __device__ __forceinline__ int units(int b) const {
+    const int n = len(b);
+    return n > start ? (n - first() + kUnit - 1) / kUnit : 0;
+  }
   // C for U units: at least kMinUnits each
   __device__ __forceinline__ int active(int U) const { return max(1, min(workers, U / kMinUnits)); }
   static constexpr int kMinUnits = 2;
@@ -105,8 +110,44 @@ struct Row {
   static constexpr int STEP = UNITS16 == 0 ? 16 : (UNITS16 & 2) ? 2 : (UNITS16 & 4) ? 4 : 8;
   static constexpr int NEED = (BYTES + 16 - STEP + 15) / 16 * 16;
   static constexpr int PITCH = (NEED / 16) % 2 ? NEED : NEED + 16;  // odd multiple of 16: 8 rows hit distinct banks
+  static constexpr int CHUNKS = NEED / 16;    // 16-byte pieces of a row
+  static constexpr int COPIES = (8 * CHUNKS + 31) / 32;  // per lane, for 8 rows
+  static constexpr bool ALWAYS = 16 * (CHUNKS - 1) < BYTES;  // every piece holds bytes of the row wherever it starts
   static constexpr int STAGE = 2 * kUnit * PITCH;
-  static constexpr int SMEM = kStreamWarps * kStages * STAGE + 16;
+  static constexpr int SMEM = kStreamWarps * kStages * STAGE;
+};
+
+// 16 bytes to shared memory, asynchronously (groups of them are waited for).
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// This lane's pieces of 8 cache rows of one head: rows start at multiples of
+// `row_bytes` from a 16-byte aligned place, plus head_off. The pieces run
+// along the rows, so a warp's copy instruction covers whole row segments.
+template <int NB>
+struct Pieces {
+  using R = Row<NB>;
+  int src[R::COPIES];  // from the first row's start; -1: none
+  int dst[R::COPIES];
+  __device__ __forceinline__ Pieces(int lane, long long row_bytes, int head_off) {
+#pragma unroll
+    for (int i = 0; i < R::COPIES; ++i) {
+      const int x = lane + 32 * i, r = x / R::CHUNKS, c = x % R::CHUNKS;
+      const int at = (int)(r * row_bytes) + head_off, off = at & 15;
+      src[i] = r < 8 && (R::ALWAYS || 16 * c < off + R::BYTES) ? at - off + 16 * c : -1;
+      dst[i] = r * R::PITCH + 16 * c;
+    }
+  }
+  __device__ __forceinline__ void copy(uint32_t to, const uint8_t* from) const {
+#pragma unroll
+    for (int i = 0; i < R::COPIES; ++i)
+      if (src[i] >= 0) copy16(to + dst[i], from + src[i]);
+  }
 };
 
 struct StreamArgs {
@@ -116,12 +157,11 @@ struct StreamArgs {
   long long num_pages;
   int ps, W, Hq, Hkv, G, QG;  // QG groups of up to 16 query heads per KV head
   const int32_t* table;
-  int prefix_len;
+  int prefix_len;  // tokens below it (a multiple of 8) lie in row 0's pages
   Split split;
   float sl;     // scale * log2(e)
   float* part;  // [segment][Hq][NB * 32] accumulators
   float2* ml;   // [segment][Hq] maximum (log2 units), sum
-  int* err;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -170,12 +210,7 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
   constexpr int RH = WIDE ? 2 : 1;  // row halves in use: query heads lane / 4 (+ 8)
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ SplitScan ss;
-  __shared__ __align__(8) uint64_t s_bar[kStreamWarps][kStages];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  if (lane == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(&s_bar[warp][i], 1);
-    fence_mbar_init();
-  }
   pdl_launch_dependents();
   scan_units(a.split, ss);
   const int U = ss.scan[kCta], C = a.split.active(U);
@@ -209,41 +244,48 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
       ++f.b;
     }
     f.n = a.split.len(f.b);
-    f.tok = a.split.start + (u - before) * kUnit;
+    f.tok = a.split.first() + (u - before) * kUnit;
   }
   Cursor cur = f;
   auto advance = [&](Cursor& x) {  // to the next tile of the row (there is one)
     x.tok += kUnit;
-    while (x.tok >= x.n) {
+    while (x.tok >= x.n || x.n <= a.split.start) {
       ++x.b;
       x.n = a.split.len(x.b);
-      x.tok = a.split.start;
+      x.tok = a.split.first();
     }
   };
-  // the page of this lane's row of tile x (-1: no such token)
-  auto page_of = [&](const Cursor& x) {
-    const int tok = x.tok + (lane & 15);
-    return tok < x.n ? a.table[(long long)(tok < a.prefix_len ? 0 : x.b) * a.W + tok / a.ps] : -1;
+  // pages of the two groups of 8 tokens of tile x (-1: no such token)
+  auto pages_of = [&](const Cursor& x) {
+    int2 p = make_int2(-1, -1);
+    const int32_t* t = a.table + (long long)(x.tok < a.prefix_len ? 0 : x.b) * a.W;
+    p.x = t[x.tok / a.ps];
+    if (x.tok + 8 < x.n) p.y = (x.tok + 8 < a.prefix_len ? a.table : a.table + (long long)x.b * a.W)[(x.tok + 8) / a.ps];
+    return p;
   };
-  // issues the copies of tile x, whose pages are `page`; the lanes with a row
-  auto issue = [&](const Cursor& x, int page, int st) -> uint32_t {
-    const int tok = x.tok + (lane & 15);
-    const bool valid = page >= 0 && page < a.num_pages;
-    const long long at = valid ? ((long long)page * a.ps + tok % a.ps) * row_bytes + head_off : 0;
-    const uint32_t off = (uint32_t)at & 15u;
-    const uint32_t bytes = valid ? (off + R::BYTES + 15u) & ~15u : 0u;
-    const uint32_t mask = __ballot_sync(0xffffffffu, valid);
-    const uint32_t total = __reduce_add_sync(0xffffffffu, bytes);
-    if (lane == 0) mbar_arrive_expect_tx(&s_bar[warp][st], total);
-    __syncwarp();
-    if (valid)
-      bulk_g2s(ring + st * R::STAGE + lane * R::PITCH, (lane < 16 ? a.k : a.v) + (at - off), bytes, &s_bar[warp][st]);
-    return mask & 0xffffu;
+  const Pieces<NB> pieces(lane, row_bytes, head_off);
+  const uint32_t ring32 = smem_u32(ring);
+  // issues the copies of tile x, whose pages are p; returns the rows present
+  auto issue = [&](const Cursor& x, int2 p, int st) -> uint32_t {
+    uint32_t mask = 0;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int page = half ? p.y : p.x, tok = x.tok + 8 * half;
+      if (page >= 0 && page < a.num_pages) {
+        const long long at = ((long long)page * a.ps + tok % a.ps) * row_bytes;
+        const uint32_t to = ring32 + st * R::STAGE + half * 8 * R::PITCH;
+        pieces.copy(to, a.k + at);
+        pieces.copy(to + kUnit * R::PITCH, a.v + at);
+        const int lo = max(0, a.split.start - tok), hi = min(8, x.n - tok);  // tokens of the group in use
+        if (hi > lo) mask |= ((1u << hi) - (1u << min(lo, 8))) << (8 * half);
+      }
+    }
+    return mask;
   };
 
   int left = ue - u;         // tiles not yet consumed
   int ahead = left;          // tiles not yet issued
-  int page = page_of(f);
+  int2 page = pages_of(f);
   uint32_t masks[kStages];   // rows present in the tiles in flight, oldest first
 #pragma unroll
   for (int i = 0; i < kStages; ++i) masks[i] = 0;
@@ -253,14 +295,13 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
       masks[i] = issue(f, page, i);
       if (--ahead > 0) {
         advance(f);
-        page = page_of(f);
+        page = pages_of(f);
       }
     }
+    copy_commit();
   }
 
-  bool dead = false;
   int st = 0;
-  uint32_t phase = 0;
   while (left > 0) {
     // ---- a segment: the worker's tiles of sequence cur.b
     const int b = cur.b;
@@ -327,20 +368,20 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
         fresh = issue(f, page, s2);
         if (--ahead > 0) {
           advance(f);
-          page = page_of(f);
+          page = pages_of(f);
         }
       }
+      copy_commit();
       const uint32_t mask = masks[0];
 #pragma unroll
       for (int i = 0; i + 1 < kStages; ++i) masks[i] = masks[i + 1];
       masks[kStages - 2] = fresh;
-      mbar_wait_or_poison(&s_bar[warp][st], phase, a.err, DEV_TIMEOUT_FULL, dead);
+      copy_wait<kStages - 1>();
       __syncwarp();
       const uint8_t* ks = ring + st * R::STAGE;
       const uint8_t* vs = ks + kUnit * R::PITCH;
-      // start of a row's blocks within its slot of the stage. Pages hold a
-      // multiple of 8 tokens, so it depends on the token index mod 8 only.
-      auto at = [&](int i) { return i * R::PITCH + ((((tok + i) & 7) * row15 + head_off) & 15); };
+      // start of a row's blocks within its slot of the stage
+      auto at = [&](int i) { return i * R::PITCH + (((i & 7) * row15 + head_off) & 15); };
 
       float s[2][2 * RH];
 #pragma unroll
@@ -444,10 +485,8 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
           if (WIDE) d[2 * RH - 2] = t4[2], d[2 * RH - 1] = t4[3];
         }
       }
-      // the stage may be refilled: order these reads before the next copy
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (++st == kStages) st = 0, phase ^= 1;
+      __syncwarp();  // the stage may be refilled
+      if (++st == kStages) st = 0;
     }
     // ---- the segment's state
     const long long seg = wk + b;
@@ -487,13 +526,14 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
 // times coarser) the high part alone is used; the queries become fp16 after
 // an exact power of two per row. d above 515 overflows the high part.
 //
-// Warps: 0-3 / 4-7 softmax of tile 0 / 1, 8 MMA issue and TMEM, 9 row copies,
-// 10-17 dequantise (64 tokens x 4 blocks: a block of 32 per thread).
-// 64-token blocks keep S at 64 registers per row, so that 18 warps fit.
+// Warps: 0-3 / 4-7 softmax of tile 0 / 1, 8 MMA issue and TMEM, 9-16 copy and
+// dequantise 8 tokens of each block (a block of 32 values per thread), each
+// from its own ring of rows. 64-token blocks keep S at 64 registers per row,
+// so that 17 warps fit.
 constexpr int kBlk = 64;
 constexpr int kTile = 128;
-constexpr int kPrefixThreads = 576;
-constexpr int kMmaWarp = 8, kCopyWarp = 9, kDeqWarp = 10, kDeqWarps = 8;
+constexpr int kPrefixThreads = 544;
+constexpr int kMmaWarp = 8, kDeqWarp = 9, kDeqWarps = 8;
 constexpr float kBias = 7.0f, kLazy = 8.0f;
 constexpr int kRaw = 6, kOps = 4;      // raw and operand stages (K and V alternate)
 constexpr int kMasks = 16;             // blocks whose row masks are kept (more than are in flight)
@@ -570,9 +610,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
   constexpr int DP = R::DP;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* raw_full = reinterpret_cast<uint64_t*>(smem + R::OFF_BAR);
-  uint64_t* raw_empty = raw_full + kRaw;
-  uint64_t* op_full = raw_empty + kRaw;
+  uint64_t* op_full = reinterpret_cast<uint64_t*>(smem + R::OFF_BAR);
   uint64_t* op_empty = op_full + kOps;
   uint64_t* s_full = op_empty + kOps;  // S of a tile is there (and its earlier P V is done)
   uint64_t* p_full = s_full + 2;       // P of a tile is there, its S is read
@@ -580,7 +618,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
   uint64_t* q_full = o_full + 2;       // the tiles' queries are in TMEM
   uint64_t* row_mask = q_full + 1;     // rows present in block j, at j % kMasks
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(row_mask + kMasks);
-  static_assert((2 * kRaw + 2 * kOps + 7 + kMasks) * 8 + 4 <= 512, "barrier area");
+  static_assert((2 * kOps + 7 + kMasks) * 8 + 4 <= 512, "barrier area");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
 
@@ -591,10 +629,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
   const int j0 = (int)((long long)blocks * chunk / a.chunks), n = (int)((long long)blocks * (chunk + 1) / a.chunks) - j0;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kRaw; ++i) {
-      mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], kDeqWarps);
-    }
     for (int i = 0; i < kOps; ++i) {
       mbar_init(&op_full[i], kDeqWarps);
       mbar_init(&op_empty[i], 1);
@@ -616,61 +650,70 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
   const int head_off = h * Row<NB>::BYTES, row15 = (int)(row_bytes & 15);
   bool dead = false;
 
-  if (warp == kCopyWarp) {
-    // ---- raw rows: two per lane, from the 16-byte boundary below them
-    auto pages = [&](int j, int x) {
-      const int tok = (j0 + j) * kBlk + lane + 32 * x;
-      return j < n && tok < a.prefix_len ? a.table[tok / a.ps] : -1;
-    };
-    int page[2] = {pages(0, 0), pages(0, 1)};
-    for (int j = 0; j < n; ++j) {
-      long long at[2];
-      uint32_t bytes[2], mask[2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const bool valid = page[x] >= 0 && page[x] < a.num_pages;
-        const int tok = (j0 + j) * kBlk + lane + 32 * x;
-        at[x] = valid ? ((long long)page[x] * a.ps + tok % a.ps) * row_bytes + head_off : 0;
-        bytes[x] = valid ? (((uint32_t)at[x] & 15u) + Row<NB>::BYTES + 15u) & ~15u : 0u;
-        mask[x] = __ballot_sync(0xffffffffu, valid);
-        page[x] = pages(j + 1, x);
-      }
-      const uint32_t total = __reduce_add_sync(0xffffffffu, bytes[0] + bytes[1]);
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const int i = 2 * j + kv, st = i % kRaw;
-        if (i >= kRaw) mbar_wait_idle_or_poison(&raw_empty[st], ((i / kRaw) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
-        if (lane == 0) {
-          if (kv == 0) row_mask[j % kMasks] = (uint64_t)mask[1] << 32 | mask[0];
-          mbar_arrive_expect_tx(&raw_full[st], total);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (bytes[x])
-            bulk_g2s(smem + R::OFF_RAW + st * R::RAW + (lane + 32 * x) * Row<NB>::PITCH,
-                     (kv ? a.v : a.k) + (at[x] & ~15ll), bytes[x], &raw_full[st]);
-      }
-    }
-  } else if (warp >= kDeqWarp) {
+  if (warp >= kDeqWarp) {
     // ---- one block of 32 values per thread: token 8 w + lane % 8, block lane / 8
-    const int tok = (warp - kDeqWarp) * 8 + (lane & 7), blk = lane >> 3;
-    const int off = ((lane & 7) * row15 + head_off & 15) + blk * kQ8;  // blocks start at a multiple of 64 tokens
+    const int dw = warp - kDeqWarp, tok = dw * 8 + (lane & 7), blk = lane >> 3;
+    const int off = (((lane & 7) * row15 + head_off) & 15) + blk * kQ8;
     const uint32_t sh = (uint32_t)(off & 2) * 8;
     const bool used = blk * 32 < DP, real = blk < NB;
     uint8_t* dst = smem + (blk >> 1) * R::PANEL;
+    uint8_t* ring = smem + R::OFF_RAW + dw * kRaw * 8 * Row<NB>::PITCH;
+    const uint32_t ring32 = smem_u32(ring);
+    const Pieces<NB> pieces(lane, row_bytes, head_off);
+    // 8 tokens of a block lie in one page (pages hold a multiple of 8)
+    auto page_of = [&](int j) {
+      const int t = (j0 + j) * kBlk + dw * 8;
+      return j < n && t < a.prefix_len ? a.table[t / a.ps] : -1;
+    };
+    auto rows_of = [&](int j, int page) {
+      const int left = a.prefix_len - ((j0 + j) * kBlk + dw * 8);
+      return page >= 0 && page < a.num_pages ? (left >= 8 ? 0xffu : (1u << max(left, 0)) - 1u) : 0u;
+    };
+    int page = page_of(0);
+    uint32_t rows_at[kRaw / 2];  // rows of the blocks in flight, oldest first
+    // copies of block j: K into ring stage (2 j) % kRaw, V into the next
+    auto issue = [&](int j) -> uint32_t {
+      const uint32_t present = j < n ? rows_of(j, page) : 0u;
+      if (present) {
+        const int t = (j0 + j) * kBlk + dw * 8;
+        const long long at = ((long long)page * a.ps + t % a.ps) * row_bytes;
+        const uint32_t to = ring32 + (2 * j % kRaw) * 8 * Row<NB>::PITCH;
+        pieces.copy(to, a.k + at);
+        copy_commit();
+        pieces.copy(to + 8 * Row<NB>::PITCH, a.v + at);
+        copy_commit();
+      } else {
+        copy_commit();
+        copy_commit();
+      }
+      page = page_of(j + 1);
+      return present;
+    };
+#pragma unroll
+    for (int i = 0; i < kRaw / 2; ++i) rows_at[i] = 0;
+#pragma unroll
+    for (int i = 0; i < kRaw / 2 - 1; ++i) rows_at[i] = issue(i);
     for (int i = 0; i < 2 * n; ++i) {
-      const int rs = i % kRaw, os = i % kOps;
-      mbar_wait_or_poison(&raw_full[rs], (i / kRaw) & 1, a.err, DEV_TIMEOUT_FULL, dead);
-      const bool present = real && (row_mask[(i >> 1) % kMasks] >> tok & 1);
+      const int rs = i % kRaw, os = i % kOps, j = i >> 1;
+      if ((i & 1) == 0) {
+        rows_at[kRaw / 2 - 1] = issue(j + kRaw / 2 - 1);
+        if (lane == 0) reinterpret_cast<uint8_t*>(&row_mask[j % kMasks])[dw] = (uint8_t)rows_at[0];
+      }
+      // groups after item i: V of its block (for K), and kRaw / 2 - 1 blocks
+      if (i & 1) copy_wait<kRaw - 2>();
+      else copy_wait<kRaw - 1>();
+      __syncwarp();
+      const bool present = real && (rows_at[0] >> (lane & 7) & 1);
       uint32_t w[9];
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(smem + R::OFF_RAW + rs * R::RAW + tok * Row<NB>::PITCH + (off & ~3));
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(ring + (rs * 8 + (lane & 7)) * Row<NB>::PITCH + (off & ~3));
 #pragma unroll
       for (int x = 0; x < 9; ++x) w[x] = present && (x < 8 || sh) ? src[x] : 0u;
       if (present && !sh) w[8] = *reinterpret_cast<const uint16_t*>(src + 8);
-      fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&raw_empty[rs]);
+      if (i & 1) {
+#pragma unroll
+        for (int x = 0; x + 1 < kRaw / 2; ++x) rows_at[x] = rows_at[x + 1];
+      }
       if (i >= kOps) mbar_wait_or_poison(&op_empty[os], ((i / kOps) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
       if (used) {
         // an absent row is zero throughout: whatever its slot held must not meet P = 0
@@ -967,7 +1010,8 @@ __global__ void __launch_bounds__(kCta) fa_paged_combine_kernel(const CombineArg
     }
 }
 
-// ---- pages of other sizes than a multiple of 8 tokens -----------------------------------
+// ---- pages of other sizes than a multiple of 8 tokens, or a prefix that ends within 8
+// tokens where the prefix kernel does not run (D > 128) ------------------------------------
 // One warp per (sequence, query head), 32 tokens per step: a lane per token
 // for q . k, then a lane per dimension for p . v.
 constexpr int kWarps = 4;
@@ -1123,7 +1167,10 @@ kq_status_t launch_stream_nb(const StreamArgs& a, int grid, bool pdl, cudaStream
 size_t fa_paged_workspace(const FaPagedArgs& a) { return workspace_of(a).total; }
 
 kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s) {
-  if (a.ps % 8) {
+  const int chunks = prefix_chunks(a);
+  // streamed through row 0's table: B > 1 without the prefix kernel
+  const int through0 = chunks == 0 && a.B > 1 ? a.prefix_len : 0;
+  if (a.ps % 8 || through0 % 8) {
     const long long items = (long long)a.B * a.Hq;
     const unsigned grid = (unsigned)((items + kWarps - 1) / kWarps);
     if (dtype == KQ_F16) fa_paged_simple_kernel<__half><<<grid, kWarps * 32, 0, s>>>(a);
@@ -1132,11 +1179,10 @@ kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s) {
   }
   const Workspace w = workspace_of(a);
   char* ws = static_cast<char*>(a.ws);
-  const int chunks = prefix_chunks(a);
   StreamArgs p{};
   p.q = a.q, p.q_bf16 = dtype == KQ_BF16;
   p.k = a.k, p.v = a.v, p.num_pages = a.num_pages;
-  p.ps = a.ps, p.W = a.W, p.Hq = a.Hq, p.Hkv = a.Hkv, p.table = a.table, p.prefix_len = a.prefix_len;
+  p.ps = a.ps, p.W = a.W, p.Hq = a.Hq, p.Hkv = a.Hkv, p.table = a.table, p.prefix_len = through0;
   p.G = a.Hq / a.Hkv;
   p.QG = (p.G + 15) / 16;
   p.split.seq_lens = a.seq_lens, p.split.B = a.B, p.split.start = chunks ? a.prefix_len : 0;
@@ -1144,7 +1190,6 @@ kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s) {
   p.split.workers = workers_of(a);
   p.sl = a.scale * 1.44269504088896340736f;
   p.part = reinterpret_cast<float*>(ws + w.part), p.ml = reinterpret_cast<float2*>(ws + w.ml);
-  p.err = device_error_word();
   kq_status_t st = KQ_OK;
   if (chunks) {
     PrefixArgs x{};
@@ -1155,7 +1200,7 @@ kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s) {
     x.flip = p.sl < 0.0f ? 0x80000000u : 0u;
     x.sl = fmaxf(fabsf(p.sl), 1e-30f);  // a scale of 0 keeps -inf for hidden keys
     x.part = reinterpret_cast<float*>(ws + w.ppart), x.ml = reinterpret_cast<float2*>(ws + w.pml);
-    x.err = p.err;
+    x.err = device_error_word();
     const int pgrid = prefix_groups(a) * chunks;
     switch (a.D / 32) {
       case 1: st = launch_prefix_nb<1>(x, pgrid, s); break;

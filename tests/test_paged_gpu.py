@@ -337,7 +337,7 @@ def paged_case(g, lens, prefix, ps, hkv, d, spare=3, one_table=False):
     return random_cache(g, pages, ps, hkv, d), random_cache(g, pages, ps, hkv, d), table
 
 
-def decode_ref(q, kc, vc, table, lens, scale):
+def decode_ref(q, kc, vc, table, lens, scale, prefix=0):
     B, Hq, D = q.shape
     ps, hkv = kc.shape[1], kc.shape[2]
     g = Hq // hkv
@@ -347,6 +347,9 @@ def decode_ref(q, kc, vc, table, lens, scale):
             continue
         pages = table[b, :-(-n // ps)].long()
         k, v = (values(c[pages]).flatten(0, 1)[:n] for c in (kc, vc))
+        if prefix:
+            first = table[0, :-(-prefix // ps)].long()
+            k, v = (torch.cat([values(c[first]).flatten(0, 1)[:min(n, prefix)], x[prefix:]]) for c, x in ((kc, k), (vc, v)))
         seen = torch.ones((g, n), dtype=torch.bool, device="cuda")
         seen &= (pages >= 0).repeat_interleave(ps)[:n]
         for h in range(hkv):
@@ -381,6 +384,24 @@ def test_decode(cuda, dtype, lens, prefix, ps, Hq, Hkv, D):
     for bound in (None, max(lens)):
         got = kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix, max_seqlen=bound)
         check_out(got, ref, spread, top, dtype, f"max_seqlen={bound}")
+
+
+@pytest.mark.parametrize("D,ps", [(128, 16), (64, 8), (256, 16), (96, 24), (32, 5)])
+@pytest.mark.parametrize("prefix", [40, 43, 200])
+def test_decode_copied_last_page(cuda, D, ps, prefix):
+    """A prefix that ends inside a page: every sequence holds its own copy of that page, and only the
+    first sequence's copy has the prefix's tokens (the others' are NaN there)."""
+    import kq
+    g = gen(prefix + D)
+    lens = [prefix + n for n in (30, 7, 100, 1, 55)]
+    kc, vc, table = paged_case(g, lens, prefix - prefix % ps, ps, 2, D)
+    nan = torch.tensor([float("nan")], dtype=torch.float16, device=cuda).view(torch.uint8)
+    for b in range(1, len(lens)):
+        for c in (kc, vc):
+            c[table[b, prefix // ps].item(), :prefix % ps, ..., :2] = nan
+    q = rows(g, len(lens), 8, D, torch.float16)
+    ref, spread, top = decode_ref(q, kc, vc, table, lens, D ** -0.5, prefix)
+    check_out(kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix), ref, spread, top, torch.float16)
 
 
 @pytest.mark.parametrize("prefix", [0, 128])
