@@ -578,32 +578,10 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
 // fp16 operands, fp32 D, M = 128; bit 16: B is MN-major (V: dims across, tokens down).
 __host__ __device__ constexpr uint32_t idesc_h(int n, bool b_mn) {
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-// V block as B operand: 64-dim panels `panel` bytes apart, 8 tokens per 1024 bytes, SWIZZLE_128B.
-__device__ __forceinline__ uint64_t v_desc(uint32_t saddr, uint32_t panel) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-
 template <int NB, bool LO>
 __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(const PrefixArgs a) {
   using R = PrefixTraits<NB, LO>;
@@ -693,31 +671,41 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
     for (int i = 0; i < kRaw / 2; ++i) rows_at[i] = 0;
 #pragma unroll
     for (int i = 0; i < kRaw / 2 - 1; ++i) rows_at[i] = issue(i);
-    for (int i = 0; i < 2 * n; ++i) {
-      const int rs = i % kRaw, os = i % kOps, j = i >> 1;
+    // the words of item i (K or V of block i / 2), once its copies are there:
+    // 9 that cover the thread's block of 34 bytes; 0 for an absent row, since
+    // whatever its slot holds must not meet P = 0
+    auto load = [&](int i, uint32_t (&w)[9]) {
+      const int rs = i % kRaw, j = i >> 1;
       if ((i & 1) == 0) {
+        if (i > 0) {
+#pragma unroll
+          for (int x = 0; x + 1 < kRaw / 2; ++x) rows_at[x] = rows_at[x + 1];
+        }
         rows_at[kRaw / 2 - 1] = issue(j + kRaw / 2 - 1);
         if (lane == 0) reinterpret_cast<uint8_t*>(&row_mask[j % kMasks])[dw] = (uint8_t)rows_at[0];
+        copy_wait<kRaw - 1>();  // later groups: V of this block, and kRaw / 2 - 1 blocks
+      } else {
+        copy_wait<kRaw - 2>();
       }
-      // groups after item i: V of its block (for K), and kRaw / 2 - 1 blocks
-      if (i & 1) copy_wait<kRaw - 2>();
-      else copy_wait<kRaw - 1>();
       __syncwarp();
       const bool present = real && (rows_at[0] >> (lane & 7) & 1);
-      uint32_t w[9];
       const uint32_t* src = reinterpret_cast<const uint32_t*>(ring + (rs * 8 + (lane & 7)) * Row<NB>::PITCH + (off & ~3));
 #pragma unroll
-      for (int x = 0; x < 9; ++x) w[x] = present && (x < 8 || sh) ? src[x] : 0u;
-      if (present && !sh) w[8] = *reinterpret_cast<const uint16_t*>(src + 8);
+      for (int x = 0; x < 8; ++x) w[x] = present ? src[x] : 0u;
+      w[8] = !present ? 0u : sh ? src[8] : *reinterpret_cast<const uint16_t*>(src + 8);
       __syncwarp();
-      if (i & 1) {
+    };
+    uint32_t next[9];
+    if (n > 0) load(0, next);
+    for (int i = 0; i < 2 * n; ++i) {
+      const int os = i % kOps;
+      uint32_t w[9];
 #pragma unroll
-        for (int x = 0; x + 1 < kRaw / 2; ++x) rows_at[x] = rows_at[x + 1];
-      }
+      for (int x = 0; x < 9; ++x) w[x] = next[x];
+      if (i + 1 < 2 * n) load(i + 1, next);
       if (i >= kOps) mbar_wait_or_poison(&op_empty[os], ((i / kOps) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
       if (used) {
-        // an absent row is zero throughout: whatever its slot held must not meet P = 0
-        const uint32_t d = (w[0] >> sh) & 0xffffu, d2 = present ? d | d << 16 : 0u;
+        const uint32_t d = (w[0] >> sh) & 0xffffu, d2 = d | d << 16;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           uint32_t hi[4], lo[4];
@@ -742,32 +730,28 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
     }
   } else if (warp == kMmaWarp) {
     constexpr uint32_t idesc_s = idesc_h(kBlk, false), idesc_o = idesc_h(DP, true);
-    const uint32_t base = smem_u32(smem);
+    const uint32_t base = smem_u32(smem), go = tc::elect_one();
     const int tiles = two ? 2 : 1;
     auto score = [&](int t, int j) {
       const int st = 2 * j % kOps;
       mbar_wait_or_poison(&op_full[st], (2 * j / kOps) & 1, a.err, DEV_TIMEOUT_FULL, dead);
       tc::tc_fence_after();
-      if (lane == 0) {
-        const uint64_t kd = tc::sw128_desc(base + st * R::OP);
+      const uint64_t kd = tc::sw128_desc(base + st * R::OP);
 #pragma unroll
-        for (int part = 0; part < (LO ? 2 : 1); ++part)
+      for (int part = 0; part < (LO ? 2 : 1); ++part)
 #pragma unroll
-          for (int k = 0; k < DP / 16; ++k)
-            mma_ts(tmem + kColS + t * kBlk, tmem + kColQ + t * 64 + 8 * k,
-                   kd + (uint64_t)(part * (R::PART >> 4) + (k >> 2) * (R::PANEL >> 4) + (k & 3) * 2), idesc_s,
-                   (part > 0 || k > 0) ? 1u : 0u);
-        tc::mma_commit(&s_full[t]);
-      }
-      __syncwarp();
+        for (int k = 0; k < DP / 16; ++k)
+          tc::mma_ts_go(tmem + kColS + t * kBlk, tmem + kColQ + t * 64 + 8 * k,
+                        kd + (uint64_t)(part * (R::PART >> 4) + (k >> 2) * (R::PANEL >> 4) + (k & 3) * 2), idesc_s,
+                        (part > 0 || k > 0) ? 1u : 0u, go);
+      tc::mma_commit_go(&s_full[t], go);
     };
     mbar_wait_or_poison(q_full, 0, a.err, DEV_TIMEOUT_FULL, dead);
     tc::tc_fence_after();
     if (n > 0) {
       for (int t = 0; t < tiles; ++t) score(t, 0);
-      if (lane == 0) tc::mma_commit(&op_empty[0]);
+      tc::mma_commit_go(&op_empty[0], go);
     }
-    __syncwarp();
     for (int j = 0; j < n; ++j) {
       const int sv = (2 * j + 1) % kOps;
 #pragma unroll 1
@@ -775,25 +759,21 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
         mbar_wait_or_poison(&op_full[sv], ((2 * j + 1) / kOps) & 1, a.err, DEV_TIMEOUT_FULL, dead);
         mbar_wait_or_poison(&p_full[t], j & 1, a.err, DEV_TIMEOUT_FULL, dead);
         tc::tc_fence_after();
-        if (lane == 0) {
-          const uint64_t vd = v_desc(base + sv * R::OP, R::PANEL);
+        const uint64_t vd = tc::sw128_desc_mn(base + sv * R::OP, R::PANEL);  // dims across, tokens down
 #pragma unroll
-          for (int part = 0; part < (LO ? 2 : 1); ++part)
+        for (int part = 0; part < (LO ? 2 : 1); ++part)
 #pragma unroll
-            for (int k = 0; k < kBlk / 16; ++k)
-              mma_ts(tmem + kColO + t * DP, tmem + kColS + t * kBlk + 8 * k,
-                     vd + (uint64_t)(part * (R::PART >> 4) + k * (2048 >> 4)), idesc_o, (j > 0 || part > 0 || k > 0) ? 1u : 0u);
-          if (j + 1 == n) tc::mma_commit(&o_full[t]);
-        }
-        __syncwarp();
+          for (int k = 0; k < kBlk / 16; ++k)
+            tc::mma_ts_go(tmem + kColO + t * DP, tmem + kColS + t * kBlk + 8 * k,
+                          vd + (uint64_t)(part * (R::PART >> 4) + k * (2048 >> 4)), idesc_o,
+                          (j > 0 || part > 0 || k > 0) ? 1u : 0u, go);
+        if (j + 1 == n) tc::mma_commit_go(&o_full[t], go);
         if (j + 1 < n) score(t, j + 1);
       }
-      if (lane == 0) {
-        tc::mma_commit(&op_empty[sv]);
-        if (j + 1 < n) tc::mma_commit(&op_empty[(2 * j + 2) % kOps]);
-      }
-      __syncwarp();
+      tc::mma_commit_go(&op_empty[sv], go);
+      if (j + 1 < n) tc::mma_commit_go(&op_empty[(2 * j + 2) % kOps], go);
     }
+    __syncwarp();
   } else {
     // ---- softmax, a thread per row
     const int t = warp >> 2, r = row0 + threadIdx.x, b = r / a.G, gq = r % a.G;
@@ -837,7 +817,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
               w[i] = pack_h2(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down);
           }
           __syncwarp();
-          tmem_st32(tmem + lanes + kColQ + t * 64 + p * 32, w);
+          tc::tmem_st32(tmem + lanes + kColQ + t * 64 + p * 32, w);
         }
         tc::tmem_st_wait();
         tc::tc_fence_before();
@@ -884,7 +864,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
             tc::tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st32(o_addr + 32 * x, o);
+            tc::tmem_st32(o_addr + 32 * x, o);
           }
         }
         const float off = m == -INFINITY ? 0.0f : kBias - m;
@@ -900,7 +880,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
         }
         l += sum[0] + sum[1];
         __syncwarp();
-        tmem_st32(s_addr, p);
+        tc::tmem_st32(s_addr, p);
         tc::tmem_st_wait();
         tc::tc_fence_before();
         __syncwarp();

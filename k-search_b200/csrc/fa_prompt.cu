@@ -175,18 +175,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
@@ -194,25 +182,6 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
-
-// V block as the B operand of P V: N = dims (64 per 128-byte panel, LBO from
-// panel to panel), K = tokens (128 bytes apart, SBO per 8 of them): MN-major,
-// SWIZZLE_128B.
-__device__ __forceinline__ uint64_t v_desc(uint32_t saddr, uint32_t panel) {
-  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-
 // Instruction descriptor, kind::f16: fp32 D, A and B of type T, M = 128; bit 16: B is MN-major.
 template <typename T>
 __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
@@ -327,29 +296,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else if (warp == kMmaWarp) {
     constexpr uint32_t idesc_s = idesc<T>(kTile, false), idesc_o = idesc<T>(DP, true);
     const uint32_t q_base = smem_u32(smem + R::OFF_Q), kv_base = smem_u32(smem + R::OFF_KV);
+    const uint32_t go = tc::elect_one();
     // S_t = Q_t K_j^T
     auto score = [&](int t, int j) {
       const int st = 2 * j % STAGES;
       mbar_wait_or_poison(&kv_full[st], (2 * j / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
       tc::tc_fence_after();
-      if (lane == 0) {
-        const uint64_t qd = tc::sw128_desc(q_base + t * R::OPERAND), kd = tc::sw128_desc(kv_base + st * R::OPERAND);
+      const uint64_t qd = tc::sw128_desc(q_base + t * R::OPERAND), kd = tc::sw128_desc(kv_base + st * R::OPERAND);
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint64_t off = (uint64_t)((k >> 2) * (R::PANEL >> 4) + (k & 3) * 2);
-          mma_ss(tmem + kColS + t * kTile, qd + off, kd + off, idesc_s, k > 0);
-        }
-        tc::mma_commit(&s_full[t]);
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint64_t off = (uint64_t)((k >> 2) * (R::PANEL >> 4) + (k & 3) * 2);
+        tc::mma_ss_go(tmem + kColS + t * kTile, qd + off, kd + off, idesc_s, k > 0, go);
       }
-      __syncwarp();
+      tc::mma_commit_go(&s_full[t], go);
     };
     for (int t = 0; t < 2; ++t)
       if ((t ? n1 : n0) > 0) {
         mbar_wait_or_poison(&q_full[t], 0, a.err, DEV_TIMEOUT_FULL, dead);
         score(t, 0);
       }
-    if (n > 0 && lane == 0) tc::mma_commit(&kv_empty[0]);
-    __syncwarp();
+    if (n > 0) tc::mma_commit_go(&kv_empty[0], go);
     for (int j = 0; j < n; ++j) {
       const int sv = (2 * j + 1) % STAGES;
 #pragma unroll 1
@@ -359,23 +325,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mbar_wait_or_poison(&kv_full[sv], ((2 * j + 1) / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
         mbar_wait_or_poison(&p_full[t], j & 1, a.err, DEV_TIMEOUT_FULL, dead);
         tc::tc_fence_after();
-        if (lane == 0) {
-          const uint64_t vd = v_desc(kv_base + sv * R::OPERAND, R::PANEL);
+        const uint64_t vd = tc::sw128_desc_mn(kv_base + sv * R::OPERAND, R::PANEL);  // dims across, tokens down
 #pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            mma_ts(tmem + kColO + t * DP, tmem + kColS + t * kTile + 8 * k, vd + (uint64_t)(k * (2048 >> 4)), idesc_o,
-                   (j > 0 || k > 0) ? 1u : 0u);
-          if (j + 1 == nt) tc::mma_commit(&o_full[t]);
-        }
-        __syncwarp();
+        for (int k = 0; k < kTile / 16; ++k)
+          tc::mma_ts_go(tmem + kColO + t * DP, tmem + kColS + t * kTile + 8 * k, vd + (uint64_t)(k * (2048 >> 4)), idesc_o,
+                        (j > 0 || k > 0) ? 1u : 0u, go);
+        if (j + 1 == nt) tc::mma_commit_go(&o_full[t], go);
         if (j + 1 < nt) score(t, j + 1);
       }
-      if (lane == 0) {
-        tc::mma_commit(&kv_empty[sv]);
-        if (j + 1 < n) tc::mma_commit(&kv_empty[(2 * j + 2) % STAGES]);
-      }
-      __syncwarp();
+      tc::mma_commit_go(&kv_empty[sv], go);
+      if (j + 1 < n) tc::mma_commit_go(&kv_empty[(2 * j + 2) % STAGES], go);
     }
+    __syncwarp();
   } else {
     const int t = warp >> 2, row = threadIdx.x & 127, nt = t ? n1 : n0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -437,7 +398,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tc::tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-          tmem_st32(o_addr + 32 * c, o);
+          tc::tmem_st32(o_addr + 32 * c, o);
         }
       }
       const float off = m == -INFINITY ? 0.0f : kBias - m;
@@ -453,8 +414,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       __syncwarp();
-      tmem_st32(s_addr, p);
-      tmem_st32(s_addr + 32, p + 32);
+      tc::tmem_st32(s_addr, p);
+      tc::tmem_st32(s_addr + 32, p + 32);
       tc::tmem_st_wait();
       tc::tc_fence_before();
       __syncwarp();

@@ -102,6 +102,58 @@ __device__ __forceinline__ void tmem_st32_const(uint32_t taddr, uint32_t v) {
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 
+// 1 on one lane of a converged warp. Single-thread tcgen05 instructions issued
+// by the whole warp under this predicate keep their operands in uniform
+// registers: in a chain of N = 64 products an `if (lane == 0)` block issued
+// one every 45 clocks, the predicate one every 25 (the product takes 32).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(r));
+  return r;
+}
+// D (+)= A x B^T where `go` (see elect_one): kind::f16, A from shared memory.
+__device__ __forceinline__ void mma_ss_go(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc),
+      "r"(go)
+      : "memory");
+}
+// The same with A from TMEM.
+__device__ __forceinline__ void mma_ts_go(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc),
+      "r"(go)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit_go(uint64_t* bar, uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(go)
+      : "memory");
+}
+
+// 32 consecutive 32-bit TMEM columns of this thread's lane <- v
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+
+// UMMA shared-memory descriptor of a [rows][64 x 16-bit] panel read across its
+// rows (MN-major, SWIZZLE_128B): 64-wide panels `panel` bytes apart (LBO),
+// groups of 8 rows 1024 B apart (SBO).
+__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t panel) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
 // UMMA shared-memory descriptor: K-major, SWIZZLE_128B, 8-row groups 1024 B
 // apart (SBO), version 1 (sm_100).
 __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
