@@ -37,7 +37,6 @@ __device__ __forceinline__ void store_f(__nv_bfloat16* p, float v) { *p = __floa
 // sequence b is one segment with its own softmax state, stored at index c + b
 // (unique: c and b only grow along the row).
 constexpr int kUnit = 16;
-constexpr int kCta = 256;
 
 struct Split {
   const int32_t* seq_lens;
@@ -55,15 +54,20 @@ struct Split {
 };
 __device__ __forceinline__ int unit_begin(int U, int C, int c) { return (int)((long long)U * c / C); }
 
-// Prefix sums of the units of B sequences, kCta contiguous runs of them (one
-// per thread): scan[i] = units before run i, scan[kCta] = all.
+// Prefix sums of the units of B sequences, T contiguous runs of them (one per
+// thread): scan[i] = units before run i, scan[T] = all.
+template <int T>
 struct SplitScan {
-  int scan[kCta + 1];
-  int warp_sums[kCta / 32];
+  int scan[T + 1];
+  int warp_sums[T / 32];
 };
-__device__ __forceinline__ int run_len(const Split& sp) { return (sp.B + kCta - 1) / kCta; }
-__device__ __forceinline__ void scan_units(const Split& sp, SplitScan& ss) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = run_len(sp);
+template <int T>
+__device__ __forceinline__ int run_len(const Split& sp) {
+  return (sp.B + T - 1) / T;
+}
+template <int T>
+__device__ __forceinline__ void scan_units(const Split& sp, SplitScan<T>& ss) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per = run_len<T>(sp);
   int v = 0;
   for (int b = tid * per; b < min(sp.B, (tid + 1) * per); ++b) v += sp.units(b);
 #pragma unroll
@@ -79,8 +83,9 @@ __device__ __forceinline__ void scan_units(const Split& sp, SplitScan& ss) {
   __syncthreads();
 }
 // Units before sequence b.
-__device__ __forceinline__ int units_before(const Split& sp, const SplitScan& ss, int b) {
-  const int per = run_len(sp), run = b / per;
+template <int T>
+__device__ __forceinline__ int units_before(const Split& sp, const SplitScan<T>& ss, int b) {
+  const int per = run_len<T>(sp), run = b / per;
   int u = ss.scan[run];
   for (int i = run * per; i < b; ++i) u += sp.units(i);
   return u;
@@ -99,8 +104,9 @@ __device__ __forceinline__ int units_before(const Split& sp, const SplitScan& ss
 //     that small scales stay in fp16's normal range. d_v up to 1023 fits.
 // The head dimension is permuted inside a block so that every operand word is
 // one 32-bit load (a word of 4 codes) per lane.
-constexpr int kStreamWarps = kCta / 32;
-constexpr int kStages = 3;
+constexpr int kStreamWarps = 12;
+constexpr int kStreamThreads = kStreamWarps * 32;
+constexpr int kStages = 4;
 constexpr float kPBits = 6.0f, kPScale = 64.0f;
 
 template <int NB>
@@ -114,7 +120,9 @@ struct Row {
   static constexpr int COPIES = (8 * CHUNKS + 31) / 32;  // per lane, for 8 rows
   static constexpr bool ALWAYS = 16 * (CHUNKS - 1) < BYTES;  // every piece holds bytes of the row wherever it starts
   static constexpr int STAGE = 2 * kUnit * PITCH;
-  static constexpr int SMEM = kStreamWarps * kStages * STAGE;
+  // fewer stages where the rows are long
+  static constexpr int STAGES = kStreamWarps * kStages * STAGE <= 221184 ? kStages : 2;
+  static constexpr int SMEM = kStreamWarps * STAGES * STAGE;
 };
 
 // 16 bytes to shared memory, asynchronously (groups of them are waited for).
@@ -190,77 +198,102 @@ __device__ __forceinline__ void codes_h2(uint32_t w, uint32_t& lo, uint32_t& hi)
   lo = hsub2(__byte_perm(u, 0x64646464u, 0x4140), 0x64806480u);
   hi = hsub2(__byte_perm(u, 0x64646464u, 0x4342), 0x64806480u);
 }
-// The word at byte offset `off` (even) of 4-byte aligned shared memory.
-__device__ __forceinline__ uint32_t word_at(const uint8_t* p, int off) {
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(p + (off & ~3));
-  return (off & 2) ? __funnelshift_r(w[0], w[1], 16) : w[0];
-}
-__device__ __forceinline__ float scale_at(const uint8_t* p, int off) {
-  return __half2float(*reinterpret_cast<const __half*>(p + off));
+// The 32-bit word `off` bytes (even) behind `at` in shared memory. Rows of an
+// even number of blocks start at multiples of 4, so a constant `off` decides
+// between one load and two; the others decide per lane.
+template <int NB>
+__device__ __forceinline__ uint32_t word_at(const uint8_t* at, int off) {
+  if constexpr (NB % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(at + (off & ~3));
+    return (off & 2) ? __funnelshift_r(w[0], w[1], 16) : w[0];
+  } else {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(at) + off;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(x & ~(uintptr_t)3);
+    return (x & 2) ? __funnelshift_r(w[0], w[1], 16) : w[0];
+  }
 }
 
 // A position in a worker's row of units.
 struct Cursor {
   int b, tok, n;  // sequence, first token of the tile, the sequence's end
+  int col, off;   // its page (a column of the table) and place in it
 };
 
 template <int NB, bool WIDE>
-__global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_stream_kernel(const StreamArgs a) {
+__global__ void __launch_bounds__(kStreamThreads, 1) fa_paged_stream_kernel(const StreamArgs a) {
   using R = Row<NB>;
+  constexpr int kSt = R::STAGES;
   constexpr int RH = WIDE ? 2 : 1;  // row halves in use: query heads lane / 4 (+ 8)
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ SplitScan ss;
+  __shared__ __align__(16) float s_scale[kStreamWarps][2][NB][kUnit];  // K and V scales of the tile at hand
+  auto& ss = *reinterpret_cast<SplitScan<kStreamThreads>*>(smem);        // before the rings are in use
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   pdl_launch_dependents();
   scan_units(a.split, ss);
-  const int U = ss.scan[kCta], C = a.split.active(U);
+  const int U = ss.scan[kStreamThreads], C = a.split.active(U);
   const int per_worker = a.Hkv * a.QG;
   const int gw = blockIdx.x * kStreamWarps + warp;
   const int wk = gw / per_worker, hw = gw % per_worker, h = hw / a.QG, qg = hw % a.QG;
   // a programmatic dependent of the prefix kernel, whose results it does not
   // read: it only may not end before it (the combine waits for this grid)
-  if (wk >= C) return pdl_wait();
-  int u = unit_begin(U, C, wk);
-  const int ue = unit_begin(U, C, wk + 1);
+  int u = 0, ue = 0;
+  Cursor f{};  // the worker's first tile
+  if (wk < C) {
+    u = unit_begin(U, C, wk), ue = unit_begin(U, C, wk + 1);
+    if (u < ue) {
+      int lo = 0, hi = kStreamThreads;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (ss.scan[mid] <= u) lo = mid;
+        else hi = mid;
+      }
+      f.b = lo * run_len<kStreamThreads>(a.split);
+      int before = ss.scan[lo], here;
+      while (before + (here = a.split.units(f.b)) <= u) {
+        before += here;
+        ++f.b;
+      }
+      f.n = a.split.len(f.b);
+      f.tok = a.split.first() + (u - before) * kUnit;
+      f.col = f.tok / a.ps, f.off = f.tok % a.ps;
+    }
+  }
+  __syncthreads();  // the scan is read: the rings may be written
   if (u >= ue) return pdl_wait();
 
-  uint8_t* ring = smem + warp * kStages * R::STAGE;
+  uint8_t* ring = smem + warp * kSt * R::STAGE;
   const long long row_bytes = (long long)a.Hkv * R::BYTES;
   const int head_off = h * R::BYTES, row15 = (int)(row_bytes & 15);
 
-  // the worker's first tile
-  Cursor f;
-  {
-    int lo = 0, hi = kCta;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (ss.scan[mid] <= u) lo = mid;
-      else hi = mid;
-    }
-    f.b = lo * run_len(a.split);
-    int before = ss.scan[lo], here;
-    while (before + (here = a.split.units(f.b)) <= u) {
-      before += here;
-      ++f.b;
-    }
-    f.n = a.split.len(f.b);
-    f.tok = a.split.first() + (u - before) * kUnit;
-  }
-  Cursor cur = f;
+  // The tile being consumed, in the same row of units.
+  int cb = f.b, ctok = f.tok, cn = f.n;
+  // Places in a stage: rows start at the 16-byte boundary below them, and 8
+  // rows of a unit follow each other in a page, so the start within the first
+  // 16 bytes depends on the row index mod 8 only.
+  auto row_at = [&](int i) { return i * R::PITCH + (((i & 7) * row15 + head_off) & 15); };
+  const int at_k = row_at(g) + 4 * c;                                  // K row g (g + 8: 8 rows on)
+  const int at_v0 = kUnit * R::PITCH + row_at(2 * c) + 4 * g;          // V rows 2 c, 2 c + 1 (and + 8)
+  const int at_v1 = kUnit * R::PITCH + row_at(2 * c + 1) + 4 * g;
+  const int at_s = (lane >> 4) * kUnit * R::PITCH + row_at(lane & 15);  // this lane's row, for its scales
   auto advance = [&](Cursor& x) {  // to the next tile of the row (there is one)
     x.tok += kUnit;
-    while (x.tok >= x.n || x.n <= a.split.start) {
-      ++x.b;
-      x.n = a.split.len(x.b);
+    x.off += kUnit;
+    while (x.off >= a.ps) x.off -= a.ps, ++x.col;
+    if (x.tok >= x.n) {
+      do {
+        ++x.b;
+        x.n = a.split.len(x.b);
+      } while (x.n <= a.split.start);
       x.tok = a.split.first();
+      x.col = x.tok / a.ps, x.off = x.tok % a.ps;
     }
   };
   // pages of the two groups of 8 tokens of tile x (-1: no such token)
   auto pages_of = [&](const Cursor& x) {
     int2 p = make_int2(-1, -1);
-    const int32_t* t = a.table + (long long)(x.tok < a.prefix_len ? 0 : x.b) * a.W;
-    p.x = t[x.tok / a.ps];
-    if (x.tok + 8 < x.n) p.y = (x.tok + 8 < a.prefix_len ? a.table : a.table + (long long)x.b * a.W)[(x.tok + 8) / a.ps];
+    const int32_t* t = a.table + (long long)x.b * a.W;
+    p.x = (x.tok < a.prefix_len ? a.table : t)[x.col];
+    if (x.tok + 8 < x.n) p.y = (x.tok + 8 < a.prefix_len ? a.table : t)[x.col + (x.off + 8 >= a.ps)];
     return p;
   };
   const Pieces<NB> pieces(lane, row_bytes, head_off);
@@ -272,7 +305,8 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
     for (int half = 0; half < 2; ++half) {
       const int page = half ? p.y : p.x, tok = x.tok + 8 * half;
       if (page >= 0 && page < a.num_pages) {
-        const long long at = ((long long)page * a.ps + tok % a.ps) * row_bytes;
+        const int off = x.off + 8 * half;
+        const long long at = ((long long)page * a.ps + (off >= a.ps ? off - a.ps : off)) * row_bytes;
         const uint32_t to = ring32 + st * R::STAGE + half * 8 * R::PITCH;
         pieces.copy(to, a.k + at);
         pieces.copy(to + kUnit * R::PITCH, a.v + at);
@@ -286,11 +320,11 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
   int left = ue - u;         // tiles not yet consumed
   int ahead = left;          // tiles not yet issued
   int2 page = pages_of(f);
-  uint32_t masks[kStages];   // rows present in the tiles in flight, oldest first
+  uint32_t masks[kSt];   // rows present in the tiles in flight, oldest first
 #pragma unroll
-  for (int i = 0; i < kStages; ++i) masks[i] = 0;
+  for (int i = 0; i < kSt; ++i) masks[i] = 0;
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
+  for (int i = 0; i < kSt - 1; ++i) {
     if (ahead > 0) {
       masks[i] = issue(f, page, i);
       if (--ahead > 0) {
@@ -304,7 +338,7 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
   int st = 0;
   while (left > 0) {
     // ---- a segment: the worker's tiles of sequence cur.b
-    const int b = cur.b;
+    const int b = cb;
     uint32_t qa[2 * NB][2 * RH];
     float sl[RH];
 #pragma unroll
@@ -352,19 +386,20 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
 #pragma unroll
     for (int r = 0; r < RH; ++r) m[r] = -INFINITY, l[r] = 0.0f;
 
-    int tiles = min(left, (cur.n - cur.tok + kUnit - 1) / kUnit);
+    int tiles = min(left, (cn - ctok + kUnit - 1) / kUnit);
     left -= tiles;
-    int tok = cur.tok;
     if (left > 0) {
-      cur.tok = cur.n - 1;  // the last tile of this sequence, then the next
-      advance(cur);
+      do {
+        cn = a.split.len(++cb);
+      } while (cn <= a.split.start);
+      ctok = a.split.first();
     }
-    for (; tiles > 0; --tiles, tok += kUnit) {
+    for (; tiles > 0; --tiles) {
       // keep the ring full: the stage read in the previous step is free
       uint32_t fresh = 0;
       if (ahead > 0) {
-        int s2 = st + kStages - 1;
-        s2 = s2 >= kStages ? s2 - kStages : s2;
+        int s2 = st + kSt - 1;
+        s2 = s2 >= kSt ? s2 - kSt : s2;
         fresh = issue(f, page, s2);
         if (--ahead > 0) {
           advance(f);
@@ -374,19 +409,28 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
       copy_commit();
       const uint32_t mask = masks[0];
 #pragma unroll
-      for (int i = 0; i + 1 < kStages; ++i) masks[i] = masks[i + 1];
-      masks[kStages - 2] = fresh;
-      copy_wait<kStages - 1>();
+      for (int i = 0; i + 1 < kSt; ++i) masks[i] = masks[i + 1];
+      masks[kSt - 2] = fresh;
+      copy_wait<kSt - 1>();
       __syncwarp();
-      const uint8_t* ks = ring + st * R::STAGE;
-      const uint8_t* vs = ks + kUnit * R::PITCH;
-      // start of a row's blocks within its slot of the stage
-      auto at = [&](int i) { return i * R::PITCH + (((i & 7) * row15 + head_off) & 15); };
+      const uint8_t* stage = ring + st * R::STAGE;
+      {
+        // a row per lane: its scales in fp32. An absent row may hold anything:
+        // its weight is 0, not 0 x scale
+        const uint8_t* row = stage + at_s;
+        const bool there = mask >> (lane & 15) & 1;
+        const float unit = lane < 16 ? 1.0f : kPScale;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+          s_scale[warp][lane >> 4][j][lane & 15] = there ? __half2float(*reinterpret_cast<const __half*>(row + j * kQ8)) * unit : 0.0f;
+      }
+      __syncwarp();
+      auto scales = [&](int kv, int j, int i) { return *reinterpret_cast<const float2*>(&s_scale[warp][kv][j][i]); };
 
       float s[2][2 * RH];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int kr = at(8 * t + g), k0 = at(8 * t + 2 * c), k1 = at(8 * t + 2 * c + 1);
+        const uint8_t* kr = stage + at_k + t * 8 * R::PITCH;
 #pragma unroll
         for (int r = 0; r < 2 * RH; ++r) s[t][r] = 0.0f;
 #pragma unroll
@@ -395,15 +439,15 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             uint32_t b0, b1;
-            codes_h2(word_at(ks, kr + j * kQ8 + 2 + 16 * x + 4 * c), b0, b1);
+            codes_h2(word_at<NB>(kr, j * kQ8 + 2 + 16 * x), b0, b1);
             const uint32_t* q = qa[2 * j + x];
             mma16816(d, q[0], WIDE ? q[1] : 0u, q[RH], WIDE ? q[2 * RH - 1] : 0u, b0, b1);
           }
-          const float d0 = scale_at(ks, k0 + j * kQ8), d1 = scale_at(ks, k1 + j * kQ8);
+          const float2 dk = scales(0, j, 8 * t + 2 * c);
 #pragma unroll
           for (int r = 0; r < RH; ++r) {
-            s[t][2 * r] = fmaf(d[2 * r], d0, s[t][2 * r]);
-            s[t][2 * r + 1] = fmaf(d[2 * r + 1], d1, s[t][2 * r + 1]);
+            s[t][2 * r] = fmaf(d[2 * r], dk.x, s[t][2 * r]);
+            s[t][2 * r + 1] = fmaf(d[2 * r + 1], dk.y, s[t][2 * r + 1]);
           }
         }
       }
@@ -446,29 +490,18 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
 #pragma unroll
           for (int r = 0; r < 2 * RH; ++r) acc[i][r] *= f_[r >> 1];
       }
-      int vr[4];
-      bool von[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int ti = 2 * c + (i & 1) + 8 * (i >> 1);
-        vr[i] = at(ti);
-        von[i] = on[i >> 1][i & 1];
-      }
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
-        float dv[4];
         uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // an absent row may hold anything: its weight is 0, not 0 x scale
-          dv[i] = von[i] ? scale_at(vs, vr[i] + j * kQ8) * kPScale : 0.0f;
-          w[i] = word_at(vs, vr[i] + j * kQ8 + 2 + 4 * g) ^ 0x80808080u;
-        }
+        for (int i = 0; i < 4; ++i)
+          w[i] = word_at<NB>(stage + ((i & 1) ? at_v1 : at_v0) + (i >> 1) * 8 * R::PITCH, j * kQ8 + 2) ^ 0x80808080u;
+        const float2 d0 = scales(1, j, 2 * c), d1 = scales(1, j, 8 + 2 * c);
         uint32_t pa[2 * RH];
 #pragma unroll
         for (int r = 0; r < RH; ++r) {
-          pa[r] = pack_h2(p[0][2 * r] * dv[0], p[0][2 * r + 1] * dv[1]);
-          pa[RH + r] = pack_h2(p[1][2 * r] * dv[2], p[1][2 * r + 1] * dv[3]);
+          pa[r] = pack_h2(p[0][2 * r] * d0.x, p[0][2 * r + 1] * d0.y);
+          pa[RH + r] = pack_h2(p[1][2 * r] * d1.x, p[1][2 * r + 1] * d1.y);
         }
         // byte i of the two tokens of a pair, for the 4 dims of the word
         const uint32_t x01 = __byte_perm(w[0], w[1], 0x5140), x23 = __byte_perm(w[0], w[1], 0x7362);
@@ -486,7 +519,7 @@ __global__ void __launch_bounds__(kCta, (NB <= 4 && !WIDE) ? 2 : 1) fa_paged_str
         }
       }
       __syncwarp();  // the stage may be refilled
-      if (++st == kStages) st = 0;
+      if (++st == kSt) st = 0;
     }
     // ---- the segment's state
     const long long seg = wk + b;
@@ -912,8 +945,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
 }
 
 // ---- combine -------------------------------------------------------------------------
-// One warp per (sequence, query head): the states of its segments, merged with
-// the maximum of their maxima; out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i.
+// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's states (the
+// prefix chunks, then its segments), M the largest m_i. WR warps share a row:
+// warp w takes states w, w + WR, ..., kAtOnce loads in flight, and the first
+// one adds the others' sums from shared memory in their order.
 struct CombineArgs {
   Split split;
   const float* part;
@@ -924,62 +959,107 @@ struct CombineArgs {
   int Hq, D;
   void* out;
 };
+constexpr int kAtOnce = 8;
+constexpr int kCta = 256;
 
-template <typename T>
+template <typename T, int WR>
 __global__ void __launch_bounds__(kCta) fa_paged_combine_kernel(const CombineArgs a) {
-  __shared__ SplitScan ss;
+  __shared__ SplitScan<kCta> ss;
+  __shared__ float4 s_o[kCta / 32][kMaxNB * 32 / 4];
+  __shared__ float2 s_ml[kCta / 32];
   scan_units(a.split, ss);
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * kStreamWarps + warp;
-  if (row >= (long long)a.split.B * a.Hq) return;
-  const int b = (int)(row / a.Hq), h = (int)(row % a.Hq);
-  const int U = ss.scan[kCta], C = a.split.active(U);
-  const int u0 = units_before(a.split, ss, b), u1 = u0 + a.split.units(b);
-  // workers whose range meets [u0, u1): the last c with begin(c) <= u, for both ends
-  auto worker_of = [&](int u) {
-    int c = (int)((long long)u * C / max(U, 1));
-    while (c + 1 < C && unit_begin(U, C, c + 1) <= u) ++c;
-    while (c > 0 && unit_begin(U, C, c) > u) --c;
-    return c;
-  };
-  const int c0 = u1 > u0 ? worker_of(u0) : 0, n = u1 > u0 ? worker_of(u1 - 1) - c0 + 1 : 0;
+  constexpr int ROWS = kCta / 32 / WR;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp % WR;
+  const long long brows = (long long)a.split.B * a.Hq;
+  const long long row = (long long)blockIdx.x * ROWS + warp / WR;
+  const bool real = row < brows;
   constexpr int kVec = kMaxNB * 32 / 128;
   float4 o[kVec];
 #pragma unroll
   for (int i = 0; i < kVec; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float M = -INFINITY, L = 0.0f;
-  // state i of the row: a prefix chunk, then a segment
-  const long long brows = (long long)a.split.B * a.Hq;
-  const int total = a.chunks + n;
-  auto index = [&](int i) { return i < a.chunks ? i * brows + row : ((long long)c0 + b + i - a.chunks) * a.Hq + h; };
-  for (int i0 = 0; i0 < total; i0 += 32) {
-    float2 s = make_float2(-INFINITY, 0.0f);
-    if (i0 + lane < total) s = (i0 + lane < a.chunks ? a.pml : a.ml)[index(i0 + lane)];
-    const float Mn = fmaxf(M, warp_max(s.x));
-    const float base = Mn == -INFINITY ? 0.0f : Mn;
-    const float f = ex2(M - base), wgt = ex2(s.x - base);
-    float t = wgt * s.y;
+  if (real) {
+    const int b = (int)(row / a.Hq), h = (int)(row % a.Hq);
+    const int U = ss.scan[kCta], C = a.split.active(U);
+    const int u0 = units_before(a.split, ss, b), u1 = u0 + a.split.units(b);
+    // workers whose range meets [u0, u1): the last c with begin(c) <= u, for both ends
+    auto worker_of = [&](int u) {
+      int c = (int)((long long)u * C / max(U, 1));
+      while (c + 1 < C && unit_begin(U, C, c + 1) <= u) ++c;
+      while (c > 0 && unit_begin(U, C, c) > u) --c;
+      return c;
+    };
+    const int c0 = u1 > u0 ? worker_of(u0) : 0, n = u1 > u0 ? worker_of(u1 - 1) - c0 + 1 : 0;
+    const int total = a.chunks + n;
+    auto index = [&](int i) { return i < a.chunks ? i * brows + row : ((long long)c0 + b + i - a.chunks) * a.Hq + h; };
+    for (int i0 = w; i0 < total; i0 += 32 * WR) {
+      float2 s = make_float2(-INFINITY, 0.0f);
+      const int mine = i0 + lane * WR;
+      if (mine < total) s = (mine < a.chunks ? a.pml : a.ml)[index(mine)];
+      const float Mn = fmaxf(M, warp_max(s.x));
+      const float base = Mn == -INFINITY ? 0.0f : Mn;
+      const float f = ex2(M - base), wgt = ex2(s.x - base);
+      float t = wgt * s.y;
 #pragma unroll
-    for (int x = 16; x >= 1; x >>= 1) t += __shfl_xor_sync(0xffffffffu, t, x);
-    L = L * f + t;
-    M = Mn;
+      for (int x = 16; x >= 1; x >>= 1) t += __shfl_xor_sync(0xffffffffu, t, x);
+      L = L * f + t;
+      M = Mn;
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) o[i].x *= f, o[i].y *= f, o[i].z *= f, o[i].w *= f;
-    const int cnt = min(32, total - i0);
-#pragma unroll 4
-    for (int k = 0; k < cnt; ++k) {
-      const float wk = __shfl_sync(0xffffffffu, wgt, k);
-      const float4* p = reinterpret_cast<const float4*>((i0 + k < a.chunks ? a.ppart : a.part) + index(i0 + k) * a.D);
+      for (int i = 0; i < kVec; ++i) o[i].x *= f, o[i].y *= f, o[i].z *= f, o[i].w *= f;
+      const int cnt = min(32, (total - i0 + WR - 1) / WR);
+      for (int k0 = 0; k0 < cnt; k0 += kAtOnce) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          if (i * 128 >= a.D) break;
+          float4 v[kAtOnce];
+#pragma unroll
+          for (int k = 0; k < kAtOnce; ++k) {
+            const int x = i0 + min(k0 + k, cnt - 1) * WR;  // the last one again past the end, with weight 0
+            const float4* p = reinterpret_cast<const float4*>((x < a.chunks ? a.ppart : a.part) + index(x) * a.D);
+            v[k] = i * 128 + lane * 4 < a.D ? p[i * 32 + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          }
+#pragma unroll
+          for (int k = 0; k < kAtOnce; ++k) {
+            const float wk = k0 + k < cnt ? __shfl_sync(0xffffffffu, wgt, min(k0 + k, 31)) : 0.0f;
+            o[i].x = fmaf(wk, v[k].x, o[i].x), o[i].y = fmaf(wk, v[k].y, o[i].y);
+            o[i].z = fmaf(wk, v[k].z, o[i].z), o[i].w = fmaf(wk, v[k].w, o[i].w);
+          }
+        }
+      }
+    }
+  }
+  if (WR > 1) {
+    if (w > 0) {
 #pragma unroll
       for (int i = 0; i < kVec; ++i)
-        if (i * 128 + lane * 4 < a.D) {
-          const float4 v = p[i * 32 + lane];
-          o[i].x = fmaf(wk, v.x, o[i].x), o[i].y = fmaf(wk, v.y, o[i].y);
-          o[i].z = fmaf(wk, v.z, o[i].z), o[i].w = fmaf(wk, v.w, o[i].w);
+        if (i * 128 < a.D) s_o[warp][i * 32 + lane] = o[i];
+      if (lane == 0) s_ml[warp] = make_float2(M, L);
+    }
+    __syncthreads();
+    if (w > 0) return;
+    float top = M;
+#pragma unroll
+    for (int k = 1; k < WR; ++k) top = fmaxf(top, s_ml[warp + k].x);
+    const float base = top == -INFINITY ? 0.0f : top, f = ex2(M - base);
+    L *= f;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) o[i].x *= f, o[i].y *= f, o[i].z *= f, o[i].w *= f;
+#pragma unroll
+    for (int k = 1; k < WR; ++k) {
+      const float2 s = s_ml[warp + k];
+      const float fk = ex2(s.x - base);
+      L = fmaf(fk, s.y, L);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        if (i * 128 < a.D) {
+          const float4 v = s_o[warp + k][i * 32 + lane];
+          o[i].x = fmaf(fk, v.x, o[i].x), o[i].y = fmaf(fk, v.y, o[i].y);
+          o[i].z = fmaf(fk, v.z, o[i].z), o[i].w = fmaf(fk, v.w, o[i].w);
         }
     }
   }
+  if (!real) return;
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   T* out = static_cast<T*>(a.out) + row * a.D;
 #pragma unroll
@@ -1068,10 +1148,10 @@ __global__ void __launch_bounds__(kWarps * 32) fa_paged_simple_kernel(const FaPa
     if (t < nb) store_f(out + t * 32 + lane, acc[t] * inv);
 }
 
-// Workers per KV head (and group of 16 of its query heads): two CTAs' warps per SM in all.
+// Workers per KV head (and group of 16 of its query heads): one CTA's warps per SM in all.
 int workers_of(const FaPagedArgs& a) {
   const int qg = (a.Hq / a.Hkv + 15) / 16;
-  return std::max(1, sm_count() * 2 * kStreamWarps / (a.Hkv * qg));
+  return std::max(1, sm_count() * kStreamWarps / (a.Hkv * qg));
 }
 // The prefix kernel's pass: head dimensions up to 128, whole groups of 8
 // tokens per page, and a batch (one sequence alone streams its prefix).
@@ -1116,11 +1196,11 @@ kq_status_t launch_prefix_nb(const PrefixArgs& a, int grid, cudaStream_t s) {
 // Launches `kernel` as a programmatic dependent of the previous kernel on s
 // (plainly where !pdl).
 template <typename... Params, typename Arg>
-kq_status_t launch_after(void (*kernel)(Params...), int grid, int smem, bool pdl, cudaStream_t s, const Arg& arg,
+kq_status_t launch_after(void (*kernel)(Params...), int grid, int threads, int smem, bool pdl, cudaStream_t s, const Arg& arg,
                          const char* what) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kCta);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr{};
@@ -1135,11 +1215,18 @@ template <int NB, bool WIDE>
 kq_status_t launch_stream(const StreamArgs& a, int grid, bool pdl, cudaStream_t s) {
   auto kernel = fa_paged_stream_kernel<NB, WIDE>;
   if (kq_status_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), Row<NB>::SMEM, "fa_paged")) return st;
-  return launch_after(kernel, grid, Row<NB>::SMEM, pdl, s, a, "fa_paged_stream");
+  return launch_after(kernel, grid, kStreamThreads, Row<NB>::SMEM, pdl, s, a, "fa_paged_stream");
 }
 template <int NB>
 kq_status_t launch_stream_nb(const StreamArgs& a, int grid, bool pdl, cudaStream_t s) {
   return a.G > 8 ? launch_stream<NB, true>(a, grid, pdl, s) : launch_stream<NB, false>(a, grid, pdl, s);
+}
+
+template <typename T>
+kq_status_t launch_combine(const CombineArgs& a, long long rows, cudaStream_t s) {
+  if (rows <= sm_count() * 4)
+    return launch_after(fa_paged_combine_kernel<T, 8>, (int)rows, kCta, 0, true, s, a, "fa_paged_combine");
+  return launch_after(fa_paged_combine_kernel<T, 2>, (int)((rows + 3) / 4), kCta, 0, true, s, a, "fa_paged_combine");
 }
 
 }  // namespace
@@ -1205,9 +1292,9 @@ kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s) {
   if (st) return st;
   CombineArgs ca{p.split, p.part, p.ml, reinterpret_cast<float*>(ws + w.ppart), reinterpret_cast<float2*>(ws + w.pml),
                  chunks, a.Hq, a.D, a.out};
-  const int cgrid = (int)(((long long)a.B * a.Hq + kStreamWarps - 1) / kStreamWarps);
-  return dtype == KQ_F16 ? launch_after(fa_paged_combine_kernel<__half>, cgrid, 0, true, s, ca, "fa_paged_combine")
-                         : launch_after(fa_paged_combine_kernel<__nv_bfloat16>, cgrid, 0, true, s, ca, "fa_paged_combine");
+  // eight warps per row while that leaves the SMs room, else two
+  const long long rows = (long long)a.B * a.Hq;
+  return dtype == KQ_F16 ? launch_combine<__half>(ca, rows, s) : launch_combine<__nv_bfloat16>(ca, rows, s);
 }
 
 }  // namespace kq
