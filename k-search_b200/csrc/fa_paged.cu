@@ -177,11 +177,12 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// d = a b + (c0, c1, c2, c3)
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                                         uint32_t b1, float c0, float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -435,14 +436,15 @@ __global__ void __launch_bounds__(kStreamThreads, 1) fa_paged_stream_kernel(cons
         for (int r = 0; r < 2 * RH; ++r) s[t][r] = 0.0f;
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            uint32_t b0, b1;
-            codes_h2(word_at<NB>(kr, j * kQ8 + 2 + 16 * x), b0, b1);
-            const uint32_t* q = qa[2 * j + x];
-            mma16816(d, q[0], WIDE ? q[1] : 0u, q[RH], WIDE ? q[2 * RH - 1] : 0u, b0, b1);
-          }
+          float d[4];
+          uint32_t b0, b1;
+          const uint32_t* q = qa[2 * j];
+          codes_h2(word_at<NB>(kr, j * kQ8 + 2), b0, b1);
+          mma16816(d, q[0], WIDE ? q[1] : 0u, q[RH], WIDE ? q[2 * RH - 1] : 0u, b0, b1, 0.0f, 0.0f, 0.0f, 0.0f);
+          q = qa[2 * j + 1];
+          codes_h2(word_at<NB>(kr, j * kQ8 + 18), b0, b1);
+          mma16816(d, q[0], WIDE ? q[1] : 0u, q[RH], WIDE ? q[2 * RH - 1] : 0u, b0, b1, d[0], d[1], WIDE ? d[2] : 0.0f,
+                   WIDE ? d[3] : 0.0f);
           const float2 dk = scales(0, j, 8 * t + 2 * c);
 #pragma unroll
           for (int r = 0; r < RH; ++r) {
@@ -451,11 +453,17 @@ __global__ void __launch_bounds__(kStreamThreads, 1) fa_paged_stream_kernel(cons
           }
         }
       }
-      bool on[2][2];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) on[t][x] = (mask >> (8 * t + 2 * c + x)) & 1u;
+        for (int r = 0; r < 2 * RH; ++r) s[t][r] *= sl[r >> 1];
+      if (mask != 0xffffu) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 2 * RH; ++r)
+            if (!(mask >> (8 * t + 2 * c + (r & 1)) & 1u)) s[t][r] = -INFINITY;
+      }
       float p[2][2 * RH], f_[RH];
       bool moved = false;
 #pragma unroll
@@ -464,10 +472,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) fa_paged_stream_kernel(cons
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            s[t][2 * r + x] = on[t][x] ? s[t][2 * r + x] * sl[r] : -INFINITY;
-            mx = fmaxf(mx, s[t][2 * r + x]);
-          }
+          for (int x = 0; x < 2; ++x) mx = fmaxf(mx, s[t][2 * r + x]);
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float base = mx == -INFINITY ? 0.0f : mx;
@@ -512,8 +517,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1) fa_paged_stream_kernel(cons
           const uint32_t b0 = hsub2(__byte_perm(i < 2 ? x01 : x23, 0x64646464u, sel), 0x64806480u);
           const uint32_t b1 = hsub2(__byte_perm(i < 2 ? y01 : y23, 0x64646464u, sel), 0x64806480u);
           float* d = acc[4 * j + i];
-          float t4[4] = {d[0], d[1], WIDE ? d[2 * RH - 2] : 0.0f, WIDE ? d[2 * RH - 1] : 0.0f};
-          mma16816(t4, pa[0], WIDE ? pa[1] : 0u, pa[RH], WIDE ? pa[2 * RH - 1] : 0u, b0, b1);
+          float t4[4];
+          mma16816(t4, pa[0], WIDE ? pa[1] : 0u, pa[RH], WIDE ? pa[2 * RH - 1] : 0u, b0, b1, d[0], d[1],
+                   WIDE ? d[2 * RH - 2] : 0.0f, WIDE ? d[2 * RH - 1] : 0.0f);
           d[0] = t4[0], d[1] = t4[1];
           if (WIDE) d[2 * RH - 2] = t4[2], d[2 * RH - 1] = t4[3];
         }
