@@ -14,8 +14,6 @@ is read back to the host. Tensors belong to one device. Caches are uint8
 """
 from __future__ import annotations
 
-import ctypes
-import math
 from typing import NamedTuple
 
 import torch
@@ -33,72 +31,75 @@ class PagePlan(NamedTuple):
     counts: torch.Tensor      # int32 [2]: pages the step needs, new tokens without a slot
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
+# The checks run on every call, in front of kernels of a few microseconds: they
+# read each attribute once and build messages only to raise.
 def _tensor(t, name: str, dtype, device=None) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
     return t
 
 
-def _ints(t, name: str, device, shape) -> torch.Tensor:
-    _tensor(t, name, torch.int32, device)
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t
-
-
-def _rows(t, name: str, dtype, device=None) -> torch.Tensor:
+def _vector(t, name: str, dtype, device, n: int) -> torch.Tensor:
     _tensor(t, name, dtype, device)
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {list(t.shape)}")
-    if t.stride(2) != 1 and t.shape[2] > 1 and t.numel() > 0:
-        raise ValueError(f"{name}'s head dimension must be contiguous")
+    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous [{n}], got {list(t.shape)}")
     return t
+
+
+def _table(t, device, B: int | None) -> torch.Size:
+    _tensor(t, "block_tables", torch.int32, device)
+    shape = t.shape
+    if len(shape) != 2 or (B is not None and shape[0] != B) or not t.is_contiguous():
+        raise ValueError(f"block_tables must be contiguous [{'B' if B is None else B}, max_blocks], got {list(shape)}")
+    return shape
+
+
+def _rows(t, name: str, dtype, device=None) -> torch.Size:
+    _tensor(t, name, dtype, device)
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {list(shape)}")
+    if t.stride(2) != 1 and shape[2] > 1 and t.numel() > 0:
+        raise ValueError(f"{name}'s head dimension must be contiguous")
+    return shape
 
 
 def _float16(t, name: str) -> int:
-    if not isinstance(t, torch.Tensor) or t.dtype not in DTYPES:
+    dt = DTYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
+    if dt is None:
         raise ValueError(f"{name} must be a float16 or bfloat16 CUDA tensor")
-    return DTYPES[t.dtype]
+    return dt
 
 
-def _caches(k_cache, v_cache, device) -> tuple[int, int, int, int]:
-    """(num_pages, page_size, Hkv, D) of a checked cache pair."""
+def _caches(k_cache, v_cache, device) -> torch.Size:
+    """[num_pages, page_size, Hkv, D/32, 34] of a checked cache pair."""
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         _tensor(t, name, torch.uint8, device)
-        if t.dim() != 5 or t.shape[4] != 34 or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous uint8 [num_pages, page_size, Hkv, D/32, 34], got {list(t.shape)}")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError(f"k_cache {list(k_cache.shape)} and v_cache {list(v_cache.shape)} differ")
-    pages, ps, hkv, nb, _ = k_cache.shape
-    return pages, ps, hkv, nb * 32
+        shape = t.shape
+        if len(shape) != 5 or shape[4] != 34 or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous uint8 [num_pages, page_size, Hkv, D/32, 34], got {list(shape)}")
+    if k_cache.shape != shape:
+        raise ValueError(f"k_cache {list(k_cache.shape)} and v_cache {list(shape)} differ")
+    return shape
 
 
-class _on:
-    """Makes the tensors' device current for a launch (nothing to do when it is already)."""
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
-    def __init__(self, device):
-        self.device = device
-        self.before = torch.cuda.current_device()
 
-    def __enter__(self):
-        if self.device.index != self.before:
-            torch.cuda.set_device(self.device)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *_):
-        if self.device.index != self.before:
-            torch.cuda.set_device(self.before)
+def _call(entry: str, device: torch.device, *args) -> None:
+    """entry(*args, current stream of `device`) with that device current."""
+    before = torch.cuda.current_device()
+    if device.index == before:
+        status = getattr(lib(), entry)(*args, _raw_stream(before))
+    else:
+        with torch.cuda.device(device):
+            status = getattr(lib(), entry)(*args, _raw_stream(device.index))
+    if status:
+        check(status, entry)
 
 
 def page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor, free_pages: torch.Tensor,
@@ -114,29 +115,26 @@ def page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
     tokens got no slot. ``out``: an earlier plan whose tensors are reused."""
     dev = _tensor(cached_lens, "cached_lens", torch.int32).device
     B = cached_lens.numel()
-    _ints(cached_lens, "cached_lens", dev, (B,))
-    _ints(new_lens, "new_lens", dev, (B,))
-    _tensor(block_tables, "block_tables", torch.int32, dev)
-    _need(block_tables.dim() == 2 and block_tables.shape[0] == B and block_tables.is_contiguous(),
-          f"block_tables must be contiguous [{B}, max_blocks]")
-    F = free_pages.numel() if isinstance(free_pages, torch.Tensor) else -1
-    _ints(free_pages, "free_pages", dev, (F,))
+    _vector(cached_lens, "cached_lens", torch.int32, dev, B)
+    _vector(new_lens, "new_lens", torch.int32, dev, B)
+    W = _table(block_tables, dev, B)[1]
+    F = _tensor(free_pages, "free_pages", torch.int32, dev).numel()
+    _vector(free_pages, "free_pages", torch.int32, dev, F)
     if out is None:
+        slots = torch.empty(total_new, dtype=torch.int64, device=dev)
         ints = torch.empty(3 * B + 4, dtype=torch.int32, device=dev)
-        out = PagePlan(torch.empty(total_new, dtype=torch.int64, device=dev), ints[:B], ints[B:2 * B + 1],
-                       ints[2 * B + 1:3 * B + 2], ints[3 * B + 2:])
+        seq_lens, cu_new, cu_seqlens, counts = ints.split_with_sizes((B, B + 1, B + 1, 2))
+        out = PagePlan(slots, seq_lens, cu_new, cu_seqlens, counts)
     else:
-        _tensor(out.slots, "out.slots", torch.int64, dev)
-        _need(out.slots.shape == (total_new,) and out.slots.is_contiguous(), f"out.slots must be [{total_new}]")
-        _ints(out.seq_lens, "out.seq_lens", dev, (B,))
-        _ints(out.cu_new, "out.cu_new", dev, (B + 1,))
-        _ints(out.cu_seqlens, "out.cu_seqlens", dev, (B + 1,))
-        _ints(out.counts, "out.counts", dev, (2,))
-    with _on(dev) as stream:
-        check(lib().kq_page_plan(cached_lens.data_ptr(), new_lens.data_ptr(), B, block_tables.data_ptr(),
-                                 block_tables.shape[1], free_pages.data_ptr(), F, page_size, total_new,
-                                 out.slots.data_ptr(), out.seq_lens.data_ptr(), out.cu_new.data_ptr(),
-                                 out.cu_seqlens.data_ptr(), out.counts.data_ptr(), stream), "kq_page_plan")
+        slots, seq_lens, cu_new, cu_seqlens, counts = out
+        _vector(slots, "out.slots", torch.int64, dev, total_new)
+        _vector(seq_lens, "out.seq_lens", torch.int32, dev, B)
+        _vector(cu_new, "out.cu_new", torch.int32, dev, B + 1)
+        _vector(cu_seqlens, "out.cu_seqlens", torch.int32, dev, B + 1)
+        _vector(counts, "out.counts", torch.int32, dev, 2)
+    _call("kq_page_plan", dev, cached_lens.data_ptr(), new_lens.data_ptr(), B, block_tables.data_ptr(), W,
+          free_pages.data_ptr(), F, page_size, total_new, slots.data_ptr(), seq_lens.data_ptr(), cu_new.data_ptr(),
+          cu_seqlens.data_ptr(), counts.data_ptr())
     return out
 
 
@@ -146,17 +144,16 @@ def page_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: t
     into the q8_0 cache rows slots[t] (int64; rows with a negative slot, or one
     past the cache, are skipped)."""
     dt = _float16(k, "k")
-    dev = _rows(k, "k", k.dtype).device
-    _rows(v, "v", k.dtype, dev)
-    pages, ps, hkv, d = _caches(k_cache, v_cache, dev)
-    T = k.shape[0]
-    _need(k.shape == v.shape and k.shape[1:] == (hkv, d), f"k and v must be [T, {hkv}, {d}], got {list(k.shape)} and {list(v.shape)}")
-    _tensor(slots, "slots", torch.int64, dev)
-    _need(slots.shape == (T,) and slots.is_contiguous(), f"slots must be contiguous [{T}]")
-    with _on(dev) as stream:
-        check(lib().kq_page_write_q8_0(dt, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
-                                       v.stride(1), slots.data_ptr(), T, hkv, d, k_cache.data_ptr(),
-                                       v_cache.data_ptr(), pages * ps, stream), "kq_page_write_q8_0")
+    shape = _rows(k, "k", k.dtype)
+    dev = k.device
+    pages, ps, hkv, nb, _ = _caches(k_cache, v_cache, dev)
+    T, h, d = shape
+    if _rows(v, "v", k.dtype, dev) != shape or h != hkv or d != nb * 32:
+        raise ValueError(f"k and v must be [T, {hkv}, {nb * 32}], got {list(shape)} and {list(v.shape)}")
+    _vector(slots, "slots", torch.int64, dev, T)
+    ks, vs = k.stride(), v.stride()
+    _call("kq_page_write_q8_0", dev, dt, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), T, hkv,
+          d, k_cache.data_ptr(), v_cache.data_ptr(), pages * ps)
 
 
 def page_read(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -164,20 +161,27 @@ def page_read(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.
     """The sequences' cache rows in packed order: k, v [total_rows, Hkv, D] of
     ``dtype``, row cu_seqlens[b] + i being token i of sequence b. For the
     prompt attention of a chunk that follows cached tokens."""
-    _need(dtype in DTYPES, f"dtype must be float16 or bfloat16, got {dtype}")
+    dt = DTYPES.get(dtype)
+    if dt is None:
+        raise ValueError(f"dtype must be float16 or bfloat16, got {dtype}")
     dev = _tensor(k_cache, "k_cache", torch.uint8).device
-    pages, ps, hkv, d = _caches(k_cache, v_cache, dev)
-    _tensor(block_tables, "block_tables", torch.int32, dev)
-    _need(block_tables.dim() == 2 and block_tables.is_contiguous(), "block_tables must be contiguous [B, max_blocks]")
-    B = block_tables.shape[0]
-    _ints(cu_seqlens, "cu_seqlens", dev, (B + 1,))
-    k = torch.empty((total_rows, hkv, d), dtype=dtype, device=dev)
+    pages, ps, hkv, nb, _ = _caches(k_cache, v_cache, dev)
+    B, W = _table(block_tables, dev, None)
+    _vector(cu_seqlens, "cu_seqlens", torch.int32, dev, B + 1)
+    k = torch.empty((total_rows, hkv, nb * 32), dtype=dtype, device=dev)
     v = torch.empty_like(k)
-    with _on(dev) as stream:
-        check(lib().kq_page_read_q8_0(DTYPES[dtype], k_cache.data_ptr(), v_cache.data_ptr(), pages, ps, hkv, d,
-                                      block_tables.data_ptr(), block_tables.shape[1], cu_seqlens.data_ptr(), B,
-                                      total_rows, k.data_ptr(), v.data_ptr(), stream), "kq_page_read_q8_0")
+    _call("kq_page_read_q8_0", dev, dt, k_cache.data_ptr(), v_cache.data_ptr(), pages, ps, hkv, nb * 32,
+          block_tables.data_ptr(), W, cu_seqlens.data_ptr(), B, total_rows, k.data_ptr(), v.data_ptr())
     return k, v
+
+
+def _out_like(q: torch.Tensor, out) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _tensor(out, "out", q.dtype, q.device)
+    if out.shape != q.shape or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {list(q.shape)}, got {list(out.shape)}")
+    return out
 
 
 def _workspace(nbytes: int, device) -> tuple[torch.Tensor | None, int]:
@@ -187,14 +191,6 @@ def _workspace(nbytes: int, device) -> tuple[torch.Tensor | None, int]:
         return None, 0
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     return ws, ws.data_ptr()
-
-
-def _out_like(q: torch.Tensor, out) -> torch.Tensor:
-    if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _tensor(out, "out", q.dtype, q.device)
-    _need(out.shape == q.shape and out.is_contiguous(), f"out must be contiguous {list(q.shape)}")
-    return out
 
 
 def flash_prompt_ragged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
@@ -207,32 +203,29 @@ def flash_prompt_ragged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_se
     of a sequence sees keys up to i + (len_k - len_q), so a chunk sees the
     context before it; a row without keys is zero."""
     dt = _float16(q, "q")
-    dev = _rows(q, "q", q.dtype).device
-    _rows(k, "k", q.dtype, dev)
-    _rows(v, "v", q.dtype, dev)
-    Tq, Hq, D = q.shape
-    Tk, Hkv = k.shape[0], k.shape[1]
-    _need(k.shape == v.shape and k.shape[2] == D, f"k and v must be [Tk, Hkv, {D}], got {list(k.shape)} and {list(v.shape)}")
-    _tensor(cu_seqlens_q, "cu_seqlens_q", torch.int32, dev)
-    B = cu_seqlens_q.numel() - 1
-    _need(B >= 0, "cu_seqlens_q must be [B + 1]")
-    _ints(cu_seqlens_q, "cu_seqlens_q", dev, (B + 1,))
-    if cu_seqlens_k is None:
-        _need(Tq == Tk, f"cu_seqlens_k is needed where q has {Tq} rows and k {Tk}")
+    Tq, Hq, D = _rows(q, "q", q.dtype)
+    dev = q.device
+    kshape = _rows(k, "k", q.dtype, dev)
+    Tk, Hkv, Dk = kshape
+    if _rows(v, "v", q.dtype, dev) != kshape or Dk != D:
+        raise ValueError(f"k and v must be [Tk, Hkv, {D}], got {list(kshape)} and {list(v.shape)}")
+    B = _tensor(cu_seqlens_q, "cu_seqlens_q", torch.int32, dev).numel() - 1
+    _vector(cu_seqlens_q, "cu_seqlens_q", torch.int32, dev, max(B, 0) + 1)
+    if cu_seqlens_k is not None:
+        _vector(cu_seqlens_k, "cu_seqlens_k", torch.int32, dev, B + 1)
+    elif Tq == Tk:
         cu_seqlens_k = cu_seqlens_q
     else:
-        _ints(cu_seqlens_k, "cu_seqlens_k", dev, (B + 1,))
+        raise ValueError(f"cu_seqlens_k is needed where q has {Tq} rows and k {Tk}")
     if scale is None:
-        scale = 1.0 / math.sqrt(D)
+        scale = D ** -0.5
     out = _out_like(q, out)
-    L = lib()
-    nbytes = L.kq_fa_prompt_workspace(B, Tq, Tk, Hq, Hkv, D)
-    with _on(dev) as stream:
-        ws, ptr = _workspace(nbytes, dev)
-        check(L.kq_fa_prompt(dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0),
-                             k.stride(1), v.stride(0), v.stride(1), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
-                             B, Tq, Tk, Hq, Hkv, D, int(causal), ctypes.c_float(scale), out.data_ptr(), ptr, nbytes,
-                             stream), "kq_fa_prompt")
+    nbytes = lib().kq_fa_prompt_workspace(B, Tq, Tk, Hq, Hkv, D)
+    ws, ptr = _workspace(nbytes, dev)
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    _call("kq_fa_prompt", dev, dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
+          cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), B, Tq, Tk, Hq, Hkv, D, int(causal), scale, out.data_ptr(),
+          ptr, nbytes)
     return out
 
 
@@ -247,26 +240,22 @@ def flash_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     bounds seq_lens, longer sequences are cut to it; it defaults to the
     tables' width."""
     dt = _float16(q, "q")
-    dev = _rows(q, "q", q.dtype).device
-    _need(q.is_contiguous(), "q must be contiguous")
-    pages, ps, hkv, d = _caches(k_cache, v_cache, dev)
-    B, Hq, D = q.shape
-    _need(D == d, f"q has head dimension {D}, the caches {d}")
-    _tensor(block_tables, "block_tables", torch.int32, dev)
-    _need(block_tables.dim() == 2 and block_tables.shape[0] == B and block_tables.is_contiguous(),
-          f"block_tables must be contiguous [{B}, max_blocks]")
-    _ints(seq_lens, "seq_lens", dev, (B,))
-    W = block_tables.shape[1]
+    B, Hq, D = _rows(q, "q", q.dtype)
+    dev = q.device
+    if not q.is_contiguous():
+        raise ValueError("q must be contiguous")
+    pages, ps, hkv, nb, _ = _caches(k_cache, v_cache, dev)
+    if D != nb * 32:
+        raise ValueError(f"q has head dimension {D}, the caches {nb * 32}")
+    W = _table(block_tables, dev, B)[1]
+    _vector(seq_lens, "seq_lens", torch.int32, dev, B)
     max_seqlen = W * ps if max_seqlen is None else min(int(max_seqlen), W * ps)
     if scale is None:
-        scale = 1.0 / math.sqrt(D)
+        scale = D ** -0.5
     out = _out_like(q, out)
-    L = lib()
-    nbytes = L.kq_fa_decode_paged_workspace(B, Hq, hkv, D, prefix_len, max_seqlen)
-    with _on(dev) as stream:
-        ws, ptr = _workspace(nbytes, dev)
-        check(L.kq_fa_decode_paged(dt, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages, ps,
-                                   block_tables.data_ptr(), W, seq_lens.data_ptr(), B, Hq, hkv, D, prefix_len,
-                                   max_seqlen, ctypes.c_float(scale), out.data_ptr(), ptr, nbytes, stream),
-              "kq_fa_decode_paged")
+    nbytes = lib().kq_fa_decode_paged_workspace(B, Hq, hkv, D, prefix_len, max_seqlen)
+    ws, ptr = _workspace(nbytes, dev)
+    _call("kq_fa_decode_paged", dev, dt, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages, ps,
+          block_tables.data_ptr(), W, seq_lens.data_ptr(), B, Hq, hkv, D, prefix_len, max_seqlen, scale, out.data_ptr(),
+          ptr, nbytes)
     return out
