@@ -112,47 +112,58 @@ __global__ void __launch_bounds__(kSimpleWarps * 32) fa_prompt_simple_kernel(con
 }
 
 // ---- tensor cores: D <= 128, rows TMA can address -------------------------------
-// One CTA takes up to two query tiles of one KV head. A tile is 128 rows: TQ =
-// 128 / G tokens x the G query heads that share the KV head (row = token * G +
-// g), so K and V are read once per group and short prompts fill the tile.
-// Keys come in blocks of 128. Per block and tile:
+// A CTA takes TILES query tiles of one KV head. A tile is 128 rows: TQ = 128 / G
+// tokens x the G query heads that share the KV head (row = token * G + g), so K
+// and V are read once per group and short prompts fill the tile. Keys come in
+// blocks of 64. Per block and tile:
 //   S = Q K^T   tcgen05, Q and K in shared memory, S fp32 in TMEM
 //   P = 2^(S sl - m + kBias)   one thread per row (TMEM lane), P to TMEM over S
 //   O += P V    tcgen05, P from TMEM, V in shared memory, O fp32 in TMEM
-// The two tiles alternate: while the softmax warps of one work, the tensor
-// core runs the other's two products. The running maximum m only moves when a
-// row's maximum grows by more than 2^kLazy (then O is rescaled in TMEM): p
-// stays below 2^(kBias + kLazy), inside fp16, and the factor cancels in O / l.
-// P is rounded to the inputs' type, as the product with V needs both operands
-// in it; l sums the unrounded p in fp32.
+// S has two buffers per tile: the product for block j + 1 runs while the
+// softmax warps work on block j, so they never wait in steady state; 64-key
+// blocks make room for that in TMEM (4 x 64 columns of S, 2 x 128 of O).
+// The running maximum m only moves when a row's maximum grows by more than
+// 2^kLazy (then O is rescaled in TMEM): p stays below 2^(kBias + kLazy), inside
+// fp16, and the factor cancels in O / l. P is rounded to the inputs' type, as
+// the product with V needs both operands in it; l sums the unrounded p in fp32.
 //
-// Warps: 0-3 softmax of tile 0, 4-7 of tile 1 (warp w reaches TMEM lanes
-// 32 (w % 4) ..), 8 MMA issue and TMEM, 9 TMA.
-constexpr int kTile = 128;            // rows of a query tile, keys of a block
-constexpr int kTcThreads = 320;
-constexpr int kMmaWarp = 8, kLoadWarp = 9;
+// What bounds it: per 256 rows x 128 keys the tensor core needs 2048 clocks
+// and the special-function unit, at 16 exponentials per clock, another 2048;
+// kPoly of every 64 exponentials therefore run as a polynomial on the FMA pipe.
+//
+// TILES = 2: one CTA per SM, K and V read once for 256 rows. TILES = 1: two
+// CTAs per SM, each hiding the other's start and end; for short sequences.
+// Warps: 4 softmax warps per tile (warp w reaches TMEM lanes 32 (w % 4) ..),
+// one that issues MMAs, one that issues TMA.
+constexpr int kTile = 128;            // rows of a query tile
+constexpr int kBlk = 64;              // keys of a block
 constexpr float kBias = 7.0f, kLazy = 8.0f;
+constexpr int kPoly = 16;             // exponentials of each 64 on the FMA pipe
 
-template <int DP>
+template <int DP, int TILES>
 struct TcTraits {
-  static constexpr int PANELS = DP / 64;           // 128-byte swizzled panels of 64 dims
-  static constexpr int PANEL = kTile * 128;        // bytes
-  static constexpr int OPERAND = PANELS * PANEL;   // a Q tile, K block or V block
-  static constexpr int STAGES = DP == 128 ? 5 : 10;  // K and V blocks in flight (alternating)
-  static constexpr int OFF_Q = 0;
-  static constexpr int OFF_KV = 2 * OPERAND;
+  static constexpr int THREADS = TILES * 128 + 64;
+  static constexpr int PANELS = DP / 64;            // 128-byte swizzled panels of 64 dims
+  static constexpr int QPANEL = kTile * 128, PANEL = kBlk * 128;
+  static constexpr int QTILE = PANELS * QPANEL, OPERAND = PANELS * PANEL;
+  static constexpr int STAGES = (TILES == 2 ? 10 : 5) * (128 / DP);  // K and V blocks in flight
+  static constexpr int OFF_KV = TILES * QTILE;
   static constexpr int OFF_BAR = OFF_KV + STAGES * OPERAND;
-  static constexpr int SMEM = OFF_BAR + 256 + 1024;
+  static constexpr int SMEM = OFF_BAR + 512;
+  static constexpr int COLS = TILES * 256;          // TMEM columns: S buffers, then O
+  static_assert((2 * STAGES + 6 * TILES) * 8 + 4 <= 512, "barrier area");
+  static_assert(2 * (SMEM + 1024) <= 233472 || TILES == 2, "two CTAs per SM");
   static_assert(SMEM <= 232448, "shared memory budget");
 };
-constexpr uint32_t kColS = 0, kColO = 256;         // TMEM: S0 S1 | O0 O1 (O tiles DP columns apart)
 
 struct TcArgs {
   const int32_t *cu_q, *cu_k;
-  int B, Tq, Hq, Hkv, G, TQ, D, causal, tiles, slots;
+  int B, Tq, Hq, Hkv, G, TQ, D, causal, slots, splits;
   float sl;             // scale * log2(e), not negative
   uint32_t flip;        // sign bit where scale < 0: scores are negated first
   void* out;
+  float* part;          // splits > 1: [split][Tq * Hq][D] unnormalised outputs
+  float2* ml;           //             [split][Tq * Hq] maximum (log2 units), sum
   int* err;
 };
 
@@ -174,6 +185,62 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+// Two fp32 lanes per instruction.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack(F2 a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+// 2^x for x <= 126 (below -126 as at -126): x = i + f with i the nearest
+// integer, 2^f by the degree-4 polynomial of smallest relative error on
+// [-1/2, 1/2] (2.6e-6, from a Remez iteration), times 2^i built in the
+// exponent field. A product, not an integer addition to the exponent, so that
+// NaN stays NaN.
+__device__ __forceinline__ F2 exp2_poly(F2 x2) {
+  float x, y;
+  unpack(x2, x, y);
+  x2 = f2(max_nan(x, -126.0f), max_nan(y, -126.0f));
+  const F2 t = add2(x2, f2(12582912.0f, 12582912.0f));  // 1.5 * 2^23: i in the low bits
+  const F2 i = add2(t, f2(-12582912.0f, -12582912.0f));
+  const F2 f = fma2(i, f2(-1.0f, -1.0f), x2);
+  F2 p = fma2(f, f2(0.009570102207362652f, 0.009570102207362652f), f2(0.05591785907745361f, 0.05591785907745361f));
+  p = fma2(p, f, f2(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f, f2(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(p, f, f2(0.9999992847442627f, 0.9999992847442627f));
+  float tx, ty;
+  unpack(t, tx, ty);
+  return mul2(p, f2(__uint_as_float((__float_as_uint(tx) << 23) + 0x3f800000u),
+                    __uint_as_float((__float_as_uint(ty) << 23) + 0x3f800000u)));
+}
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
@@ -182,6 +249,7 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
+
 // Instruction descriptor, kind::f16: fp32 D, A and B of type T, M = 128; bit 16: B is MN-major.
 template <typename T>
 __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
@@ -196,8 +264,7 @@ struct Work {
 // Slot -> (sequence, tile): sequence b owns slots cu_q[b] / TT + b .., at
 // least ceil(len / TT) of them, so no prefix sum over tiles is needed; slots
 // past a sequence's end are empty (at most one or two per sequence).
-__device__ __forceinline__ bool find_work(const TcArgs& a, int slot, Work& w) {
-  const int tt = a.TQ * a.tiles;
+__device__ __forceinline__ bool find_work(const TcArgs& a, int tt, int slot, Work& w) {
   int lo = 0, hi = a.B;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -218,37 +285,43 @@ __device__ __forceinline__ int keys_of(const TcArgs& a, const Work& w, int i) {
 // Key blocks of tile t (0 when it has no token or sees no key).
 __device__ __forceinline__ int blocks_of(const TcArgs& a, const Work& w, int t) {
   const int first = w.tok + t * a.TQ;
-  if (t >= a.tiles || first >= w.lq) return 0;
-  return (keys_of(a, w, min(w.lq, first + a.TQ) - 1) + kTile - 1) / kTile;
+  if (first >= w.lq) return 0;
+  return (keys_of(a, w, min(w.lq, first + a.TQ) - 1) + kBlk - 1) / kBlk;
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kTcThreads, 1)
+template <typename T, int DP, int TILES>
+__global__ void __launch_bounds__(TILES * 128 + 64, TILES == 2 ? 1 : 2)
     fa_prompt_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcArgs a) {
-  using R = TcTraits<DP>;
-  constexpr int STAGES = R::STAGES;
+  using R = TcTraits<DP, TILES>;
+  constexpr int STAGES = R::STAGES, kMmaWarp = TILES * 4, kLoadWarp = kMmaWarp + 1;
+  constexpr uint32_t kColO = TILES * 2 * kBlk;       // S of tile t, buffer x at (2 t + x) * kBlk
   const int head = blockIdx.x % a.Hkv;
   Work w;
   // later tiles of a causal sequence see more keys: they start first
-  if (!find_work(a, a.slots - 1 - blockIdx.x / a.Hkv, w)) return;
+  if (!find_work(a, a.TQ * TILES, a.slots - 1 - blockIdx.x / a.Hkv, w)) return;
 
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + R::OFF_BAR);
-  uint64_t* kv_full = q_full + 2;
+  uint64_t* kv_full = q_full + TILES;
   uint64_t* kv_empty = kv_full + STAGES;
-  uint64_t* s_full = kv_empty + STAGES;   // S of a tile is there (and its earlier P V is done)
-  uint64_t* p_full = s_full + 2;          // P of a tile is there, its S is read
-  uint64_t* o_full = p_full + 2;          // the tile's last P V is done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint64_t* s_full = kv_empty + STAGES;   // [tile][buffer]: S is there
+  uint64_t* p_full = s_full + 2 * TILES;  // P of a tile is there
+  uint64_t* pv_done = p_full + TILES;     // the tile's latest P V is done
+  uint64_t* o_full = pv_done + TILES;     // the tile's last P V is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + TILES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
+  if (smem_u32(smem) & 1023u) {  // swizzled tiles need it
+    if (threadIdx.x == 0) record_error(a.err, DEV_BAD_SHAPE);
+    return;
+  }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < TILES; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&s_full[i], 1);
+      mbar_init(&s_full[2 * i], 1);
+      mbar_init(&s_full[2 * i + 1], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
       mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < STAGES; ++i) {
@@ -258,17 +331,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     fence_mbar_init();
   }
   // rows of a query tile that no token fills stay zero
-  for (int i = threadIdx.x; i < 2 * R::PANELS * (kTile - a.TQ * a.G) * 8; i += kTcThreads) {
+  for (int i = threadIdx.x; i < TILES * R::PANELS * (kTile - a.TQ * a.G) * 8; i += R::THREADS) {
     const int rows = kTile - a.TQ * a.G, c = i % 8, r = i / 8 % rows, panel = i / 8 / rows;
-    *reinterpret_cast<uint4*>(smem + R::OFF_Q + panel * R::PANEL + (a.TQ * a.G + r) * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(smem + panel * R::QPANEL + (a.TQ * a.G + r) * 128 + c * 16) = make_uint4(0, 0, 0, 0);
   }
   fence_proxy_async_smem();
-  if (warp == kMmaWarp) tc::tmem_alloc(tmem_slot, 512);
+  if (warp == kMmaWarp) tc::tmem_alloc(tmem_slot, R::COLS);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int n0 = blocks_of(a, w, 0), n1 = blocks_of(a, w, 1), n = max(n0, n1);
+  // this split's range of key blocks, and its share of every tile
+  int cnt[TILES], n = 0;
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) cnt[t] = blocks_of(a, w, t), n = max(n, cnt[t]);
+  const int j0 = (int)((long long)n * blockIdx.y / a.splits), j1 = (int)((long long)n * (blockIdx.y + 1) / a.splits);
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) cnt[t] = max(0, min(cnt[t], j1) - j0);
+  n = j1 - j0;
+  // K and V blocks in the order they are used: K0 K1 V0 K2 V1 .. V(n - 1)
+  auto item_k = [&](int i) { return i == 0 ? 0 : 2 * i - 1; };
+  auto item_v = [&](int i) { return i + 1 == n ? 2 * i + 1 : 2 * i + 2; };
   bool dead = false;
 
   if (warp == kLoadWarp) {
@@ -276,103 +359,110 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc::prefetch_tmap(&map_q);
       tc::prefetch_tmap(&map_k);
       tc::prefetch_tmap(&map_v);
-      for (int t = 0; t < 2; ++t) {
-        if ((t ? n1 : n0) == 0) continue;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        if (cnt[t] == 0) continue;
         mbar_arrive_expect_tx(&q_full[t], R::PANELS * a.TQ * a.G * 128);
         for (int p = 0; p < R::PANELS; ++p)
-          tma_load_3d(smem + R::OFF_Q + t * R::OPERAND + p * R::PANEL, &map_q, p * 64, head * a.G,
-                      w.q0 + w.tok + t * a.TQ, &q_full[t]);
+          tma_load_3d(smem + t * R::QTILE + p * R::QPANEL, &map_q, p * 64, head * a.G, w.q0 + w.tok + t * a.TQ, &q_full[t]);
       }
-      for (int i = 0; i < 2 * n; ++i) {  // K0 V0 K1 V1 ..
-        const int st = i % STAGES;
-        if (i >= STAGES) mbar_wait_idle_or_poison(&kv_empty[st], ((i / STAGES) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
+      for (int x = 0; x < 2 * n; ++x) {
+        const bool is_v = x > 0 && ((x & 1) == 0 || x + 1 == 2 * n);
+        const int i = x == 0 ? 0 : is_v ? (x + 1 == 2 * n ? n - 1 : (x - 2) >> 1) : (x + 1) >> 1;
+        const int st = x % STAGES;
+        if (x >= STAGES) mbar_wait_idle_or_poison(&kv_empty[st], ((x / STAGES) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
         mbar_arrive_expect_tx(&kv_full[st], R::OPERAND);
         for (int p = 0; p < R::PANELS; ++p)
-          tma_load_3d(smem + R::OFF_KV + st * R::OPERAND + p * R::PANEL, (i & 1) ? &map_v : &map_k, p * 64, head,
-                      w.k0 + (i >> 1) * kTile, &kv_full[st]);
+          tma_load_3d(smem + R::OFF_KV + st * R::OPERAND + p * R::PANEL, is_v ? &map_v : &map_k, p * 64, head,
+                      w.k0 + (j0 + i) * kBlk, &kv_full[st]);
       }
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    constexpr uint32_t idesc_s = idesc<T>(kTile, false), idesc_o = idesc<T>(DP, true);
-    const uint32_t q_base = smem_u32(smem + R::OFF_Q), kv_base = smem_u32(smem + R::OFF_KV);
+    constexpr uint32_t idesc_s = idesc<T>(kBlk, false), idesc_o = idesc<T>(DP, true);
+    const uint32_t q_base = smem_u32(smem), kv_base = q_base + R::OFF_KV;
     const uint32_t go = tc::elect_one();
-    // S_t = Q_t K_j^T
-    auto score = [&](int t, int j) {
-      const int st = 2 * j % STAGES;
-      mbar_wait_or_poison(&kv_full[st], (2 * j / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+    // S_t = Q_t K_i^T into buffer i & 1
+    auto scores = [&](int i) {
+      const int st = item_k(i) % STAGES;
+      mbar_wait_or_poison(&kv_full[st], (item_k(i) / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
       tc::tc_fence_after();
-      const uint64_t qd = tc::sw128_desc(q_base + t * R::OPERAND), kd = tc::sw128_desc(kv_base + st * R::OPERAND);
+      const uint64_t kd = tc::sw128_desc(kv_base + st * R::OPERAND);
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        const uint64_t off = (uint64_t)((k >> 2) * (R::PANEL >> 4) + (k & 3) * 2);
-        tc::mma_ss_go(tmem + kColS + t * kTile, qd + off, kd + off, idesc_s, k > 0, go);
+      for (int t = 0; t < TILES; ++t) {
+        if (i >= cnt[t]) continue;
+        if (i == 0) {
+          mbar_wait_or_poison(&q_full[t], 0, a.err, DEV_TIMEOUT_FULL, dead);
+          tc::tc_fence_after();
+        }
+        const uint64_t qd = tc::sw128_desc(q_base + t * R::QTILE);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+          tc::mma_ss_go(tmem + (2 * t + (i & 1)) * kBlk, qd + (uint64_t)((k >> 2) * (R::QPANEL >> 4) + (k & 3) * 2),
+                        kd + (uint64_t)((k >> 2) * (R::PANEL >> 4) + (k & 3) * 2), idesc_s, k > 0, go);
+        tc::mma_commit_go(&s_full[2 * t + (i & 1)], go);
       }
-      tc::mma_commit_go(&s_full[t], go);
+      tc::mma_commit_go(&kv_empty[st], go);
     };
-    for (int t = 0; t < 2; ++t)
-      if ((t ? n1 : n0) > 0) {
-        mbar_wait_or_poison(&q_full[t], 0, a.err, DEV_TIMEOUT_FULL, dead);
-        score(t, 0);
-      }
-    if (n > 0) tc::mma_commit_go(&kv_empty[0], go);
-    for (int j = 0; j < n; ++j) {
-      const int sv = (2 * j + 1) % STAGES;
-#pragma unroll 1
-      for (int t = 0; t < 2; ++t) {
-        const int nt = t ? n1 : n0;
-        if (j >= nt) continue;
-        mbar_wait_or_poison(&kv_full[sv], ((2 * j + 1) / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
-        mbar_wait_or_poison(&p_full[t], j & 1, a.err, DEV_TIMEOUT_FULL, dead);
-        tc::tc_fence_after();
-        const uint64_t vd = tc::sw128_desc_mn(kv_base + sv * R::OPERAND, R::PANEL);  // dims across, tokens down
+    if (n > 0) scores(0);
+    for (int i = 0; i < n; ++i) {
+      // buffer (i + 1) & 1 held P of block i - 1, whose product was issued before
+      if (i + 1 < n) scores(i + 1);
+      const int st = item_v(i) % STAGES;
+      mbar_wait_or_poison(&kv_full[st], (item_v(i) / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+      const uint64_t vd = tc::sw128_desc_mn(kv_base + st * R::OPERAND, R::PANEL);  // dims across, tokens down
 #pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          tc::mma_ts_go(tmem + kColO + t * DP, tmem + kColS + t * kTile + 8 * k, vd + (uint64_t)(k * (2048 >> 4)), idesc_o,
-                        (j > 0 || k > 0) ? 1u : 0u, go);
-        if (j + 1 == nt) tc::mma_commit_go(&o_full[t], go);
-        if (j + 1 < nt) score(t, j + 1);
+      for (int t = 0; t < TILES; ++t) {
+        if (i >= cnt[t]) continue;
+        mbar_wait_or_poison(&p_full[t], i & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        tc::tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < kBlk / 16; ++k)
+          tc::mma_ts_go(tmem + kColO + t * DP, tmem + (2 * t + (i & 1)) * kBlk + 8 * k, vd + (uint64_t)(k * (2048 >> 4)),
+                        idesc_o, (i > 0 || k > 0) ? 1u : 0u, go);
+        tc::mma_commit_go(i + 1 == cnt[t] ? &o_full[t] : &pv_done[t], go);
       }
-      tc::mma_commit_go(&kv_empty[sv], go);
-      if (j + 1 < n) tc::mma_commit_go(&kv_empty[(2 * j + 2) % STAGES], go);
+      tc::mma_commit_go(&kv_empty[st], go);
     }
     __syncwarp();
   } else {
-    const int t = warp >> 2, row = threadIdx.x & 127, nt = t ? n1 : n0;
+    const int t = warp >> 2, row = threadIdx.x & 127, nt = cnt[TILES == 2 ? t : 0];
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + kColS + t * kTile, o_addr = tmem + lanes + kColO + t * DP;
+    const uint32_t s_addr = tmem + lanes + 2 * t * kBlk, o_addr = tmem + lanes + kColO + t * DP;
     const int first = w.tok + t * a.TQ;                     // the tile's first token
     const int tok = first + row / a.G, g = row % a.G;
-    const bool mine = row < a.TQ * a.G && t < a.tiles && tok < w.lq;
+    const bool mine = row < a.TQ * a.G && tok < w.lq;
     const int keys = mine ? keys_of(a, w, tok) : 0;
     const int all_see = keys_of(a, w, first);               // keys that every row of the tile sees
-    float m = -INFINITY, l = 0.0f;
-    for (int j = 0; j < nt; ++j) {
-      mbar_wait_or_poison(&s_full[t], j & 1, a.err, DEV_TIMEOUT_FULL, dead);
+    float m = -INFINITY;
+    F2 l2 = f2(0.0f, 0.0f);
+    for (int i = 0; i < nt; ++i) {
+      const int key0 = (j0 + i) * kBlk;
+      mbar_wait_or_poison(&s_full[2 * t + (i & 1)], (i >> 1) & 1, a.err, DEV_TIMEOUT_FULL, dead);
       __syncwarp();
       tc::tc_fence_after();
-      uint32_t s[kTile];
-#pragma unroll
-      for (int c = 0; c < kTile / 32; ++c) tc::tmem_ld32(s_addr + 32 * c, reinterpret_cast<uint32_t(&)[32]>(s[32 * c]));
+      uint32_t s[kBlk];
+      tc::tmem_ld32(s_addr + (i & 1) * kBlk, reinterpret_cast<uint32_t(&)[32]>(s[0]));
+      tc::tmem_ld32(s_addr + (i & 1) * kBlk + 32, reinterpret_cast<uint32_t(&)[32]>(s[32]));
       tc::tmem_ld_wait();
       if (a.flip) {
 #pragma unroll
-        for (int i = 0; i < kTile; ++i) s[i] ^= a.flip;
+        for (int x = 0; x < kBlk; ++x) s[x] ^= a.flip;
       }
-      if ((j + 1) * kTile > all_see) {
-        const int lim = keys - j * kTile;
+      if (key0 + kBlk > all_see) {
+        const int lim = keys - key0;
 #pragma unroll
-        for (int i = 0; i < kTile; ++i)
-          if (i >= lim) s[i] = 0xff800000u;
-        const int valid = w.lk - j * kTile;
-        if (valid < kTile) {
+        for (int x = 0; x < kBlk; ++x)
+          if (x >= lim) s[x] = 0xff800000u;
+        const int valid = w.lk - key0;
+        if (valid < kBlk) {
           // rows of V behind the sequence's end belong to others: what they
           // hold must not meet P (0 x inf); both tiles write the same zeros
-          const int sv = (2 * j + 1) % STAGES;
-          mbar_wait_or_poison(&kv_full[sv], ((2 * j + 1) / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
-          for (int i = row; i < (kTile - valid) * 8 * R::PANELS; i += kTile) {
-            const int c = i % 8, p = i / 8 % R::PANELS, r = valid + i / (8 * R::PANELS);
-            *reinterpret_cast<uint4*>(smem + R::OFF_KV + sv * R::OPERAND + p * R::PANEL + r * 128 + c * 16) =
+          const int st = item_v(i) % STAGES;
+          mbar_wait_or_poison(&kv_full[st], (item_v(i) / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+          for (int x = row; x < (kBlk - valid) * 8 * R::PANELS; x += kTile) {
+            const int c = x % 8, p = x / 8 % R::PANELS, r = valid + x / (8 * R::PANELS);
+            *reinterpret_cast<uint4*>(smem + R::OFF_KV + st * R::OPERAND + p * R::PANEL + r * 128 + c * 16) =
                 make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
@@ -380,82 +470,149 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       float mx[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(s[i]);
+      for (int x = 0; x < 4; ++x) mx[x] = __uint_as_float(s[x]);
 #pragma unroll
-      for (int i = 4; i < kTile; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
-      const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl;
+      for (int x = 4; x < kBlk; x += 8)
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if (x + y + 4 < kBlk) mx[y] = max3(mx[y], __uint_as_float(s[x + y]), __uint_as_float(s[x + y + 4]));
+          else mx[y] = fmaxf(mx[y], __uint_as_float(s[x + y]));
+      const float mn = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * a.sl;
       float f = 1.0f;
       if (mn > m + kLazy) {  // also the row's first keys (m = -inf)
         f = ex2(m - mn);
         m = mn;
-        l *= f;
+        l2 = mul2(l2, f2(f, f));
       }
-      if (j > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
+      if (i > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
+        // the product of block i - 2 is done (S of block i came after it)
+        mbar_wait_or_poison(&pv_done[t], (i - 1) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        __syncwarp();
+        tc::tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < DP / 32; ++c) {
           uint32_t o[32];
           tc::tmem_ld32(o_addr + 32 * c, o);
           tc::tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+          for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
           tc::tmem_st32(o_addr + 32 * c, o);
         }
       }
       const float off = m == -INFINITY ? 0.0f : kBias - m;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      uint32_t p[kTile / 2];
+      const F2 sl2 = f2(a.sl, a.sl), off2 = f2(off, off);
+      F2 sum = f2(0.0f, 0.0f);
+      uint32_t p[kBlk / 2];
 #pragma unroll
-      for (int i = 0; i < kTile / 2; ++i) {
-        const float p0 = ex2(fmaf(__uint_as_float(s[2 * i]), a.sl, off));
-        const float p1 = ex2(fmaf(__uint_as_float(s[2 * i + 1]), a.sl, off));
-        sum[(2 * i) & 3] += p0;
-        sum[(2 * i + 1) & 3] += p1;
-        p[i] = pack2<T>(p0, p1);
+      for (int x = 0; x < kBlk / 2; ++x) {
+        F2 e = fma2(f2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), sl2, off2);
+        float e0, e1;
+        // the polynomial's elements are spread among the others
+        if ((x * kPoly / kBlk) != ((x + 1) * kPoly / kBlk) && kPoly > 0) {
+          e = exp2_poly(e);
+          unpack(e, e0, e1);
+        } else {
+          unpack(e, e0, e1);
+          e0 = ex2(e0), e1 = ex2(e1);
+          e = f2(e0, e1);
+        }
+        sum = add2(sum, e);
+        p[x] = pack2<T>(e0, e1);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l2 = add2(l2, sum);
       __syncwarp();
-      tc::tmem_st32(s_addr, p);
-      tc::tmem_st32(s_addr + 32, p + 32);
+      tc::tmem_st32(s_addr + (i & 1) * kBlk, p);
       tc::tmem_st_wait();
       tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[t]);
     }
-    // O / l
+    float l, l1;
+    unpack(l2, l, l1);
+    l += l1;
     if (nt > 0) {
       mbar_wait_or_poison(&o_full[t], 0, a.err, DEV_TIMEOUT_FULL, dead);
       __syncwarp();
       tc::tc_fence_after();
     }
-    T* out = static_cast<T*>(a.out) + ((long long)(w.q0 + tok) * a.Hq + head * a.G + g) * a.D;
-    const bool none = nt == 0 || l == 0.0f;
-    const float inv = 1.0f / l;
+    const bool none = m == -INFINITY && l == l;             // no key seen (a NaN score is one)
+    const long long at = (long long)(w.q0 + tok) * a.Hq + head * a.G + g;
+    if (a.splits > 1) {
+      const long long prow = (long long)blockIdx.y * a.Tq * a.Hq + at;
 #pragma unroll 1
-    for (int c = 0; c < DP / 32; ++c) {
-      uint32_t o[32];
-      __syncwarp();
-      if (nt > 0) {
-        tc::tmem_ld32(o_addr + 32 * c, o);
-        tc::tmem_ld_wait();
-      }
-      if (mine) {
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t o[32];
+        __syncwarp();
+        if (nt > 0) {
+          tc::tmem_ld32(o_addr + 32 * c, o);
+          tc::tmem_ld_wait();
+        }
+        if (mine && !none) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (!none) {
-            v.x = pack2<T>(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
-            v.y = pack2<T>(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
-            v.z = pack2<T>(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
-            v.w = pack2<T>(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
+          for (int x = 0; x < 8; ++x)
+            if (32 * c + 4 * x < a.D)
+              *reinterpret_cast<uint4*>(a.part + prow * a.D + 32 * c + 4 * x) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        }
+      }
+      if (mine) a.ml[prow] = make_float2(none ? -INFINITY : m, none ? 0.0f : l);
+    } else {
+      T* out = static_cast<T*>(a.out) + at * a.D;
+      const float inv = 1.0f / l;
+#pragma unroll 1
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t o[32];
+        __syncwarp();
+        if (nt > 0) {
+          tc::tmem_ld32(o_addr + 32 * c, o);
+          tc::tmem_ld_wait();
+        }
+        if (mine) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (!none) {
+              v.x = pack2<T>(__uint_as_float(o[8 * x]) * inv, __uint_as_float(o[8 * x + 1]) * inv);
+              v.y = pack2<T>(__uint_as_float(o[8 * x + 2]) * inv, __uint_as_float(o[8 * x + 3]) * inv);
+              v.z = pack2<T>(__uint_as_float(o[8 * x + 4]) * inv, __uint_as_float(o[8 * x + 5]) * inv);
+              v.w = pack2<T>(__uint_as_float(o[8 * x + 6]) * inv, __uint_as_float(o[8 * x + 7]) * inv);
+            }
+            if (32 * c + 8 * x < a.D) *reinterpret_cast<uint4*>(out + 32 * c + 8 * x) = v;
           }
-          if (32 * c + 8 * i < a.D) *reinterpret_cast<uint4*>(out + 32 * c + 8 * i) = v;
         }
       }
     }
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
+  if (warp == kMmaWarp) tc::tmem_dealloc(tmem, R::COLS);
+}
+
+// Merges the splits of a row: one warp per (row, query head), 4 dims per lane.
+// A split that saw none of the row's keys has l = 0 and no output.
+template <typename T>
+__global__ void __launch_bounds__(256) fa_prompt_combine_kernel(const TcArgs a) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long rows = (long long)a.Tq * a.Hq, row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const float2 s = lane < a.splits ? a.ml[lane * rows + row] : make_float2(-INFINITY, 0.0f);
+  const float M = warp_max(s.x), base = M == -INFINITY ? 0.0f : M;
+  const float wgt = s.y == 0.0f ? 0.0f : ex2(s.x - base);
+  float L = wgt * s.y;
+#pragma unroll
+  for (int x = 16; x >= 1; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int i = 0; i < a.splits; ++i) {
+    const float wi = __shfl_sync(0xffffffffu, wgt, i), li = __shfl_sync(0xffffffffu, s.y, i);
+    if (li == 0.0f || 4 * lane >= a.D) continue;
+    const float4 v = *reinterpret_cast<const float4*>(a.part + (i * rows + row) * a.D + 4 * lane);
+    o.x = fmaf(wi, v.x, o.x), o.y = fmaf(wi, v.y, o.y), o.z = fmaf(wi, v.z, o.z), o.w = fmaf(wi, v.w, o.w);
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  if (4 * lane < a.D)
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + row * a.D + 4 * lane) =
+        make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
 }
 
 // [T, H, D] rows as a 3-D map of 64-dim x `heads` x `tokens` boxes, 128-byte swizzled
@@ -482,42 +639,81 @@ bool tc_supported(const FaPromptArgs& a) {
          tma_rows(a.k, a.Hkv, a.Tk, a.k_head, a.k_row) && tma_rows(a.v, a.Hkv, a.Tk, a.v_head, a.v_row);
 }
 
-template <typename T, int DP>
-kq_status_t launch_tc(const FaPromptArgs& a, int dtype, cudaStream_t s) {
+// How a call is cut up.
+struct Plan {
+  int tiles, slots, splits;  // query tiles per CTA, CTAs per KV head, key splits
+};
+constexpr int kMaxSplits = 32;
+Plan plan_of(const FaPromptArgs& a) {
+  const int TQ = kTile / (a.Hq / a.Hkv);
+  const long long keys = a.Tk / std::max(a.B, 1);  // per sequence, on average
+  Plan p;
+  p.tiles = keys >= 1024 ? 2 : 1;
+  p.slots = a.Tq / (TQ * p.tiles) + a.B;
+  // few CTAs against many keys: split the keys so that the SMs are full once,
+  // with at least 512 keys each
+  const long long ctas = ((a.Tq + (long long)TQ * p.tiles - 1) / (TQ * p.tiles)) * a.Hkv;
+  const long long room = (long long)sm_count() * (p.tiles == 2 ? 1 : 2);
+  p.splits = (int)std::max(1ll, std::min({room / std::max(ctas, 1ll), keys / 512, (long long)kMaxSplits}));
+  return p;
+}
+
+template <typename T, int DP, int TILES>
+kq_status_t launch_tc(const FaPromptArgs& a, int dtype, const Plan& plan, cudaStream_t s) {
+  using R = TcTraits<DP, TILES>;
   TcArgs p{};
   p.cu_q = a.cu_q, p.cu_k = a.cu_k;
   p.B = a.B, p.Tq = a.Tq, p.Hq = a.Hq, p.Hkv = a.Hkv, p.D = a.D, p.causal = a.causal;
   p.G = a.Hq / a.Hkv;
   p.TQ = kTile / p.G;
-  // two tiles per CTA where that still gives every SM work
-  p.tiles = (long long)(a.Tq / (2 * p.TQ)) * a.Hkv >= sm_count() ? 2 : 1;
-  p.slots = a.Tq / (p.TQ * p.tiles) + a.B;
+  p.slots = plan.slots;
+  p.splits = plan.splits;
   const float sl = a.scale * 1.44269504088896340736f;
   p.flip = sl < 0.0f ? 0x80000000u : 0u;
   p.sl = fmaxf(fabsf(sl), 1e-30f);  // a scale of 0 keeps -inf for hidden keys
   p.out = a.out;
+  p.part = static_cast<float*>(a.ws);
+  p.ml = reinterpret_cast<float2*>(p.part + (size_t)plan.splits * a.Tq * a.Hq * a.D);
   p.err = device_error_word();
   CUtensorMap mq, mk, mv;
   if (!encode_rows(&mq, dtype, a.q, a.D, a.Hq, a.Tq, a.q_head, a.q_row, p.G, p.TQ) ||
-      !encode_rows(&mk, dtype, a.k, a.D, a.Hkv, a.Tk, a.k_head, a.k_row, 1, kTile) ||
-      !encode_rows(&mv, dtype, a.v, a.D, a.Hkv, a.Tk, a.v_head, a.v_row, 1, kTile))
+      !encode_rows(&mk, dtype, a.k, a.D, a.Hkv, a.Tk, a.k_head, a.k_row, 1, kBlk) ||
+      !encode_rows(&mv, dtype, a.v, a.D, a.Hkv, a.Tk, a.v_head, a.v_row, 1, kBlk))
     return fail(KQ_ERR_CUDA, "fa_prompt: tensor map encoding failed");
-  auto kernel = fa_prompt_tc_kernel<T, DP>;
-  if (kq_status_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), TcTraits<DP>::SMEM, "fa_prompt")) return st;
-  kernel<<<(unsigned)(p.slots * a.Hkv), kTcThreads, TcTraits<DP>::SMEM, s>>>(mq, mk, mv, p);
-  return check_launch("fa_prompt_tc");
+  auto kernel = fa_prompt_tc_kernel<T, DP, TILES>;
+  if (kq_status_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), R::SMEM, "fa_prompt")) return st;
+  kernel<<<dim3((unsigned)(p.slots * a.Hkv), (unsigned)p.splits), R::THREADS, R::SMEM, s>>>(mq, mk, mv, p);
+  if (kq_status_t st = check_launch("fa_prompt_tc")) return st;
+  if (p.splits == 1) return KQ_OK;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(((long long)a.Tq * a.Hq + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, fa_prompt_combine_kernel<T>, p), "fa_prompt_combine");
+}
+template <typename T>
+kq_status_t launch_tc_any(const FaPromptArgs& a, int dtype, cudaStream_t s) {
+  const Plan p = plan_of(a);
+  if (a.D <= 64) return p.tiles == 2 ? launch_tc<T, 64, 2>(a, dtype, p, s) : launch_tc<T, 64, 1>(a, dtype, p, s);
+  return p.tiles == 2 ? launch_tc<T, 128, 2>(a, dtype, p, s) : launch_tc<T, 128, 1>(a, dtype, p, s);
 }
 
 }  // namespace
 
-size_t fa_prompt_workspace(const FaPromptArgs&) { return 0; }
+size_t fa_prompt_workspace(const FaPromptArgs& a) {
+  if (a.D > 128 || a.Hq / a.Hkv > kTile || a.Tq == 0) return 0;
+  const int splits = plan_of(a).splits;
+  return splits == 1 ? 0 : (size_t)splits * a.Tq * a.Hq * (a.D * sizeof(float) + sizeof(float2));
+}
 
 kq_status_t launch_fa_prompt(const FaPromptArgs& a, int dtype, cudaStream_t s) {
-  if (tc_supported(a)) {
-    if (a.D <= 64)
-      return dtype == KQ_F16 ? launch_tc<__half, 64>(a, dtype, s) : launch_tc<__nv_bfloat16, 64>(a, dtype, s);
-    return dtype == KQ_F16 ? launch_tc<__half, 128>(a, dtype, s) : launch_tc<__nv_bfloat16, 128>(a, dtype, s);
-  }
+  if (tc_supported(a))
+    return dtype == KQ_F16 ? launch_tc_any<__half>(a, dtype, s) : launch_tc_any<__nv_bfloat16>(a, dtype, s);
   const long long items = (long long)a.Tq * a.Hq;
   const unsigned grid = (unsigned)((items + kSimpleWarps - 1) / kSimpleWarps);
   if (dtype == KQ_F16) fa_prompt_simple_kernel<__half><<<grid, kSimpleWarps * 32, 0, s>>>(a);
