@@ -115,43 +115,47 @@ __global__ void __launch_bounds__(kSimpleWarps * 32) fa_prompt_simple_kernel(con
 // A CTA takes TILES query tiles of one KV head. A tile is 128 rows: TQ = 128 / G
 // tokens x the G query heads that share the KV head (row = token * G + g), so K
 // and V are read once per group and short prompts fill the tile. Keys come in
-// blocks of 64. Per block and tile:
+// blocks of BLK. Per block and tile:
 //   S = Q K^T   tcgen05, Q and K in shared memory, S fp32 in TMEM
 //   P = 2^(S sl - m + kBias)   one thread per row (TMEM lane), P to TMEM over S
 //   O += P V    tcgen05, P from TMEM, V in shared memory, O fp32 in TMEM
-// S has two buffers per tile: the product for block j + 1 runs while the
-// softmax warps work on block j, so they never wait in steady state; 64-key
-// blocks make room for that in TMEM (4 x 64 columns of S, 2 x 128 of O).
 // The running maximum m only moves when a row's maximum grows by more than
 // 2^kLazy (then O is rescaled in TMEM): p stays below 2^(kBias + kLazy), inside
 // fp16, and the factor cancels in O / l. P is rounded to the inputs' type, as
 // the product with V needs both operands in it; l sums the unrounded p in fp32.
 //
-// What bounds it: per 256 rows x 128 keys the tensor core needs 2048 clocks
-// and the special-function unit, at 16 exponentials per clock, another 2048;
-// kPoly of every 64 exponentials therefore run as a polynomial on the FMA pipe.
-//
-// TILES = 2: one CTA per SM, K and V read once for 256 rows. TILES = 1: two
-// CTAs per SM, each hiding the other's start and end; for short sequences.
+// TILES = 2, BLK = 128: one CTA per SM, K and V read once for 256 rows. The
+// tiles alternate: the softmax warps of one work while the tensor core runs
+// the other's products; P is handed over in halves of 64 keys, so that the
+// product with V starts under the second half's exponentials. Per block the
+// tensor core needs 2048 clocks, shared memory about as many (each product
+// reads both operands of S there; 64-key blocks would read Q twice as often),
+// the special-function unit another 2048 at 16 exponentials a clock: kPoly of
+// every 64 run as a polynomial on the FMA pipe instead.
+// TILES = 1, BLK = 64: two CTAs per SM, each hiding the other's start and end,
+// with two S buffers; for short sequences.
 // Warps: 4 softmax warps per tile (warp w reaches TMEM lanes 32 (w % 4) ..),
-// one that issues MMAs, one that issues TMA.
+// one that issues MMAs, one that issues TMA (and two idle ones that complete
+// the warpgroup whose registers go to the softmax warps where TILES = 2).
 constexpr int kTile = 128;            // rows of a query tile
-constexpr int kBlk = 64;              // keys of a block
 constexpr float kBias = 7.0f, kLazy = 8.0f;
 constexpr int kPoly = 16;             // exponentials of each 64 on the FMA pipe
 
 template <int DP, int TILES>
 struct TcTraits {
-  static constexpr int THREADS = TILES * 128 + 64;
+  static constexpr int THREADS = TILES == 2 ? 384 : 192;
+  static constexpr int BLK = TILES == 2 ? 128 : 64;  // keys of a block
+  static constexpr int NBUF = 128 / BLK;             // S buffers of a tile
+  static constexpr int HALVES = BLK / 64;            // parts in which P is handed over
   static constexpr int PANELS = DP / 64;            // 128-byte swizzled panels of 64 dims
-  static constexpr int QPANEL = kTile * 128, PANEL = kBlk * 128;
+  static constexpr int QPANEL = kTile * 128, PANEL = BLK * 128;
   static constexpr int QTILE = PANELS * QPANEL, OPERAND = PANELS * PANEL;
-  static constexpr int STAGES = (TILES == 2 ? 10 : 5) * (128 / DP);  // K and V blocks in flight
+  static constexpr int STAGES = (TILES == 2 ? 5 : 4) * (128 / DP);  // K and V blocks in flight
   static constexpr int OFF_KV = TILES * QTILE;
   static constexpr int OFF_BAR = OFF_KV + STAGES * OPERAND;
-  static constexpr int SMEM = OFF_BAR + 512;
-  static constexpr int COLS = TILES * 256;          // TMEM columns: S buffers, then O
-  static_assert((2 * STAGES + 6 * TILES) * 8 + 4 <= 512, "barrier area");
+  static constexpr int SMEM = OFF_BAR + 512 + 1024;
+  static constexpr int COLS = TILES * 256;          // TMEM columns: 128 of S per tile, then O
+  static_assert((2 * STAGES + (3 + NBUF + HALVES) * TILES) * 8 + 4 <= 512, "barrier area");
   static_assert(2 * (SMEM + 1024) <= 233472 || TILES == 2, "two CTAs per SM");
   static_assert(SMEM <= 232448, "shared memory budget");
 };
@@ -282,45 +286,42 @@ __device__ __forceinline__ bool find_work(const TcArgs& a, int tt, int slot, Wor
 __device__ __forceinline__ int keys_of(const TcArgs& a, const Work& w, int i) {
   return a.causal ? max(0, min(w.lk, i + w.lk - w.lq + 1)) : w.lk;
 }
-// Key blocks of tile t (0 when it has no token or sees no key).
-__device__ __forceinline__ int blocks_of(const TcArgs& a, const Work& w, int t) {
+// Blocks of blk keys of tile t (0 when it has no token or sees no key).
+__device__ __forceinline__ int blocks_of(const TcArgs& a, const Work& w, int t, int blk) {
   const int first = w.tok + t * a.TQ;
   if (first >= w.lq) return 0;
-  return (keys_of(a, w, min(w.lq, first + a.TQ) - 1) + kBlk - 1) / kBlk;
+  return (keys_of(a, w, min(w.lq, first + a.TQ) - 1) + blk - 1) / blk;
 }
 
 template <typename T, int DP, int TILES>
-__global__ void __launch_bounds__(TILES * 128 + 64, TILES == 2 ? 1 : 2)
+__global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
     fa_prompt_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcArgs a) {
   using R = TcTraits<DP, TILES>;
-  constexpr int STAGES = R::STAGES, kMmaWarp = TILES * 4, kLoadWarp = kMmaWarp + 1;
-  constexpr uint32_t kColO = TILES * 2 * kBlk;       // S of tile t, buffer x at (2 t + x) * kBlk
+  constexpr int STAGES = R::STAGES, BLK = R::BLK, NBUF = R::NBUF, HALVES = R::HALVES;
+  constexpr int kMmaWarp = TILES * 4, kLoadWarp = kMmaWarp + 1;
+  constexpr uint32_t kColO = TILES * 128;  // S of tile t, buffer x at 128 t + BLK x; O of tile t at kColO + DP t
   const int head = blockIdx.x % a.Hkv;
   Work w;
   // later tiles of a causal sequence see more keys: they start first
   if (!find_work(a, a.TQ * TILES, a.slots - 1 - blockIdx.x / a.Hkv, w)) return;
 
-  extern __shared__ __align__(1024) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + R::OFF_BAR);
   uint64_t* kv_full = q_full + TILES;
   uint64_t* kv_empty = kv_full + STAGES;
-  uint64_t* s_full = kv_empty + STAGES;   // [tile][buffer]: S is there
-  uint64_t* p_full = s_full + 2 * TILES;  // P of a tile is there
-  uint64_t* pv_done = p_full + TILES;     // the tile's latest P V is done
+  uint64_t* s_full = kv_empty + STAGES;      // [tile][buffer]: S is there
+  uint64_t* p_full = s_full + NBUF * TILES;  // [tile][half]: 64 keys of P are there
+  uint64_t* pv_done = p_full + HALVES * TILES;  // the tile's latest P V is done
   uint64_t* o_full = pv_done + TILES;     // the tile's last P V is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + TILES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (smem_u32(smem) & 1023u) {  // swizzled tiles need it
-    if (threadIdx.x == 0) record_error(a.err, DEV_BAD_SHAPE);
-    return;
-  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < TILES; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&s_full[2 * i], 1);
-      mbar_init(&s_full[2 * i + 1], 1);
-      mbar_init(&p_full[i], 4);
+      for (int x = 0; x < NBUF; ++x) mbar_init(&s_full[NBUF * i + x], 1);
+      for (int x = 0; x < HALVES; ++x) mbar_init(&p_full[HALVES * i + x], 4);
       mbar_init(&pv_done[i], 1);
       mbar_init(&o_full[i], 1);
     }
@@ -344,7 +345,7 @@ __global__ void __launch_bounds__(TILES * 128 + 64, TILES == 2 ? 1 : 2)
   // this split's range of key blocks, and its share of every tile
   int cnt[TILES], n = 0;
 #pragma unroll
-  for (int t = 0; t < TILES; ++t) cnt[t] = blocks_of(a, w, t), n = max(n, cnt[t]);
+  for (int t = 0; t < TILES; ++t) cnt[t] = blocks_of(a, w, t, BLK), n = max(n, cnt[t]);
   const int j0 = (int)((long long)n * blockIdx.y / a.splits), j1 = (int)((long long)n * (blockIdx.y + 1) / a.splits);
 #pragma unroll
   for (int t = 0; t < TILES; ++t) cnt[t] = max(0, min(cnt[t], j1) - j0);
@@ -354,6 +355,10 @@ __global__ void __launch_bounds__(TILES * 128 + 64, TILES == 2 ? 1 : 2)
   auto item_v = [&](int i) { return i + 1 == n ? 2 * i + 1 : 2 * i + 2; };
   bool dead = false;
 
+  // 384 x 168 registers at launch: 256 x 208 + 128 x 88
+  if constexpr (TILES == 2) {
+    if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  }
   if (warp == kLoadWarp) {
     if (lane == 0) {
       tc::prefetch_tmap(&map_q);
@@ -374,61 +379,70 @@ __global__ void __launch_bounds__(TILES * 128 + 64, TILES == 2 ? 1 : 2)
         mbar_arrive_expect_tx(&kv_full[st], R::OPERAND);
         for (int p = 0; p < R::PANELS; ++p)
           tma_load_3d(smem + R::OFF_KV + st * R::OPERAND + p * R::PANEL, is_v ? &map_v : &map_k, p * 64, head,
-                      w.k0 + (j0 + i) * kBlk, &kv_full[st]);
+                      w.k0 + (j0 + i) * BLK, &kv_full[st]);
       }
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    constexpr uint32_t idesc_s = idesc<T>(kBlk, false), idesc_o = idesc<T>(DP, true);
+    constexpr uint32_t idesc_s = idesc<T>(BLK, false), idesc_o = idesc<T>(DP, true);
     const uint32_t q_base = smem_u32(smem), kv_base = q_base + R::OFF_KV;
     const uint32_t go = tc::elect_one();
-    // S_t = Q_t K_i^T into buffer i & 1
-    auto scores = [&](int i) {
+    // S_t = Q_t K_i^T into buffer i % NBUF
+    auto score = [&](int t, int i) {
       const int st = item_k(i) % STAGES;
       mbar_wait_or_poison(&kv_full[st], (item_k(i) / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+      if (i == 0) mbar_wait_or_poison(&q_full[t], 0, a.err, DEV_TIMEOUT_FULL, dead);
       tc::tc_fence_after();
-      const uint64_t kd = tc::sw128_desc(kv_base + st * R::OPERAND);
+      const uint64_t kd = tc::sw128_desc(kv_base + st * R::OPERAND), qd = tc::sw128_desc(q_base + t * R::QTILE);
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        if (i >= cnt[t]) continue;
-        if (i == 0) {
-          mbar_wait_or_poison(&q_full[t], 0, a.err, DEV_TIMEOUT_FULL, dead);
-          tc::tc_fence_after();
-        }
-        const uint64_t qd = tc::sw128_desc(q_base + t * R::QTILE);
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k)
-          tc::mma_ss_go(tmem + (2 * t + (i & 1)) * kBlk, qd + (uint64_t)((k >> 2) * (R::QPANEL >> 4) + (k & 3) * 2),
-                        kd + (uint64_t)((k >> 2) * (R::PANEL >> 4) + (k & 3) * 2), idesc_s, k > 0, go);
-        tc::mma_commit_go(&s_full[2 * t + (i & 1)], go);
-      }
-      tc::mma_commit_go(&kv_empty[st], go);
+      for (int k = 0; k < DP / 16; ++k)
+        tc::mma_ss_go(tmem + t * 128 + (i % NBUF) * BLK, qd + (uint64_t)((k >> 2) * (R::QPANEL >> 4) + (k & 3) * 2),
+                      kd + (uint64_t)((k >> 2) * (R::PANEL >> 4) + (k & 3) * 2), idesc_s, k > 0, go);
+      tc::mma_commit_go(&s_full[NBUF * t + i % NBUF], go);
     };
-    if (n > 0) scores(0);
+    auto release_k = [&](int i) { tc::mma_commit_go(&kv_empty[item_k(i) % STAGES], go); };
+    if (n > 0) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+        if (cnt[t] > 0) score(t, 0);
+      release_k(0);
+    }
     for (int i = 0; i < n; ++i) {
-      // buffer (i + 1) & 1 held P of block i - 1, whose product was issued before
-      if (i + 1 < n) scores(i + 1);
+      if (NBUF == 2 && i + 1 < n) {
+        // the other buffer held P of block i - 1, whose product was issued before
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+          if (i + 1 < cnt[t]) score(t, i + 1);
+        release_k(i + 1);
+      }
       const int st = item_v(i) % STAGES;
       mbar_wait_or_poison(&kv_full[st], (item_v(i) / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
       const uint64_t vd = tc::sw128_desc_mn(kv_base + st * R::OPERAND, R::PANEL);  // dims across, tokens down
 #pragma unroll
       for (int t = 0; t < TILES; ++t) {
         if (i >= cnt[t]) continue;
-        mbar_wait_or_poison(&p_full[t], i & 1, a.err, DEV_TIMEOUT_FULL, dead);
-        tc::tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < kBlk / 16; ++k)
-          tc::mma_ts_go(tmem + kColO + t * DP, tmem + (2 * t + (i & 1)) * kBlk + 8 * k, vd + (uint64_t)(k * (2048 >> 4)),
-                        idesc_o, (i > 0 || k > 0) ? 1u : 0u, go);
+        for (int h = 0; h < HALVES; ++h) {
+          mbar_wait_or_poison(&p_full[HALVES * t + h], i & 1, a.err, DEV_TIMEOUT_FULL, dead);
+          tc::tc_fence_after();
+#pragma unroll
+          for (int k = 4 * h; k < 4 * h + 4; ++k)
+            tc::mma_ts_go(tmem + kColO + t * DP, tmem + t * 128 + (i % NBUF) * BLK + 8 * k, vd + (uint64_t)(k * (2048 >> 4)),
+                          idesc_o, (i > 0 || k > 0) ? 1u : 0u, go);
+        }
         tc::mma_commit_go(i + 1 == cnt[t] ? &o_full[t] : &pv_done[t], go);
+        // one buffer: the next scores take the place of the P just consumed (the products run in order)
+        if (NBUF == 1 && i + 1 < cnt[t]) score(t, i + 1);
       }
       tc::mma_commit_go(&kv_empty[st], go);
+      if (NBUF == 1 && i + 1 < n) release_k(i + 1);
     }
     __syncwarp();
-  } else {
+  } else if (warp < kMmaWarp) {
+    if constexpr (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = warp >> 2, row = threadIdx.x & 127, nt = cnt[TILES == 2 ? t : 0];
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + 2 * t * kBlk, o_addr = tmem + lanes + kColO + t * DP;
+    const uint32_t s_addr = tmem + lanes + t * 128, o_addr = tmem + lanes + kColO + t * DP;
     const int first = w.tok + t * a.TQ;                     // the tile's first token
     const int tok = first + row / a.G, g = row % a.G;
     const bool mine = row < a.TQ * a.G && tok < w.lq;
@@ -437,30 +451,31 @@ __global__ void __launch_bounds__(TILES * 128 + 64, TILES == 2 ? 1 : 2)
     float m = -INFINITY;
     F2 l2 = f2(0.0f, 0.0f);
     for (int i = 0; i < nt; ++i) {
-      const int key0 = (j0 + i) * kBlk;
-      mbar_wait_or_poison(&s_full[2 * t + (i & 1)], (i >> 1) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+      const int key0 = (j0 + i) * BLK;
+      const uint32_t sp = s_addr + (i % NBUF) * BLK;
+      mbar_wait_or_poison(&s_full[NBUF * t + i % NBUF], (i / NBUF) & 1, a.err, DEV_TIMEOUT_FULL, dead);
       __syncwarp();
       tc::tc_fence_after();
-      uint32_t s[kBlk];
-      tc::tmem_ld32(s_addr + (i & 1) * kBlk, reinterpret_cast<uint32_t(&)[32]>(s[0]));
-      tc::tmem_ld32(s_addr + (i & 1) * kBlk + 32, reinterpret_cast<uint32_t(&)[32]>(s[32]));
+      uint32_t s[BLK];
+#pragma unroll
+      for (int c = 0; c < BLK; c += 32) tc::tmem_ld32(sp + c, *reinterpret_cast<uint32_t(*)[32]>(s + c));
       tc::tmem_ld_wait();
       if (a.flip) {
 #pragma unroll
-        for (int x = 0; x < kBlk; ++x) s[x] ^= a.flip;
+        for (int x = 0; x < BLK; ++x) s[x] ^= a.flip;
       }
-      if (key0 + kBlk > all_see) {
+      if (key0 + BLK > all_see) {
         const int lim = keys - key0;
 #pragma unroll
-        for (int x = 0; x < kBlk; ++x)
+        for (int x = 0; x < BLK; ++x)
           if (x >= lim) s[x] = 0xff800000u;
         const int valid = w.lk - key0;
-        if (valid < kBlk) {
+        if (valid < BLK) {
           // rows of V behind the sequence's end belong to others: what they
           // hold must not meet P (0 x inf); both tiles write the same zeros
           const int st = item_v(i) % STAGES;
           mbar_wait_or_poison(&kv_full[st], (item_v(i) / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
-          for (int x = row; x < (kBlk - valid) * 8 * R::PANELS; x += kTile) {
+          for (int x = row; x < (BLK - valid) * 8 * R::PANELS; x += kTile) {
             const int c = x % 8, p = x / 8 % R::PANELS, r = valid + x / (8 * R::PANELS);
             *reinterpret_cast<uint4*>(smem + R::OFF_KV + st * R::OPERAND + p * R::PANEL + r * 128 + c * 16) =
                 make_uint4(0, 0, 0, 0);
@@ -468,16 +483,14 @@ __global__ void __launch_bounds__(TILES * 128 + 64, TILES == 2 ? 1 : 2)
           fence_proxy_async_smem();
         }
       }
-      float mx[4];
+      float mx[8];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) mx[x] = __uint_as_float(s[x]);
+      for (int x = 0; x < 8; ++x) mx[x] = fmaxf(__uint_as_float(s[x]), __uint_as_float(s[x + 8]));
 #pragma unroll
-      for (int x = 4; x < kBlk; x += 8)
+      for (int x = 16; x < BLK; x += 16)
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
-          if (x + y + 4 < kBlk) mx[y] = max3(mx[y], __uint_as_float(s[x + y]), __uint_as_float(s[x + y + 4]));
-          else mx[y] = fmaxf(mx[y], __uint_as_float(s[x + y]));
-      const float mn = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * a.sl;
+        for (int y = 0; y < 8; ++y) mx[y] = max3(mx[y], __uint_as_float(s[x + y]), __uint_as_float(s[x + y + 8]));
+      const float mn = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * a.sl;
       float f = 1.0f;
       if (mn > m + kLazy) {  // also the row's first keys (m = -inf)
         f = ex2(m - mn);
@@ -485,7 +498,7 @@ __global__ void __launch_bounds__(TILES * 128 + 64, TILES == 2 ? 1 : 2)
         l2 = mul2(l2, f2(f, f));
       }
       if (i > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
-        // the product of block i - 2 is done (S of block i came after it)
+        // the product before the latest one is done (S of this block came after it)
         mbar_wait_or_poison(&pv_done[t], (i - 1) & 1, a.err, DEV_TIMEOUT_FULL, dead);
         __syncwarp();
         tc::tc_fence_after();
@@ -502,30 +515,33 @@ __global__ void __launch_bounds__(TILES * 128 + 64, TILES == 2 ? 1 : 2)
       const float off = m == -INFINITY ? 0.0f : kBias - m;
       const F2 sl2 = f2(a.sl, a.sl), off2 = f2(off, off);
       F2 sum = f2(0.0f, 0.0f);
-      uint32_t p[kBlk / 2];
 #pragma unroll
-      for (int x = 0; x < kBlk / 2; ++x) {
-        F2 e = fma2(f2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1])), sl2, off2);
-        float e0, e1;
-        // the polynomial's elements are spread among the others
-        if ((x * kPoly / kBlk) != ((x + 1) * kPoly / kBlk) && kPoly > 0) {
-          e = exp2_poly(e);
-          unpack(e, e0, e1);
-        } else {
-          unpack(e, e0, e1);
-          e0 = ex2(e0), e1 = ex2(e1);
-          e = f2(e0, e1);
+      for (int h = 0; h < HALVES; ++h) {
+        uint32_t p[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+          F2 e = fma2(f2(__uint_as_float(s[64 * h + 2 * x]), __uint_as_float(s[64 * h + 2 * x + 1])), sl2, off2);
+          float e0, e1;
+          // the polynomial's elements are spread among the others
+          if (x * kPoly / 64 != (x + 1) * kPoly / 64) {
+            e = exp2_poly(e);
+            unpack(e, e0, e1);
+          } else {
+            unpack(e, e0, e1);
+            e0 = ex2(e0), e1 = ex2(e1);
+            e = f2(e0, e1);
+          }
+          sum = add2(sum, e);
+          p[x] = pack2<T>(e0, e1);
         }
-        sum = add2(sum, e);
-        p[x] = pack2<T>(e0, e1);
+        __syncwarp();
+        tc::tmem_st32(sp + 32 * h, p);
+        tc::tmem_st_wait();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[HALVES * t + h]);
       }
       l2 = add2(l2, sum);
-      __syncwarp();
-      tc::tmem_st32(s_addr + (i & 1) * kBlk, p);
-      tc::tmem_st_wait();
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t]);
     }
     float l, l1;
     unpack(l2, l, l1);
@@ -677,8 +693,8 @@ kq_status_t launch_tc(const FaPromptArgs& a, int dtype, const Plan& plan, cudaSt
   p.err = device_error_word();
   CUtensorMap mq, mk, mv;
   if (!encode_rows(&mq, dtype, a.q, a.D, a.Hq, a.Tq, a.q_head, a.q_row, p.G, p.TQ) ||
-      !encode_rows(&mk, dtype, a.k, a.D, a.Hkv, a.Tk, a.k_head, a.k_row, 1, kBlk) ||
-      !encode_rows(&mv, dtype, a.v, a.D, a.Hkv, a.Tk, a.v_head, a.v_row, 1, kBlk))
+      !encode_rows(&mk, dtype, a.k, a.D, a.Hkv, a.Tk, a.k_head, a.k_row, 1, R::BLK) ||
+      !encode_rows(&mv, dtype, a.v, a.D, a.Hkv, a.Tk, a.v_head, a.v_row, 1, R::BLK))
     return fail(KQ_ERR_CUDA, "fa_prompt: tensor map encoding failed");
   auto kernel = fa_prompt_tc_kernel<T, DP, TILES>;
   if (kq_status_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), R::SMEM, "fa_prompt")) return st;
