@@ -633,9 +633,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
   uint64_t* p_full = s_full + 2;       // P of a tile is there, its S is read
   uint64_t* o_full = p_full + 2;       // the tile's last P V is done
   uint64_t* q_full = o_full + 2;       // the tiles' queries are in TMEM
-  uint64_t* row_mask = q_full + 1;     // rows present in block j, at j % kMasks
+  uint64_t* drained = q_full + 1;      // all of the MMA warp's products and arrivals are done
+  uint64_t* row_mask = drained + 1;    // rows present in block j, at j % kMasks
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(row_mask + kMasks);
-  static_assert((2 * kOps + 7 + kMasks) * 8 + 4 <= 512, "barrier area");
+  static_assert((2 * kOps + 8 + kMasks) * 8 + 4 <= 512, "barrier area");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
 
@@ -656,6 +657,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
       mbar_init(&o_full[i], 1);
     }
     mbar_init(q_full, two ? 8 : 4);
+    mbar_init(drained, 1);
     fence_mbar_init();
   }
   if (warp == kMmaWarp) tc::tmem_alloc(tmem_slot, 512);
@@ -785,11 +787,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
                         (part > 0 || k > 0) ? 1u : 0u, go);
       tc::mma_commit_go(&s_full[t], go);
     };
+    // every arrival is waited for before the CTA ends: a stage is only released
+    // to an item that waits for it, and the warp drains at the end
+    auto release = [&](int item) {
+      if (item + kOps < 2 * n) tc::mma_commit_go(&op_empty[item % kOps], go);
+    };
     mbar_wait_or_poison(q_full, 0, a.err, DEV_TIMEOUT_FULL, dead);
     tc::tc_fence_after();
     if (n > 0) {
       for (int t = 0; t < tiles; ++t) score(t, 0);
-      tc::mma_commit_go(&op_empty[0], go);
+      release(0);
     }
     for (int j = 0; j < n; ++j) {
       const int sv = (2 * j + 1) % kOps;
@@ -809,9 +816,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
         if (j + 1 == n) tc::mma_commit_go(&o_full[t], go);
         if (j + 1 < n) score(t, j + 1);
       }
-      tc::mma_commit_go(&op_empty[sv], go);
-      if (j + 1 < n) tc::mma_commit_go(&op_empty[(2 * j + 2) % kOps], go);
+      release(2 * j + 1);
+      if (j + 1 < n) release(2 * j + 2);
     }
+    tc::mma_commit_go(drained, go);
+    mbar_wait_idle_or_poison(drained, 0, a.err, DEV_TIMEOUT_FULL, dead);
     __syncwarp();
   } else {
     // ---- softmax, a thread per row

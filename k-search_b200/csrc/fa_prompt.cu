@@ -155,7 +155,7 @@ struct TcTraits {
   static constexpr int OFF_BAR = OFF_KV + STAGES * OPERAND;
   static constexpr int SMEM = OFF_BAR + 512 + 1024;
   static constexpr int COLS = TILES * 256;          // TMEM columns: 128 of S per tile, then O
-  static_assert((2 * STAGES + (3 + NBUF + HALVES) * TILES) * 8 + 4 <= 512, "barrier area");
+  static_assert((2 * STAGES + (3 + NBUF + HALVES) * TILES + 1) * 8 + 4 <= 512, "barrier area");
   static_assert(2 * (SMEM + 1024) <= 233472 || TILES == 2, "two CTAs per SM");
   static_assert(SMEM <= 232448, "shared memory budget");
 };
@@ -268,12 +268,16 @@ struct Work {
 // Slot -> (sequence, tile): sequence b owns slots cu_q[b] / TT + b .., at
 // least ceil(len / TT) of them, so no prefix sum over tiles is needed; slots
 // past a sequence's end are empty (at most one or two per sequence).
+// The whole warp searches: 32 candidates per step.
 __device__ __forceinline__ bool find_work(const TcArgs& a, int tt, int slot, Work& w) {
-  int lo = 0, hi = a.B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu_q[mid] / tt + mid <= slot) lo = mid;
-    else hi = mid;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = a.B;
+  while (n > 1) {
+    const int step = (n + 31) / 32, mid = lo + lane * step;
+    const bool before = mid < lo + n && a.cu_q[mid] / tt + mid <= slot;
+    const int last = 31 - __clz(__ballot_sync(0xffffffffu, before) | 1u);
+    n = min(step, n - last * step);
+    lo += last * step;
   }
   w.q0 = a.cu_q[lo];
   w.lq = min(a.cu_q[lo + 1], a.Tq) - w.q0;
@@ -315,9 +319,30 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
   uint64_t* p_full = s_full + NBUF * TILES;  // [tile][half]: 64 keys of P are there
   uint64_t* pv_done = p_full + HALVES * TILES;  // the tile's latest P V is done
   uint64_t* o_full = pv_done + TILES;     // the tile's last P V is done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + TILES);
+  uint64_t* drained = o_full + TILES;     // all of the MMA warp's products and arrivals are done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
+  // this split's range of key blocks, and its share of every tile
+  int cnt[TILES], n = 0;
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) cnt[t] = blocks_of(a, w, t, BLK), n = max(n, cnt[t]);
+  const int j0 = (int)((long long)n * blockIdx.y / a.splits), j1 = (int)((long long)n * (blockIdx.y + 1) / a.splits);
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) cnt[t] = max(0, min(cnt[t], j1) - j0);
+  n = j1 - j0;
+  // K and V blocks in the order they are used: K0 K1 V0 K2 V1 .. V(n - 1)
+  auto item_k = [&](int i) { return i == 0 ? 0 : 2 * i - 1; };
+  auto item_v = [&](int i) { return i + 1 == n ? 2 * i + 1 : 2 * i + 2; };
+  auto load_item = [&](int x) {
+    const bool is_v = x > 0 && ((x & 1) == 0 || x + 1 == 2 * n);
+    const int i = x == 0 ? 0 : is_v ? (x + 1 == 2 * n ? n - 1 : (x - 2) >> 1) : (x + 1) >> 1;
+    const int st = x % STAGES;
+    mbar_arrive_expect_tx(&kv_full[st], R::OPERAND);
+    for (int p = 0; p < R::PANELS; ++p)
+      tma_load_3d(smem + R::OFF_KV + st * R::OPERAND + p * R::PANEL, is_v ? &map_v : &map_k, p * 64, head,
+                  w.k0 + (j0 + i) * BLK, &kv_full[st]);
+  };
+  if (threadIdx.x == kLoadWarp * 32) {
     for (int i = 0; i < TILES; ++i) {
       mbar_init(&q_full[i], 1);
       for (int x = 0; x < NBUF; ++x) mbar_init(&s_full[NBUF * i + x], 1);
@@ -329,7 +354,17 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
     }
+    mbar_init(drained, 1);
     fence_mbar_init();
+    // the first loads run under the rest of the set-up
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      if (cnt[t] == 0) continue;
+      mbar_arrive_expect_tx(&q_full[t], R::PANELS * a.TQ * a.G * 128);
+      for (int p = 0; p < R::PANELS; ++p)
+        tma_load_3d(smem + t * R::QTILE + p * R::QPANEL, &map_q, p * 64, head * a.G, w.q0 + w.tok + t * a.TQ, &q_full[t]);
+    }
+    for (int x = 0; x < min(2 * n, STAGES); ++x) load_item(x);
   }
   // rows of a query tile that no token fills stay zero
   for (int i = threadIdx.x; i < TILES * R::PANELS * (kTile - a.TQ * a.G) * 8; i += R::THREADS) {
@@ -342,17 +377,6 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // this split's range of key blocks, and its share of every tile
-  int cnt[TILES], n = 0;
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) cnt[t] = blocks_of(a, w, t, BLK), n = max(n, cnt[t]);
-  const int j0 = (int)((long long)n * blockIdx.y / a.splits), j1 = (int)((long long)n * (blockIdx.y + 1) / a.splits);
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) cnt[t] = max(0, min(cnt[t], j1) - j0);
-  n = j1 - j0;
-  // K and V blocks in the order they are used: K0 K1 V0 K2 V1 .. V(n - 1)
-  auto item_k = [&](int i) { return i == 0 ? 0 : 2 * i - 1; };
-  auto item_v = [&](int i) { return i + 1 == n ? 2 * i + 1 : 2 * i + 2; };
   bool dead = false;
 
   // 384 x 168 registers at launch: 256 x 208 + 128 x 88
@@ -360,28 +384,12 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
     if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   }
   if (warp == kLoadWarp) {
-    if (lane == 0) {
-      tc::prefetch_tmap(&map_q);
-      tc::prefetch_tmap(&map_k);
-      tc::prefetch_tmap(&map_v);
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        if (cnt[t] == 0) continue;
-        mbar_arrive_expect_tx(&q_full[t], R::PANELS * a.TQ * a.G * 128);
-        for (int p = 0; p < R::PANELS; ++p)
-          tma_load_3d(smem + t * R::QTILE + p * R::QPANEL, &map_q, p * 64, head * a.G, w.q0 + w.tok + t * a.TQ, &q_full[t]);
-      }
-      for (int x = 0; x < 2 * n; ++x) {
-        const bool is_v = x > 0 && ((x & 1) == 0 || x + 1 == 2 * n);
-        const int i = x == 0 ? 0 : is_v ? (x + 1 == 2 * n ? n - 1 : (x - 2) >> 1) : (x + 1) >> 1;
+    if (lane == 0)
+      for (int x = STAGES; x < 2 * n; ++x) {
         const int st = x % STAGES;
-        if (x >= STAGES) mbar_wait_idle_or_poison(&kv_empty[st], ((x / STAGES) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
-        mbar_arrive_expect_tx(&kv_full[st], R::OPERAND);
-        for (int p = 0; p < R::PANELS; ++p)
-          tma_load_3d(smem + R::OFF_KV + st * R::OPERAND + p * R::PANEL, is_v ? &map_v : &map_k, p * 64, head,
-                      w.k0 + (j0 + i) * BLK, &kv_full[st]);
+        mbar_wait_idle_or_poison(&kv_empty[st], ((x / STAGES) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
+        load_item(x);
       }
-    }
     __syncwarp();
   } else if (warp == kMmaWarp) {
     constexpr uint32_t idesc_s = idesc<T>(BLK, false), idesc_o = idesc<T>(DP, true);
@@ -400,12 +408,18 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
                       kd + (uint64_t)((k >> 2) * (R::PANEL >> 4) + (k & 3) * 2), idesc_s, k > 0, go);
       tc::mma_commit_go(&s_full[NBUF * t + i % NBUF], go);
     };
-    auto release_k = [&](int i) { tc::mma_commit_go(&kv_empty[item_k(i) % STAGES], go); };
+    // Every arrival must have come before the CTA ends: with two CTAs on an SM
+    // their products share one queue, and an arrival behind the other CTA's
+    // products would land in the next CTA's shared memory. So a stage is only
+    // released to a load that waits for it, and the warp drains at the end.
+    auto release = [&](int item) {
+      if (item + STAGES < 2 * n) tc::mma_commit_go(&kv_empty[item % STAGES], go);
+    };
     if (n > 0) {
 #pragma unroll
       for (int t = 0; t < TILES; ++t)
         if (cnt[t] > 0) score(t, 0);
-      release_k(0);
+      release(0);
     }
     for (int i = 0; i < n; ++i) {
       if (NBUF == 2 && i + 1 < n) {
@@ -413,7 +427,7 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
           if (i + 1 < cnt[t]) score(t, i + 1);
-        release_k(i + 1);
+        release(item_k(i + 1));
       }
       const int st = item_v(i) % STAGES;
       mbar_wait_or_poison(&kv_full[st], (item_v(i) / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
@@ -434,9 +448,11 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
         // one buffer: the next scores take the place of the P just consumed (the products run in order)
         if (NBUF == 1 && i + 1 < cnt[t]) score(t, i + 1);
       }
-      tc::mma_commit_go(&kv_empty[st], go);
-      if (NBUF == 1 && i + 1 < n) release_k(i + 1);
+      release(item_v(i));
+      if (NBUF == 1 && i + 1 < n) release(item_k(i + 1));
     }
+    tc::mma_commit_go(drained, go);
+    mbar_wait_idle_or_poison(drained, 0, a.err, DEV_TIMEOUT_FULL, dead);
     __syncwarp();
   } else if (warp < kMmaWarp) {
     if constexpr (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -552,49 +568,56 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
       tc::tc_fence_after();
     }
     const bool none = m == -INFINITY && l == l;             // no key seen (a NaN score is one)
-    const long long at = (long long)(w.q0 + tok) * a.Hq + head * a.G + g;
-    if (a.splits > 1) {
-      const long long prow = (long long)blockIdx.y * a.Tq * a.Hq + at;
+    // Rows leave through shared memory (the tile's queries are done with), 128
+    // bytes of each at a time, so that a warp's store covers 4 whole lines; a
+    // thread's own row would be 32 scattered pieces of 16 bytes.
+    const long long at = mine ? (long long)(w.q0 + tok) * a.Hq + head * a.G + g : -1;
+    uint8_t* stage = smem + t * R::QTILE + (warp & 3) * 4096;
+    const float inv = 1.0f / l;
+    const bool partial = a.splits > 1;
+    const int cols = partial ? 32 : 64, item = partial ? 4 : 2;  // columns of 128 bytes, bytes of an element
+    uint8_t* base = partial ? reinterpret_cast<uint8_t*>(a.part + (long long)blockIdx.y * a.Tq * a.Hq * a.D)
+                            : static_cast<uint8_t*>(a.out);
+    if (partial && mine)
+      a.ml[(long long)blockIdx.y * a.Tq * a.Hq + at] = make_float2(none ? -INFINITY : m, none ? 0.0f : l);
 #pragma unroll 1
-      for (int c = 0; c < DP / 32; ++c) {
+    for (int c = 0; c < a.D; c += cols) {
+      __syncwarp();
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (half == 1 && partial) break;
         uint32_t o[32];
-        __syncwarp();
         if (nt > 0) {
-          tc::tmem_ld32(o_addr + 32 * c, o);
+          tc::tmem_ld32(o_addr + c + 32 * half, o);
           tc::tmem_ld_wait();
         }
-        if (mine && !none) {
+#pragma unroll
+        for (int x = 0; x < 32; ++x)
+          if (none) o[x] = 0;
+        if (partial) {
 #pragma unroll
           for (int x = 0; x < 8; ++x)
-            if (32 * c + 4 * x < a.D)
-              *reinterpret_cast<uint4*>(a.part + prow * a.D + 32 * c + 4 * x) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
-        }
-      }
-      if (mine) a.ml[prow] = make_float2(none ? -INFINITY : m, none ? 0.0f : l);
-    } else {
-      T* out = static_cast<T*>(a.out) + at * a.D;
-      const float inv = 1.0f / l;
-#pragma unroll 1
-      for (int c = 0; c < DP / 32; ++c) {
-        uint32_t o[32];
-        __syncwarp();
-        if (nt > 0) {
-          tc::tmem_ld32(o_addr + 32 * c, o);
-          tc::tmem_ld_wait();
-        }
-        if (mine) {
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((x ^ (lane & 7)) << 4)) =
+                make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        } else {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (!none) {
-              v.x = pack2<T>(__uint_as_float(o[8 * x]) * inv, __uint_as_float(o[8 * x + 1]) * inv);
-              v.y = pack2<T>(__uint_as_float(o[8 * x + 2]) * inv, __uint_as_float(o[8 * x + 3]) * inv);
-              v.z = pack2<T>(__uint_as_float(o[8 * x + 4]) * inv, __uint_as_float(o[8 * x + 5]) * inv);
-              v.w = pack2<T>(__uint_as_float(o[8 * x + 6]) * inv, __uint_as_float(o[8 * x + 7]) * inv);
-            }
-            if (32 * c + 8 * x < a.D) *reinterpret_cast<uint4*>(out + 32 * c + 8 * x) = v;
+            uint32_t v[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              v[y] = none ? 0u : pack2<T>(__uint_as_float(o[8 * x + 2 * y]) * inv, __uint_as_float(o[8 * x + 2 * y + 1]) * inv);
+            *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * half + x) ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const int r = 4 * x + (lane >> 3), piece = lane & 7;
+        const long long dst = __shfl_sync(0xffffffffu, at, r);
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+        if (dst >= 0 && c * item + piece * 16 < a.D * item)
+          *reinterpret_cast<uint4*>(base + (dst * a.D + c) * item + piece * 16) = v;
       }
     }
   }
