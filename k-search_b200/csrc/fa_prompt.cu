@@ -127,19 +127,28 @@ __global__ void __launch_bounds__(kSimpleWarps * 32) fa_prompt_simple_kernel(con
 // TILES = 2, BLK = 128: one CTA per SM, K and V read once for 256 rows. The
 // tiles alternate: the softmax warps of one work while the tensor core runs
 // the other's products; P is handed over in halves of 64 keys, so that the
-// product with V starts under the second half's exponentials. Per block the
-// tensor core needs 2048 clocks, shared memory about as many (each product
-// reads both operands of S there; 64-key blocks would read Q twice as often),
-// the special-function unit another 2048 at 16 exponentials a clock: kPoly of
-// every 64 run as a polynomial on the FMA pipe instead.
+// product with V starts under the second half's exponentials. Per block of two
+// tiles the tensor core needs 2048 clocks, shared memory about as many (each
+// product reads both operands of S there; 64-key blocks would read Q twice as
+// often), the special-function unit another 2048 at 16 exponentials a clock. A
+// block takes about 3300: the chain S -> maximum -> P -> next S of each tile is
+// what bounds it. Without exponentials, maxima and sums it would be 2700; some
+// exponentials as a polynomial on the FMA pipe changed nothing (474 us with 16
+// of 64, 474 without, 479 with 24; 8192 tokens, 32 heads over 8).
 // TILES = 1, BLK = 64: two CTAs per SM, each hiding the other's start and end,
 // with two S buffers; for short sequences.
+// CTAs are persistent: the TMA warp looks up the next job and starts its loads
+// while the softmax warps still work on the last one, and the MMA warp runs
+// its first products under their epilogue. A short job is otherwise mostly
+// set-up: TMEM, look-ups, first loads, last stores.
 // Warps: 4 softmax warps per tile (warp w reaches TMEM lanes 32 (w % 4) ..),
-// one that issues MMAs, one that issues TMA (and two idle ones that complete
+// one that issues MMAs, one for jobs and TMA (and two idle ones that complete
 // the warpgroup whose registers go to the softmax warps where TILES = 2).
+// Every arrival has a waiter before the CTA ends: with two CTAs on an SM their
+// products share one queue, and an arrival that came after the CTA's end would
+// land in the next one's shared memory.
 constexpr int kTile = 128;            // rows of a query tile
 constexpr float kBias = 7.0f, kLazy = 8.0f;
-constexpr int kPoly = 16;             // exponentials of each 64 on the FMA pipe
 
 template <int DP, int TILES>
 struct TcTraits {
@@ -150,12 +159,13 @@ struct TcTraits {
   static constexpr int PANELS = DP / 64;            // 128-byte swizzled panels of 64 dims
   static constexpr int QPANEL = kTile * 128, PANEL = BLK * 128;
   static constexpr int QTILE = PANELS * QPANEL, OPERAND = PANELS * PANEL;
-  static constexpr int STAGES = (TILES == 2 ? 5 : 4) * (128 / DP);  // K and V blocks in flight
+  static constexpr int STAGES = 4 * (128 / DP);  // K and V blocks in flight
+  static constexpr int OUT = 2048;                   // staging of an output warp: 32 rows x 64 bytes
   static constexpr int OFF_KV = TILES * QTILE;
-  static constexpr int OFF_BAR = OFF_KV + STAGES * OPERAND;
-  static constexpr int SMEM = OFF_BAR + 512 + 1024;
+  static constexpr int OFF_OUT = OFF_KV + STAGES * OPERAND;
+  static constexpr int OFF_BAR = OFF_OUT + TILES * 4 * OUT;
+  static constexpr int SMEM = OFF_BAR + 768 + 1024;
   static constexpr int COLS = TILES * 256;          // TMEM columns: 128 of S per tile, then O
-  static_assert((2 * STAGES + (3 + NBUF + HALVES) * TILES + 1) * 8 + 4 <= 512, "barrier area");
   static_assert(2 * (SMEM + 1024) <= 233472 || TILES == 2, "two CTAs per SM");
   static_assert(SMEM <= 232448, "shared memory budget");
 };
@@ -194,11 +204,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
 // Two fp32 lanes per instruction.
 struct F2 {
   uint64_t v;
@@ -224,34 +229,36 @@ __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
 }
-// 2^x for x <= 126 (below -126 as at -126): x = i + f with i the nearest
-// integer, 2^f by the degree-4 polynomial of smallest relative error on
-// [-1/2, 1/2] (2.6e-6, from a Remez iteration), times 2^i built in the
-// exponent field. A product, not an integer addition to the exponent, so that
-// NaN stays NaN.
-__device__ __forceinline__ F2 exp2_poly(F2 x2) {
-  float x, y;
-  unpack(x2, x, y);
-  x2 = f2(max_nan(x, -126.0f), max_nan(y, -126.0f));
-  const F2 t = add2(x2, f2(12582912.0f, 12582912.0f));  // 1.5 * 2^23: i in the low bits
-  const F2 i = add2(t, f2(-12582912.0f, -12582912.0f));
-  const F2 f = fma2(i, f2(-1.0f, -1.0f), x2);
-  F2 p = fma2(f, f2(0.009570102207362652f, 0.009570102207362652f), f2(0.05591785907745361f, 0.05591785907745361f));
-  p = fma2(p, f, f2(0.240247443318367f, 0.240247443318367f));
-  p = fma2(p, f, f2(0.6931217908859253f, 0.6931217908859253f));
-  p = fma2(p, f, f2(0.9999992847442627f, 0.9999992847442627f));
-  float tx, ty;
-  unpack(t, tx, ty);
-  return mul2(p, f2(__uint_as_float((__float_as_uint(tx) << 23) + 0x3f800000u),
-                    __uint_as_float((__float_as_uint(ty) << 23) + 0x3f800000u)));
-}
-
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
           smem_u32(dst)),
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
+}
+
+// Cluster launch control: takes one CTA that has not started yet out of the
+// grid; the answer (16 bytes) arrives at `bar`. After an answer without a CTA
+// no further request is made.
+__device__ __forceinline__ void cancel_next_cta(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// Its index, -1 where there was none.
+__device__ __forceinline__ int cancelled_cta(const void* answer) {
+  int x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "mov.b32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n\t}"
+      : "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return x;
 }
 
 // Instruction descriptor, kind::f16: fp32 D, A and B of type T, M = 128; bit 16: B is MN-major.
@@ -297,6 +304,14 @@ __device__ __forceinline__ int blocks_of(const TcArgs& a, const Work& w, int t, 
   return (keys_of(a, w, min(w.lq, first + a.TQ) - 1) + blk - 1) / blk;
 }
 
+// A job as the TMA warp hands it to the others; n < 0 ends the CTA.
+struct Job {
+  Work w;
+  int head, split, j0, n;  // KV head, key split, its first block and blocks
+  int cnt[2];              // blocks of each tile
+};
+constexpr int kJobs = 3;   // jobs in the ring
+
 template <typename T, int DP, int TILES>
 __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
     fa_prompt_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -305,66 +320,43 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
   constexpr int STAGES = R::STAGES, BLK = R::BLK, NBUF = R::NBUF, HALVES = R::HALVES;
   constexpr int kMmaWarp = TILES * 4, kLoadWarp = kMmaWarp + 1;
   constexpr uint32_t kColO = TILES * 128;  // S of tile t, buffer x at 128 t + BLK x; O of tile t at kColO + DP t
-  const int head = blockIdx.x % a.Hkv;
-  Work w;
-  // later tiles of a causal sequence see more keys: they start first
-  if (!find_work(a, a.TQ * TILES, a.slots - 1 - blockIdx.x / a.Hkv, w)) return;
-
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + R::OFF_BAR);
-  uint64_t* kv_full = q_full + TILES;
+  uint64_t* job_full = reinterpret_cast<uint64_t*>(smem + R::OFF_BAR);
+  uint64_t* job_empty = job_full + kJobs;
+  uint64_t* q_full = job_empty + kJobs;      // [tile]: queries are there
+  uint64_t* q_empty = q_full + TILES;        // ... and no product reads them any more
+  uint64_t* kv_full = q_empty + TILES;
   uint64_t* kv_empty = kv_full + STAGES;
   uint64_t* s_full = kv_empty + STAGES;      // [tile][buffer]: S is there
   uint64_t* p_full = s_full + NBUF * TILES;  // [tile][half]: 64 keys of P are there
-  uint64_t* pv_done = p_full + HALVES * TILES;  // the tile's latest P V is done
-  uint64_t* o_full = pv_done + TILES;     // the tile's last P V is done
-  uint64_t* drained = o_full + TILES;     // all of the MMA warp's products and arrivals are done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  uint64_t* pv_done = p_full + HALVES * TILES;  // [tile]: the product of a block with V is done
+  uint64_t* o_empty = pv_done + TILES;       // [tile]: O is read, the next job may overwrite it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + TILES);
+  Job* jobs = reinterpret_cast<Job*>(tmem_slot + 2);
+  uint8_t* next = smem + R::OFF_BAR + 704;   // answer to a cancel request (16 bytes), and its barrier
+  uint64_t* next_full = reinterpret_cast<uint64_t*>(next + 16);
+  static_assert((2 * kJobs + 2 * STAGES + (4 + NBUF + HALVES) * TILES) * 8 + 8 + kJobs * sizeof(Job) <= 704, "barrier area");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // this split's range of key blocks, and its share of every tile
-  int cnt[TILES], n = 0;
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) cnt[t] = blocks_of(a, w, t, BLK), n = max(n, cnt[t]);
-  const int j0 = (int)((long long)n * blockIdx.y / a.splits), j1 = (int)((long long)n * (blockIdx.y + 1) / a.splits);
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) cnt[t] = max(0, min(cnt[t], j1) - j0);
-  n = j1 - j0;
-  // K and V blocks in the order they are used: K0 K1 V0 K2 V1 .. V(n - 1)
-  auto item_k = [&](int i) { return i == 0 ? 0 : 2 * i - 1; };
-  auto item_v = [&](int i) { return i + 1 == n ? 2 * i + 1 : 2 * i + 2; };
-  auto load_item = [&](int x) {
-    const bool is_v = x > 0 && ((x & 1) == 0 || x + 1 == 2 * n);
-    const int i = x == 0 ? 0 : is_v ? (x + 1 == 2 * n ? n - 1 : (x - 2) >> 1) : (x + 1) >> 1;
-    const int st = x % STAGES;
-    mbar_arrive_expect_tx(&kv_full[st], R::OPERAND);
-    for (int p = 0; p < R::PANELS; ++p)
-      tma_load_3d(smem + R::OFF_KV + st * R::OPERAND + p * R::PANEL, is_v ? &map_v : &map_k, p * 64, head,
-                  w.k0 + (j0 + i) * BLK, &kv_full[st]);
-  };
-  if (threadIdx.x == kLoadWarp * 32) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kJobs; ++i) {
+      mbar_init(&job_full[i], 1);
+      mbar_init(&job_empty[i], TILES * 4 + 1);
+    }
     for (int i = 0; i < TILES; ++i) {
       mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
       for (int x = 0; x < NBUF; ++x) mbar_init(&s_full[NBUF * i + x], 1);
       for (int x = 0; x < HALVES; ++x) mbar_init(&p_full[HALVES * i + x], 4);
       mbar_init(&pv_done[i], 1);
-      mbar_init(&o_full[i], 1);
+      mbar_init(&o_empty[i], 4);
     }
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
     }
-    mbar_init(drained, 1);
+    mbar_init(next_full, 1);
     fence_mbar_init();
-    // the first loads run under the rest of the set-up
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-      if (cnt[t] == 0) continue;
-      mbar_arrive_expect_tx(&q_full[t], R::PANELS * a.TQ * a.G * 128);
-      for (int p = 0; p < R::PANELS; ++p)
-        tma_load_3d(smem + t * R::QTILE + p * R::QPANEL, &map_q, p * 64, head * a.G, w.q0 + w.tok + t * a.TQ, &q_full[t]);
-    }
-    for (int x = 0; x < min(2 * n, STAGES); ++x) load_item(x);
   }
   // rows of a query tile that no token fills stay zero
   for (int i = threadIdx.x; i < TILES * R::PANELS * (kTile - a.TQ * a.G) * 8; i += R::THREADS) {
@@ -378,247 +370,361 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   bool dead = false;
+  // The K and V blocks of a job are loaded in the order they are used: K0 K1 V0
+  // K2 V1 .. V(n - 1); item numbers run on from job to job.
+  auto item_k = [](int i) { return i == 0 ? 0 : 2 * i - 1; };
+  auto item_v = [](int i, int n) { return i + 1 == n ? 2 * i + 1 : 2 * i + 2; };
+  // Job c, for the warps that work on it; they read it in place until they are
+  // done with it.
+  auto take_job = [&](int c) -> const Job& {
+    mbar_wait_or_poison(&job_full[c % kJobs], (c / kJobs) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+    return jobs[c % kJobs];
+  };
+  auto finish_job = [&](int c) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&job_empty[c % kJobs]);
+  };
 
-  // 384 x 168 registers at launch: 256 x 208 + 128 x 88
+  // 384 x 168 registers at launch: 256 x 216 + 128 x 72
   if constexpr (TILES == 2) {
-    if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp >= kMmaWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   }
   if (warp == kLoadWarp) {
-    if (lane == 0)
-      for (int x = STAGES; x < 2 * n; ++x) {
-        const int st = x % STAGES;
-        mbar_wait_idle_or_poison(&kv_empty[st], ((x / STAGES) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
-        load_item(x);
+    if (lane == 0) {
+      tc::prefetch_tmap(&map_q);
+      tc::prefetch_tmap(&map_k);
+      tc::prefetch_tmap(&map_v);
+    }
+    int c = 0, items = 0, queries[TILES];  // jobs, K / V blocks and query tiles so far
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) queries[t] = 0;
+    auto push = [&](const Job& j) {
+      if (c >= kJobs) mbar_wait_idle_or_poison(&job_empty[c % kJobs], ((c / kJobs) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
+      __syncwarp();
+      if (lane == 0) {
+        jobs[c % kJobs] = j;
+        mbar_arrive(&job_full[c % kJobs]);
       }
+      ++c;
+    };
+    // The CTA's first job is its own index; further ones are those of CTAs that
+    // have not started yet, which it cancels one by one (later tiles of a
+    // causal sequence see more keys and have the lower indexes). A job is taken
+    // once the loads of the last one are out: late enough for an even end.
+    for (int id = blockIdx.x, round = 0; id >= 0 && !dead; ++round) {
+      Job j;
+      j.head = id % a.Hkv;
+      j.split = id / a.Hkv % a.splits;
+      const bool real = find_work(a, a.TQ * TILES, a.slots - 1 - id / a.Hkv / a.splits, j.w);
+      if (real) {
+        int n = 0;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) j.cnt[t] = blocks_of(a, j.w, t, BLK), n = max(n, j.cnt[t]);
+        j.j0 = (int)((long long)n * j.split / a.splits);
+        const int j1 = (int)((long long)n * (j.split + 1) / a.splits);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) j.cnt[t] = max(0, min(j.cnt[t], j1) - j.j0);
+        j.n = n = j1 - j.j0;
+        push(j);
+        if (lane == 0) {
+#pragma unroll
+          for (int t = 0; t < TILES; ++t) {
+            if (j.cnt[t] == 0) continue;
+            if (queries[t] > 0) mbar_wait_idle_or_poison(&q_empty[t], (queries[t] - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
+            ++queries[t];
+            mbar_arrive_expect_tx(&q_full[t], R::PANELS * a.TQ * a.G * 128);
+            for (int p = 0; p < R::PANELS; ++p)
+              tma_load_3d(smem + t * R::QTILE + p * R::QPANEL, &map_q, p * 64, j.head * a.G, j.w.q0 + j.w.tok + t * a.TQ,
+                          &q_full[t]);
+          }
+          for (int x = 0; x < 2 * n; ++x, ++items) {
+            const bool is_v = x > 0 && ((x & 1) == 0 || x + 1 == 2 * n);
+            const int i = x == 0 ? 0 : is_v ? (x + 1 == 2 * n ? n - 1 : (x - 2) >> 1) : (x + 1) >> 1;
+            const int st = items % STAGES;
+            if (items >= STAGES)
+              mbar_wait_idle_or_poison(&kv_empty[st], ((items / STAGES) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
+            mbar_arrive_expect_tx(&kv_full[st], R::OPERAND);
+            for (int p = 0; p < R::PANELS; ++p)
+              tma_load_3d(smem + R::OFF_KV + st * R::OPERAND + p * R::PANEL, is_v ? &map_v : &map_k, p * 64, j.head,
+                          j.w.k0 + (j.j0 + i) * BLK, &kv_full[st]);
+          }
+        }
+      }
+      if (lane == 0) {
+        mbar_arrive_expect_tx(next_full, 16);
+        cancel_next_cta(next, next_full);
+        mbar_wait_idle_or_poison(next_full, round & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        id = dead ? -1 : cancelled_cta(next);
+        fence_proxy_async_smem();  // read before it is written again
+      }
+      id = __shfl_sync(0xffffffffu, id, 0);
+      dead = __shfl_sync(0xffffffffu, (int)dead, 0) != 0;
+    }
+    Job last{};
+    last.n = -1;
+    push(last);
+    if (lane == 0) {
+      // the releases that no load waited for
+      for (int x = max(0, items - STAGES); x < items; ++x)
+        mbar_wait_idle_or_poison(&kv_empty[x % STAGES], (x / STAGES) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+        if (queries[t] > 0) mbar_wait_idle_or_poison(&q_empty[t], (queries[t] - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
+    }
     __syncwarp();
   } else if (warp == kMmaWarp) {
     constexpr uint32_t idesc_s = idesc<T>(BLK, false), idesc_o = idesc<T>(DP, true);
     const uint32_t q_base = smem_u32(smem), kv_base = q_base + R::OFF_KV;
     const uint32_t go = tc::elect_one();
-    // S_t = Q_t K_i^T into buffer i % NBUF
-    auto score = [&](int t, int i) {
-      const int st = item_k(i) % STAGES;
-      mbar_wait_or_poison(&kv_full[st], (item_k(i) / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
-      if (i == 0) mbar_wait_or_poison(&q_full[t], 0, a.err, DEV_TIMEOUT_FULL, dead);
-      tc::tc_fence_after();
-      const uint64_t kd = tc::sw128_desc(kv_base + st * R::OPERAND), qd = tc::sw128_desc(q_base + t * R::QTILE);
+    int items = 0, done[TILES], queries[TILES];  // K / V blocks of earlier jobs; blocks and jobs of each tile so far
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k)
-        tc::mma_ss_go(tmem + t * 128 + (i % NBUF) * BLK, qd + (uint64_t)((k >> 2) * (R::QPANEL >> 4) + (k & 3) * 2),
-                      kd + (uint64_t)((k >> 2) * (R::PANEL >> 4) + (k & 3) * 2), idesc_s, k > 0, go);
-      tc::mma_commit_go(&s_full[NBUF * t + i % NBUF], go);
-    };
-    // Every arrival must have come before the CTA ends: with two CTAs on an SM
-    // their products share one queue, and an arrival behind the other CTA's
-    // products would land in the next CTA's shared memory. So a stage is only
-    // released to a load that waits for it, and the warp drains at the end.
-    auto release = [&](int item) {
-      if (item + STAGES < 2 * n) tc::mma_commit_go(&kv_empty[item % STAGES], go);
-    };
-    if (n > 0) {
+    for (int t = 0; t < TILES; ++t) done[t] = queries[t] = 0;
+    for (int c = 0;; ++c) {
+      const Job& j = take_job(c);
+      if (dead || j.n < 0) break;
+      const int n = j.n;
+      // S_t = Q_t K_i^T into the tile's next buffer
+      auto score = [&](int t, int i) {
+        const int x = items + item_k(i), st = x % STAGES, u = done[t] + i;
+        mbar_wait_or_poison(&kv_full[st], (x / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        if (i == 0) mbar_wait_or_poison(&q_full[t], queries[t] & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        tc::tc_fence_after();
+        const uint64_t kd = tc::sw128_desc(kv_base + st * R::OPERAND), qd = tc::sw128_desc(q_base + t * R::QTILE);
 #pragma unroll
-      for (int t = 0; t < TILES; ++t)
-        if (cnt[t] > 0) score(t, 0);
-      release(0);
-    }
-    for (int i = 0; i < n; ++i) {
-      if (NBUF == 2 && i + 1 < n) {
-        // the other buffer held P of block i - 1, whose product was issued before
+        for (int k = 0; k < DP / 16; ++k)
+          tc::mma_ss_go(tmem + t * 128 + (u % NBUF) * BLK, qd + (uint64_t)((k >> 2) * (R::QPANEL >> 4) + (k & 3) * 2),
+                        kd + (uint64_t)((k >> 2) * (R::PANEL >> 4) + (k & 3) * 2), idesc_s, k > 0, go);
+        tc::mma_commit_go(&s_full[NBUF * t + u % NBUF], go);
+        if (i + 1 == j.cnt[t]) tc::mma_commit_go(&q_empty[t], go);
+      };
+      auto release = [&](int x) { tc::mma_commit_go(&kv_empty[(items + x) % STAGES], go); };
+      if (n > 0) {
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
-          if (i + 1 < cnt[t]) score(t, i + 1);
-        release(item_k(i + 1));
+          if (j.cnt[t] > 0) score(t, 0);
+        release(0);
       }
-      const int st = item_v(i) % STAGES;
-      mbar_wait_or_poison(&kv_full[st], (item_v(i) / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
-      const uint64_t vd = tc::sw128_desc_mn(kv_base + st * R::OPERAND, R::PANEL);  // dims across, tokens down
+      for (int i = 0; i < n; ++i) {
+        if (NBUF == 2 && i + 1 < n) {
+          // the other buffer held P of block i - 1, whose product was issued before
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        if (i >= cnt[t]) continue;
-#pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
-          mbar_wait_or_poison(&p_full[HALVES * t + h], i & 1, a.err, DEV_TIMEOUT_FULL, dead);
-          tc::tc_fence_after();
-#pragma unroll
-          for (int k = 4 * h; k < 4 * h + 4; ++k)
-            tc::mma_ts_go(tmem + kColO + t * DP, tmem + t * 128 + (i % NBUF) * BLK + 8 * k, vd + (uint64_t)(k * (2048 >> 4)),
-                          idesc_o, (i > 0 || k > 0) ? 1u : 0u, go);
+          for (int t = 0; t < TILES; ++t)
+            if (i + 1 < j.cnt[t]) score(t, i + 1);
+          release(item_k(i + 1));
         }
-        tc::mma_commit_go(i + 1 == cnt[t] ? &o_full[t] : &pv_done[t], go);
-        // one buffer: the next scores take the place of the P just consumed (the products run in order)
-        if (NBUF == 1 && i + 1 < cnt[t]) score(t, i + 1);
+        const int x = items + item_v(i, n), st = x % STAGES;
+        mbar_wait_or_poison(&kv_full[st], (x / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        const uint64_t vd = tc::sw128_desc_mn(kv_base + st * R::OPERAND, R::PANEL);  // dims across, tokens down
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+          if (i >= j.cnt[t]) continue;
+          const int u = done[t] + i;
+          if (i == 0 && queries[t] > 0)  // the tile's last O is read
+            mbar_wait_or_poison(&o_empty[t], (queries[t] - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
+#pragma unroll
+          for (int h = 0; h < HALVES; ++h) {
+            mbar_wait_or_poison(&p_full[HALVES * t + h], u & 1, a.err, DEV_TIMEOUT_FULL, dead);
+            tc::tc_fence_after();
+#pragma unroll
+            for (int k = 4 * h; k < 4 * h + 4; ++k)
+              tc::mma_ts_go(tmem + kColO + t * DP, tmem + t * 128 + (u % NBUF) * BLK + 8 * k, vd + (uint64_t)(k * (2048 >> 4)),
+                            idesc_o, (i > 0 || k > 0) ? 1u : 0u, go);
+          }
+          tc::mma_commit_go(&pv_done[t], go);
+          // one buffer: the next scores take the place of the P just consumed (the products run in order)
+          if (NBUF == 1 && i + 1 < j.cnt[t]) score(t, i + 1);
+        }
+        release(item_v(i, n));
+        if (NBUF == 1 && i + 1 < n) release(item_k(i + 1));
       }
-      release(item_v(i));
-      if (NBUF == 1 && i + 1 < n) release(item_k(i + 1));
+      items += 2 * n;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) done[t] += j.cnt[t], queries[t] += j.cnt[t] > 0;
+      finish_job(c);
     }
-    tc::mma_commit_go(drained, go);
-    mbar_wait_idle_or_poison(drained, 0, a.err, DEV_TIMEOUT_FULL, dead);
     __syncwarp();
   } else if (warp < kMmaWarp) {
-    if constexpr (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int t = warp >> 2, row = threadIdx.x & 127, nt = cnt[TILES == 2 ? t : 0];
+    if constexpr (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const int t = warp >> 2, row = threadIdx.x & 127, rt = row / a.G, g = row % a.G;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + t * 128, o_addr = tmem + lanes + kColO + t * DP;
-    const int first = w.tok + t * a.TQ;                     // the tile's first token
-    const int tok = first + row / a.G, g = row % a.G;
-    const bool mine = row < a.TQ * a.G && tok < w.lq;
-    const int keys = mine ? keys_of(a, w, tok) : 0;
-    const int all_see = keys_of(a, w, first);               // keys that every row of the tile sees
-    float m = -INFINITY;
-    F2 l2 = f2(0.0f, 0.0f);
-    for (int i = 0; i < nt; ++i) {
-      const int key0 = (j0 + i) * BLK;
-      const uint32_t sp = s_addr + (i % NBUF) * BLK;
-      mbar_wait_or_poison(&s_full[NBUF * t + i % NBUF], (i / NBUF) & 1, a.err, DEV_TIMEOUT_FULL, dead);
-      __syncwarp();
-      tc::tc_fence_after();
-      uint32_t s[BLK];
-#pragma unroll
-      for (int c = 0; c < BLK; c += 32) tc::tmem_ld32(sp + c, *reinterpret_cast<uint32_t(*)[32]>(s + c));
-      tc::tmem_ld_wait();
-      if (a.flip) {
-#pragma unroll
-        for (int x = 0; x < BLK; ++x) s[x] ^= a.flip;
-      }
-      if (key0 + BLK > all_see) {
-        const int lim = keys - key0;
-#pragma unroll
-        for (int x = 0; x < BLK; ++x)
-          if (x >= lim) s[x] = 0xff800000u;
-        const int valid = w.lk - key0;
-        if (valid < BLK) {
-          // rows of V behind the sequence's end belong to others: what they
-          // hold must not meet P (0 x inf); both tiles write the same zeros
-          const int st = item_v(i) % STAGES;
-          mbar_wait_or_poison(&kv_full[st], (item_v(i) / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
-          for (int x = row; x < (BLK - valid) * 8 * R::PANELS; x += kTile) {
-            const int c = x % 8, p = x / 8 % R::PANELS, r = valid + x / (8 * R::PANELS);
-            *reinterpret_cast<uint4*>(smem + R::OFF_KV + st * R::OPERAND + p * R::PANEL + r * 128 + c * 16) =
-                make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-        }
-      }
-      float mx[8];
-#pragma unroll
-      for (int x = 0; x < 8; ++x) mx[x] = fmaxf(__uint_as_float(s[x]), __uint_as_float(s[x + 8]));
-#pragma unroll
-      for (int x = 16; x < BLK; x += 16)
-#pragma unroll
-        for (int y = 0; y < 8; ++y) mx[y] = max3(mx[y], __uint_as_float(s[x + y]), __uint_as_float(s[x + y + 8]));
-      const float mn = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * a.sl;
-      float f = 1.0f;
-      if (mn > m + kLazy) {  // also the row's first keys (m = -inf)
-        f = ex2(m - mn);
-        m = mn;
-        l2 = mul2(l2, f2(f, f));
-      }
-      if (i > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
-        // the product before the latest one is done (S of this block came after it)
-        mbar_wait_or_poison(&pv_done[t], (i - 1) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+    uint8_t* stage = smem + R::OFF_OUT + warp * R::OUT;
+    int items = 0, done = 0;  // K / V blocks of earlier jobs, this tile's blocks so far
+    for (int c = 0;; ++c) {
+      const Job& j = take_job(c);
+      if (dead || j.n < 0) break;
+      const Work& w = j.w;
+      const int nt = j.cnt[t];
+      const int first = w.tok + t * a.TQ;                     // the tile's first token
+      const int tok = first + rt;
+      const bool mine = row < a.TQ * a.G && tok < w.lq;
+      const int keys = mine ? keys_of(a, w, tok) : 0;
+      const int all_see = keys_of(a, w, first);               // keys that every row of the tile sees
+      float m = -INFINITY;
+      F2 l2 = f2(0.0f, 0.0f);
+      for (int i = 0; i < nt; ++i) {
+        const int key0 = (j.j0 + i) * BLK, u = done + i;
+        const uint32_t sp = s_addr + (u % NBUF) * BLK;
+        mbar_wait_or_poison(&s_full[NBUF * t + u % NBUF], (u / NBUF) & 1, a.err, DEV_TIMEOUT_FULL, dead);
         __syncwarp();
         tc::tc_fence_after();
-#pragma unroll 1
-        for (int c = 0; c < DP / 32; ++c) {
-          uint32_t o[32];
-          tc::tmem_ld32(o_addr + 32 * c, o);
-          tc::tmem_ld_wait();
+        uint32_t s[BLK];
 #pragma unroll
-          for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-          tc::tmem_st32(o_addr + 32 * c, o);
+        for (int x = 0; x < BLK; x += 32) tc::tmem_ld32(sp + x, *reinterpret_cast<uint32_t(*)[32]>(s + x));
+        tc::tmem_ld_wait();
+        if (a.flip) {
+#pragma unroll
+          for (int x = 0; x < BLK; ++x) s[x] ^= a.flip;
         }
-      }
-      const float off = m == -INFINITY ? 0.0f : kBias - m;
-      const F2 sl2 = f2(a.sl, a.sl), off2 = f2(off, off);
-      F2 sum = f2(0.0f, 0.0f);
+        if (key0 + BLK > all_see) {
+          const int lim = keys - key0;
 #pragma unroll
-      for (int h = 0; h < HALVES; ++h) {
-        uint32_t p[32];
+          for (int x = 0; x < BLK; ++x)
+            if (x >= lim) s[x] = 0xff800000u;
+          const int valid = w.lk - key0;
+          if (valid < BLK) {
+            // rows of V behind the sequence's end belong to others: what they
+            // hold must not meet P (0 x inf); both tiles write the same zeros
+            const int v = items + item_v(i, j.n), st = v % STAGES;
+            mbar_wait_or_poison(&kv_full[st], (v / STAGES) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+            for (int x = row; x < (BLK - valid) * 8 * R::PANELS; x += kTile) {
+              const int y = x % 8, p = x / 8 % R::PANELS, r = valid + x / (8 * R::PANELS);
+              *reinterpret_cast<uint4*>(smem + R::OFF_KV + st * R::OPERAND + p * R::PANEL + r * 128 + y * 16) =
+                  make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
+        }
+        float mx[8];
 #pragma unroll
-        for (int x = 0; x < 32; ++x) {
-          F2 e = fma2(f2(__uint_as_float(s[64 * h + 2 * x]), __uint_as_float(s[64 * h + 2 * x + 1])), sl2, off2);
-          float e0, e1;
-          // the polynomial's elements are spread among the others
-          if (x * kPoly / 64 != (x + 1) * kPoly / 64) {
-            e = exp2_poly(e);
-            unpack(e, e0, e1);
-          } else {
+        for (int x = 0; x < 8; ++x) mx[x] = fmaxf(__uint_as_float(s[x]), __uint_as_float(s[x + 8]));
+#pragma unroll
+        for (int x = 16; x < BLK; x += 16)
+#pragma unroll
+          for (int y = 0; y < 8; ++y) mx[y] = max3(mx[y], __uint_as_float(s[x + y]), __uint_as_float(s[x + y + 8]));
+        const float mn = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * a.sl;
+        float f = 1.0f;
+        if (mn > m + kLazy) {  // also the row's first keys (m = -inf)
+          f = ex2(m - mn);
+          m = mn;
+          l2 = mul2(l2, f2(f, f));
+        }
+        // Before O is touched the product of the block before must be done. With
+        // one buffer it is, as S came after it; with two, its arrival (normally
+        // long there) is taken before this block's P goes out, so that none is
+        // missed.
+        if (NBUF == 2 && i > 0) mbar_wait_or_poison(&pv_done[t], (u - 1) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        if (i > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
+          __syncwarp();
+          tc::tc_fence_after();
+#pragma unroll 1
+          for (int x = 0; x < DP / 16; ++x) {  // (small pieces: the scores are still in registers)
+            uint32_t o[16];
+            tc::tmem_ld16(o_addr + 16 * x, o);
+            tc::tmem_ld_wait();
+#pragma unroll
+            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+            tc::tmem_st16(o_addr + 16 * x, o);
+          }
+        }
+        const float off = m == -INFINITY ? 0.0f : kBias - m;
+        const F2 sl2 = f2(a.sl, a.sl), off2 = f2(off, off);
+        F2 sum = f2(0.0f, 0.0f);
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          uint32_t p[32];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            const F2 e = fma2(f2(__uint_as_float(s[64 * h + 2 * x]), __uint_as_float(s[64 * h + 2 * x + 1])), sl2, off2);
+            float e0, e1;
             unpack(e, e0, e1);
             e0 = ex2(e0), e1 = ex2(e1);
-            e = f2(e0, e1);
+            sum = add2(sum, f2(e0, e1));
+            p[x] = pack2<T>(e0, e1);
           }
-          sum = add2(sum, e);
-          p[x] = pack2<T>(e0, e1);
+          __syncwarp();
+          tc::tmem_st32(sp + 32 * h, p);
+          tc::tmem_st_wait();
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[HALVES * t + h]);
         }
-        __syncwarp();
-        tc::tmem_st32(sp + 32 * h, p);
-        tc::tmem_st_wait();
-        tc::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[HALVES * t + h]);
+        l2 = add2(l2, sum);
       }
-      l2 = add2(l2, sum);
-    }
-    float l, l1;
-    unpack(l2, l, l1);
-    l += l1;
-    if (nt > 0) {
-      mbar_wait_or_poison(&o_full[t], 0, a.err, DEV_TIMEOUT_FULL, dead);
-      __syncwarp();
-      tc::tc_fence_after();
-    }
-    const bool none = m == -INFINITY && l == l;             // no key seen (a NaN score is one)
-    // Rows leave through shared memory (the tile's queries are done with), 128
-    // bytes of each at a time, so that a warp's store covers 4 whole lines; a
-    // thread's own row would be 32 scattered pieces of 16 bytes.
-    const long long at = mine ? (long long)(w.q0 + tok) * a.Hq + head * a.G + g : -1;
-    uint8_t* stage = smem + t * R::QTILE + (warp & 3) * 4096;
-    const float inv = 1.0f / l;
-    const bool partial = a.splits > 1;
-    const int cols = partial ? 32 : 64, item = partial ? 4 : 2;  // columns of 128 bytes, bytes of an element
-    uint8_t* base = partial ? reinterpret_cast<uint8_t*>(a.part + (long long)blockIdx.y * a.Tq * a.Hq * a.D)
-                            : static_cast<uint8_t*>(a.out);
-    if (partial && mine)
-      a.ml[(long long)blockIdx.y * a.Tq * a.Hq + at] = make_float2(none ? -INFINITY : m, none ? 0.0f : l);
-#pragma unroll 1
-    for (int c = 0; c < a.D; c += cols) {
-      __syncwarp();
+      done += nt;
+      items += 2 * j.n;
+      float l, l1;
+      unpack(l2, l, l1);
+      l += l1;
+      if (nt > 0) {
+        mbar_wait_or_poison(&pv_done[t], (done - 1) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        __syncwarp();
+        tc::tc_fence_after();
+      }
+      const bool none = m == -INFINITY && l == l;             // no key seen (a NaN score is one)
+      // Rows leave through shared memory, 64 bytes of each at a time: a warp's
+      // store then covers 8 row pieces of 64 bytes (a thread's own row would
+      // be 32 scattered pieces of 16).
+      const int at = mine ? (w.q0 + tok) * a.Hq + j.head * a.G + g : -1;
+      const float inv = 1.0f / l;
+      const bool partial = a.splits > 1;
+      const int cols = partial ? 16 : 32, item = partial ? 4 : 2;  // columns of 64 bytes, bytes of an element
+      uint8_t* base = partial ? reinterpret_cast<uint8_t*>(a.part + (long long)j.split * a.Tq * a.Hq * a.D)
+                              : static_cast<uint8_t*>(a.out);
+      if (partial && mine)
+        a.ml[(long long)j.split * a.Tq * a.Hq + at] = make_float2(none ? -INFINITY : m, none ? 0.0f : l);
+      uint8_t* dst[4];                                        // of the pieces this lane stores, rows lane / 4 + 8 x
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (half == 1 && partial) break;
+      for (int x = 0; x < 4; ++x) {
+        const int r = __shfl_sync(0xffffffffu, at, 8 * x + (lane >> 2));
+        dst[x] = r >= 0 ? base + (long long)r * a.D * item + (lane & 3) * 16 : nullptr;
+      }
+#pragma unroll 1
+      for (int x0 = 0; x0 < a.D; x0 += 32) {
         uint32_t o[32];
+        __syncwarp();
         if (nt > 0) {
-          tc::tmem_ld32(o_addr + c + 32 * half, o);
+          tc::tmem_ld32(o_addr + x0, o);
           tc::tmem_ld_wait();
+          if (x0 + 32 >= a.D) {
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_empty[t]);
+          }
+        }
+        if (none) {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = 0;
+        }
+        if (!partial) {
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            o[x] = none ? 0u : pack2<T>(__uint_as_float(o[2 * x]) * inv, __uint_as_float(o[2 * x + 1]) * inv);
         }
 #pragma unroll
-        for (int x = 0; x < 32; ++x)
-          if (none) o[x] = 0;
-        if (partial) {
+        for (int half = 0; half < 2; ++half) {
+          if (half == 1 && !partial) break;
+          __syncwarp();
+          // piece c of row r lies at c ^ (r / 2 % 4): eight rows hit distinct banks
 #pragma unroll
-          for (int x = 0; x < 8; ++x)
-            *reinterpret_cast<uint4*>(stage + lane * 128 + ((x ^ (lane & 7)) << 4)) =
-                make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
-        } else {
+          for (int x = 0; x < 4; ++x)
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((x ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(o[16 * half + 4 * x], o[16 * half + 4 * x + 1], o[16 * half + 4 * x + 2], o[16 * half + 4 * x + 3]);
+          __syncwarp();
+          uint4 v[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            uint32_t v[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y)
-              v[y] = none ? 0u : pack2<T>(__uint_as_float(o[8 * x + 2 * y]) * inv, __uint_as_float(o[8 * x + 2 * y + 1]) * inv);
-            *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * half + x) ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+            const int r = 8 * x + (lane >> 2);
+            v[x] = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
           }
+          const int col = x0 + cols * half;
+          const bool inside = (col * item + (lane & 3) * 16) < a.D * item;
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (dst[x] && inside) *reinterpret_cast<uint4*>(dst[x] + col * item) = v[x];
         }
       }
-      __syncwarp();
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const int r = 4 * x + (lane >> 3), piece = lane & 7;
-        const long long dst = __shfl_sync(0xffffffffu, at, r);
-        const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
-        if (dst >= 0 && c * item + piece * 16 < a.D * item)
-          *reinterpret_cast<uint4*>(base + (dst * a.D + c) * item + piece * 16) = v;
-      }
+      finish_job(c);
     }
   }
   tc::tc_fence_before();
@@ -674,7 +780,7 @@ bool tma_rows(const void* p, int H, int64_t T, int64_t head, int64_t row) {
 }
 
 bool tc_supported(const FaPromptArgs& a) {
-  return a.D <= 128 && a.Hq / a.Hkv <= kTile && a.Tk > 0 && tma_rows(a.q, a.Hq, a.Tq, a.q_head, a.q_row) &&
+  return a.D <= 128 && a.Hq / a.Hkv <= kTile && a.Tk > 0 && (int64_t)a.Tq * a.Hq <= INT32_MAX && tma_rows(a.q, a.Hq, a.Tq, a.q_head, a.q_row) &&
          tma_rows(a.k, a.Hkv, a.Tk, a.k_head, a.k_row) && tma_rows(a.v, a.Hkv, a.Tk, a.v_head, a.v_row);
 }
 
@@ -721,7 +827,7 @@ kq_status_t launch_tc(const FaPromptArgs& a, int dtype, const Plan& plan, cudaSt
     return fail(KQ_ERR_CUDA, "fa_prompt: tensor map encoding failed");
   auto kernel = fa_prompt_tc_kernel<T, DP, TILES>;
   if (kq_status_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), R::SMEM, "fa_prompt")) return st;
-  kernel<<<dim3((unsigned)(p.slots * a.Hkv), (unsigned)p.splits), R::THREADS, R::SMEM, s>>>(mq, mk, mv, p);
+  kernel<<<(unsigned)(plan.slots * a.Hkv * plan.splits), R::THREADS, R::SMEM, s>>>(mq, mk, mv, p);
   if (kq_status_t st = check_launch("fa_prompt_tc")) return st;
   if (p.splits == 1) return KQ_OK;
   cudaLaunchConfig_t cfg{};
