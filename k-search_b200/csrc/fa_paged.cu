@@ -8,25 +8,21 @@
 // through row 0 of the table. q8_0 values are d * code; the softmax state and
 // the output accumulate in fp32. A sequence of length 0 yields zeros; a page
 // id outside the cache hides its tokens.
-#include <cuda_bf16.h>
-
 #include <algorithm>
 #include <cmath>
 
 #include "kq_internal.h"
+#include "kq_attn.cuh"
 #include "kq_device.cuh"
 #include "kq_tc.cuh"
 
 namespace kq {
 namespace {
 
+using namespace attn;
+
 constexpr int kQ8 = 34;
 constexpr int kMaxNB = 8;
-
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void store_f(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void store_f(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 // ---- work split ------------------------------------------------------------------
 // Tokens start .. n_b - 1 of every sequence (n_b its length, cut to max_seqlen
@@ -172,11 +168,6 @@ struct StreamArgs {
   float2* ml;   // [segment][Hq] maximum (log2 units), sum
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // d = a b + (c0, c1, c2, c3)
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1, float c0, float c1, float c2, float c3) {
@@ -188,10 +179,6 @@ __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
-}
-__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 // 4 codes (one word) -> two fp16 pairs: 0x64uu is 1024 + uu, uu = code + 128.
 __device__ __forceinline__ void codes_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -368,8 +355,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1) fa_paged_stream_kernel(cons
         sl[r] *= __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i) {
-          w[i].x = pack_h2(__uint_as_float(w[i].x << 16) * down, __uint_as_float(w[i].x & 0xffff0000u) * down);
-          w[i].y = pack_h2(__uint_as_float(w[i].y << 16) * down, __uint_as_float(w[i].y & 0xffff0000u) * down);
+          w[i].x = pack2<__half>(__uint_as_float(w[i].x << 16) * down, __uint_as_float(w[i].x & 0xffff0000u) * down);
+          w[i].y = pack2<__half>(__uint_as_float(w[i].y << 16) * down, __uint_as_float(w[i].y & 0xffff0000u) * down);
         }
       }
 #pragma unroll
@@ -505,8 +492,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1) fa_paged_stream_kernel(cons
         uint32_t pa[2 * RH];
 #pragma unroll
         for (int r = 0; r < RH; ++r) {
-          pa[r] = pack_h2(p[0][2 * r] * d0.x, p[0][2 * r + 1] * d0.y);
-          pa[RH + r] = pack_h2(p[1][2 * r] * d1.x, p[1][2 * r + 1] * d1.y);
+          pa[r] = pack2<__half>(p[0][2 * r] * d0.x, p[0][2 * r + 1] * d0.y);
+          pa[RH + r] = pack2<__half>(p[1][2 * r] * d1.x, p[1][2 * r + 1] * d1.y);
         }
         // byte i of the two tokens of a pair, for the 4 dims of the word
         const uint32_t x01 = __byte_perm(w[0], w[1], 0x5140), x23 = __byte_perm(w[0], w[1], 0x7362);
@@ -567,11 +554,11 @@ __global__ void __launch_bounds__(kStreamThreads, 1) fa_paged_stream_kernel(cons
 //
 // Warps: 0-3 / 4-7 softmax of tile 0 / 1, 8 MMA issue and TMEM, 9-16 copy and
 // dequantise 8 tokens of each block (a block of 32 values per thread), each
-// from its own ring of rows. 64-token blocks keep S at 64 registers per row,
-// so that 17 warps fit.
+// from its own ring of rows; 17-19 idle (they complete the last warpgroup).
+// Registers: 640 x 96 at launch, 256 x 144 + 384 x 64 after the split.
 constexpr int kBlk = 64;
 constexpr int kTile = 128;
-constexpr int kPrefixThreads = 544;
+constexpr int kPrefixThreads = 640;
 constexpr int kMmaWarp = 8, kDeqWarp = 9, kDeqWarps = 8;
 constexpr float kBias = 7.0f, kLazy = 8.0f;
 constexpr int kRaw = 6, kOps = 4;      // raw and operand stages (K and V alternate)
@@ -586,7 +573,8 @@ struct PrefixTraits {
   static constexpr int OP = PART * (LO ? 2 : 1);
   static constexpr int RAW = kBlk * Row<NB>::PITCH;
   static constexpr int OFF_RAW = kOps * OP;
-  static constexpr int OFF_BAR = OFF_RAW + kRaw * RAW;
+  static constexpr int OFF_STAGE = OFF_RAW + kRaw * RAW;  // 2 KB per softmax warp
+  static constexpr int OFF_BAR = OFF_STAGE + 8 * 2048;
   static constexpr int SMEM = OFF_BAR + 512 + 1024;
   static_assert(SMEM <= 232448, "shared memory budget");
   static_assert(OFF_RAW % 1024 == 0 && OFF_BAR % 16 == 0, "alignment");
@@ -669,7 +657,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
   const int head_off = h * Row<NB>::BYTES, row15 = (int)(row_bytes & 15);
   bool dead = false;
 
-  if (warp >= kDeqWarp) {
+  if (warp >= 2 * 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  if (warp >= kDeqWarp + kDeqWarps) {
+    // idle
+  } else if (warp >= kDeqWarp) {
     // ---- one block of 32 values per thread: token 8 w + lane % 8, block lane / 8
     const int dw = warp - kDeqWarp, tok = dw * 8 + (lane & 7), blk = lane >> 3;
     const int off = (((lane & 7) * row15 + head_off) & 15) + blk * kQ8;
@@ -824,55 +815,67 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
     __syncwarp();
   } else {
     // ---- softmax, a thread per row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     const int t = warp >> 2, r = row0 + threadIdx.x, b = r / a.G, gq = r % a.G;
     if (t == 0 || two) {
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t s_addr = tmem + lanes + kColS + t * kBlk, o_addr = tmem + lanes + kColO + t * DP;
       const bool mine = r < rows;
       const int keys = mine ? max(0, min(min(a.seq_lens[b], a.limit), a.prefix_len)) : 0;
-      const long long qrow = (long long)(mine ? b : 0) * a.Hq + h * a.G + (mine ? gq : 0);
+      const int qrow = mine ? b * a.Hq + h * a.G + gq : -1;
+      uint8_t* stage = smem + R::OFF_STAGE + warp * 2048;
+      int other[4];  // rows whose pieces this lane moves
+#pragma unroll
+      for (int x = 0; x < 4; ++x) other[x] = __shfl_sync(0xffffffffu, qrow, 8 * x + (lane >> 2));
       float sl = a.sl;
       {
-        // the row's queries to TMEM (two fp16 per column), dims past D zero
-        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + qrow * (NB * 32));
-        float down = 1.0f;
-        if (a.q_bf16 && mine) {
+        // the row's queries to TMEM (two fp16 per column), dims past D zero:
+        // all loads in flight at once, through the stage to the row's thread
+        uint4 v[NB][4];
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            v[j][x] = other[x] >= 0 ? reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                                                     (long long)other[x] * (NB * 32) + 32 * j)[lane & 3]
+                                    : make_uint4(0, 0, 0, 0);
+        uint32_t w[DP / 2];
+#pragma unroll
+        for (int j = 0; j < DP / 32; ++j) {
+          if (j < NB) {
+            __syncwarp();
+#pragma unroll
+            for (int x = 0; x < 4; ++x) *stage_piece(stage, lane, x) = v[j < NB ? j : 0][x];
+            __syncwarp();
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint4 y = j < NB ? *stage_row(stage, lane, x) : make_uint4(0, 0, 0, 0);
+            w[16 * j + 4 * x] = y.x, w[16 * j + 4 * x + 1] = y.y, w[16 * j + 4 * x + 2] = y.z, w[16 * j + 4 * x + 3] = y.w;
+          }
+        }
+        if (a.q_bf16) {
           float top = 0.0f;
-#pragma unroll 4
-          for (int i = 0; i < NB * 4; ++i) {
-            const uint4 w = q[i];
-            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              top = fmaxf(top, fmaxf(fabsf(__uint_as_float(v[x] << 16)), fabsf(__uint_as_float(v[x] & 0xffff0000u))));
-          }
+          for (int i = 0; i < DP / 2; ++i)
+            top = max3(top, fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u)));
           const int e = min(max((int)(__float_as_uint(top) >> 23) - 127 - 14, -100), 100);
-          down = __uint_as_float((uint32_t)(127 - e) << 23);
+          const float down = __uint_as_float((uint32_t)(127 - e) << 23);
           sl *= __uint_as_float((uint32_t)(127 + e) << 23);
-        }
-#pragma unroll 1
-        for (int p = 0; p < R::PANELS; ++p) {
-          uint32_t w[32];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int at = p * 8 + i;
-            const uint4 v = mine && at < NB * 4 ? q[at] : make_uint4(0, 0, 0, 0);
-            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-          }
-          if (a.q_bf16) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              w[i] = pack_h2(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down);
-          }
-          __syncwarp();
-          tc::tmem_st32(tmem + lanes + kColQ + t * 64 + p * 32, w);
+          for (int i = 0; i < DP / 2; ++i)
+            w[i] = pack2<__half>(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down);
         }
+        __syncwarp();
+#pragma unroll
+        for (int p = 0; p < R::PANELS; ++p) tc::tmem_st32(tmem + lanes + kColQ + t * 64 + p * 32, w + 32 * p);
         tc::tmem_st_wait();
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
       }
-      float m = -INFINITY, l = 0.0f;
+      float m = -INFINITY;
+      F2 l2 = f2(0.0f, 0.0f);
       for (int j = 0; j < n; ++j) {
         mbar_wait_or_poison(&s_full[t], j & 1, a.err, DEV_TIMEOUT_FULL, dead);
         __syncwarp();
@@ -892,41 +895,28 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
           for (int i = 0; i < kBlk; ++i)
             if (i >= lim || !(present >> i & 1)) s[i] = 0xff800000u;
         }
-        float mx[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(s[i]);
-#pragma unroll
-        for (int i = 4; i < kBlk; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
-        const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl;
+        const float mn = row_max(s) * sl;
         float f = 1.0f;
         if (mn > m + kLazy) {  // also the row's first keys (m = -inf)
           f = ex2(m - mn);
           m = mn;
-          l *= f;
+          l2 = mul2(l2, f2(f, f));
         }
-        if (j > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
-#pragma unroll 1
-          for (int x = 0; x < DP / 32; ++x) {
-            uint32_t o[32];
-            tc::tmem_ld32(o_addr + 32 * x, o);
-            tc::tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tc::tmem_st32(o_addr + 32 * x, o);
-          }
-        }
+        if (j > 0 && __any_sync(0xffffffffu, f != 1.0f)) rescale_row(o_addr, DP, f);
         const float off = m == -INFINITY ? 0.0f : kBias - m;
-        float sum[2] = {0.0f, 0.0f};
+        const F2 sl2 = f2(sl, sl), off2 = f2(off, off);
+        F2 sum = f2(0.0f, 0.0f);
         uint32_t p[kBlk / 2];
 #pragma unroll
         for (int i = 0; i < kBlk / 2; ++i) {
-          const float p0 = ex2(fmaf(__uint_as_float(s[2 * i]), sl, off));
-          const float p1 = ex2(fmaf(__uint_as_float(s[2 * i + 1]), sl, off));
-          sum[0] += p0;
-          sum[1] += p1;
-          p[i] = pack_h2(p0, p1);
+          const F2 e = fma2(f2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sl2, off2);
+          float e0, e1;
+          unpack(e, e0, e1);
+          e0 = ex2(e0), e1 = ex2(e1);
+          sum = add2(sum, f2(e0, e1));
+          p[i] = pack2<__half>(e0, e1);
         }
-        l += sum[0] + sum[1];
+        l2 = add2(l2, sum);
         __syncwarp();
         tc::tmem_st32(s_addr, p);
         tc::tmem_st_wait();
@@ -934,24 +924,39 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
       }
+      float l, l1;
+      unpack(l2, l, l1);
+      l += l1;
       if (n > 0) mbar_wait_or_poison(&o_full[t], 0, a.err, DEV_TIMEOUT_FULL, dead);
       __syncwarp();
       tc::tc_fence_after();
-      const long long at = (long long)chunk * a.B * a.Hq + qrow;
+      const long long base = (long long)chunk * a.B * a.Hq;
+      if (mine) a.ml[base + qrow] = make_float2(m - kBias, l);
+      const bool none = l == 0.0f;
 #pragma unroll 1
-      for (int x = 0; x < DP / 32; ++x) {
+      for (int x0 = 0; x0 < NB * 32; x0 += 32) {
         uint32_t o[32];
         __syncwarp();
-        tc::tmem_ld32(o_addr + 32 * x, o);
+        tc::tmem_ld32(o_addr + x0, o);
         tc::tmem_ld_wait();
-        if (mine && x < NB) {
-          uint4* dst = reinterpret_cast<uint4*>(a.part + at * (NB * 32) + 32 * x);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            dst[i] = l > 0.0f || l != l ? make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]) : make_uint4(0, 0, 0, 0);
+        for (int half = 0; half < 2; ++half) {
+          __syncwarp();
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int i = 16 * half + 4 * x;
+            *stage_row(stage, lane, x) = none ? make_uint4(0, 0, 0, 0) : make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+          __syncwarp();
+          uint4 v[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) v[x] = *stage_piece(stage, lane, x);
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (other[x] >= 0)
+              *reinterpret_cast<uint4*>(a.part + (base + other[x]) * (NB * 32) + x0 + 16 * half + 4 * (lane & 3)) = v[x];
         }
       }
-      if (mine) a.ml[at] = make_float2(m - kBias, l);
     }
   }
   tc::tc_fence_before();
@@ -974,13 +979,13 @@ struct CombineArgs {
   int Hq, D;
   void* out;
 };
-constexpr int kAtOnce = 8;
+constexpr int kAtOnce = 4;
 constexpr int kCta = 256;
 
-template <typename T, int WR>
-__global__ void __launch_bounds__(kCta) fa_paged_combine_kernel(const CombineArgs a) {
+template <typename T, int WR, int VEC>
+__global__ void __launch_bounds__(kCta, 4) fa_paged_combine_kernel(const CombineArgs a) {
   __shared__ SplitScan<kCta> ss;
-  __shared__ float4 s_o[kCta / 32][kMaxNB * 32 / 4];
+  __shared__ float4 s_o[kCta / 32][VEC * 32];
   __shared__ float2 s_ml[kCta / 32];
   scan_units(a.split, ss);
   pdl_wait();
@@ -989,10 +994,9 @@ __global__ void __launch_bounds__(kCta) fa_paged_combine_kernel(const CombineArg
   const long long brows = (long long)a.split.B * a.Hq;
   const long long row = (long long)blockIdx.x * ROWS + warp / WR;
   const bool real = row < brows;
-  constexpr int kVec = kMaxNB * 32 / 128;
-  float4 o[kVec];
+  float4 o[VEC];
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i = 0; i < VEC; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float M = -INFINITY, L = 0.0f;
   if (real) {
     const int b = (int)(row / a.Hq), h = (int)(row % a.Hq);
@@ -1021,11 +1025,11 @@ __global__ void __launch_bounds__(kCta) fa_paged_combine_kernel(const CombineArg
       L = L * f + t;
       M = Mn;
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) o[i].x *= f, o[i].y *= f, o[i].z *= f, o[i].w *= f;
+      for (int i = 0; i < VEC; ++i) o[i].x *= f, o[i].y *= f, o[i].z *= f, o[i].w *= f;
       const int cnt = min(32, (total - i0 + WR - 1) / WR);
       for (int k0 = 0; k0 < cnt; k0 += kAtOnce) {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
+        for (int i = 0; i < VEC; ++i) {
           if (i * 128 >= a.D) break;
           float4 v[kAtOnce];
 #pragma unroll
@@ -1047,7 +1051,7 @@ __global__ void __launch_bounds__(kCta) fa_paged_combine_kernel(const CombineArg
   if (WR > 1) {
     if (w > 0) {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i)
+      for (int i = 0; i < VEC; ++i)
         if (i * 128 < a.D) s_o[warp][i * 32 + lane] = o[i];
       if (lane == 0) s_ml[warp] = make_float2(M, L);
     }
@@ -1059,14 +1063,14 @@ __global__ void __launch_bounds__(kCta) fa_paged_combine_kernel(const CombineArg
     const float base = top == -INFINITY ? 0.0f : top, f = ex2(M - base);
     L *= f;
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) o[i].x *= f, o[i].y *= f, o[i].z *= f, o[i].w *= f;
+    for (int i = 0; i < VEC; ++i) o[i].x *= f, o[i].y *= f, o[i].z *= f, o[i].w *= f;
 #pragma unroll
     for (int k = 1; k < WR; ++k) {
       const float2 s = s_ml[warp + k];
       const float fk = ex2(s.x - base);
       L = fmaf(fk, s.y, L);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i)
+      for (int i = 0; i < VEC; ++i)
         if (i * 128 < a.D) {
           const float4 v = s_o[warp + k][i * 32 + lane];
           o[i].x = fmaf(fk, v.x, o[i].x), o[i].y = fmaf(fk, v.y, o[i].y);
@@ -1078,7 +1082,7 @@ __global__ void __launch_bounds__(kCta) fa_paged_combine_kernel(const CombineArg
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   T* out = static_cast<T*>(a.out) + row * a.D;
 #pragma unroll
-  for (int i = 0; i < kVec; ++i)
+  for (int i = 0; i < VEC; ++i)
     if (i * 128 + lane * 4 < a.D) {
       T* p = out + i * 128 + lane * 4;
       store_f(p, o[i].x * inv), store_f(p + 1, o[i].y * inv), store_f(p + 2, o[i].z * inv), store_f(p + 3, o[i].w * inv);
@@ -1237,11 +1241,17 @@ kq_status_t launch_stream_nb(const StreamArgs& a, int grid, bool pdl, cudaStream
   return a.G > 8 ? launch_stream<NB, true>(a, grid, pdl, s) : launch_stream<NB, false>(a, grid, pdl, s);
 }
 
-template <typename T>
-kq_status_t launch_combine(const CombineArgs& a, long long rows, cudaStream_t s) {
+// Eight warps per row while that leaves the SMs room, else two.
+template <typename T, int VEC>
+kq_status_t launch_combine(const CombineArgs& a, cudaStream_t s) {
+  const long long rows = (long long)a.split.B * a.Hq;
   if (rows <= sm_count() * 4)
-    return launch_after(fa_paged_combine_kernel<T, 8>, (int)rows, kCta, 0, true, s, a, "fa_paged_combine");
-  return launch_after(fa_paged_combine_kernel<T, 2>, (int)((rows + 3) / 4), kCta, 0, true, s, a, "fa_paged_combine");
+    return launch_after(fa_paged_combine_kernel<T, 8, VEC>, (int)rows, kCta, 0, true, s, a, "fa_paged_combine");
+  return launch_after(fa_paged_combine_kernel<T, 2, VEC>, (int)((rows + 3) / 4), kCta, 0, true, s, a, "fa_paged_combine");
+}
+template <typename T>
+kq_status_t launch_combine_d(const CombineArgs& a, cudaStream_t s) {
+  return a.D <= 128 ? launch_combine<T, 1>(a, s) : launch_combine<T, 2>(a, s);
 }
 
 }  // namespace
@@ -1307,9 +1317,7 @@ kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s) {
   if (st) return st;
   CombineArgs ca{p.split, p.part, p.ml, reinterpret_cast<float*>(ws + w.ppart), reinterpret_cast<float2*>(ws + w.pml),
                  chunks, a.Hq, a.D, a.out};
-  // eight warps per row while that leaves the SMs room, else two
-  const long long rows = (long long)a.B * a.Hq;
-  return dtype == KQ_F16 ? launch_combine<__half>(ca, rows, s) : launch_combine<__nv_bfloat16>(ca, rows, s);
+  return dtype == KQ_F16 ? launch_combine_d<__half>(ca, s) : launch_combine_d<__nv_bfloat16>(ca, s);
 }
 
 }  // namespace kq

@@ -7,23 +7,19 @@
 // with row i of a sequence's len_q new tokens and key j of its len_k tokens
 // (len_k > len_q: the chunk follows an earlier context). A row without keys
 // is zero. The maxima, sums and the output accumulate in fp32.
-#include <cuda_bf16.h>
-
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
 
 #include "kq_internal.h"
+#include "kq_attn.cuh"
 #include "kq_device.cuh"
 #include "kq_tc.cuh"
 
 namespace kq {
 namespace {
 
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void store_f(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void store_f(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+using namespace attn;
 
 // Sequence that owns packed row i: the last b with cu[b] <= i (empty ones
 // before it share that start and come earlier).
@@ -181,54 +177,6 @@ struct TcArgs {
   int* err;
 };
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-// Two fp32 lanes per instruction.
-struct F2 {
-  uint64_t v;
-};
-__device__ __forceinline__ F2 f2(float x, float y) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void unpack(F2 a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
@@ -595,14 +543,7 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
             fence_proxy_async_smem();
           }
         }
-        float mx[8];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) mx[x] = fmaxf(__uint_as_float(s[x]), __uint_as_float(s[x + 8]));
-#pragma unroll
-        for (int x = 16; x < BLK; x += 16)
-#pragma unroll
-          for (int y = 0; y < 8; ++y) mx[y] = max3(mx[y], __uint_as_float(s[x + y]), __uint_as_float(s[x + y + 8]));
-        const float mn = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * a.sl;
+        const float mn = row_max(s) * a.sl;
         float f = 1.0f;
         if (mn > m + kLazy) {  // also the row's first keys (m = -inf)
           f = ex2(m - mn);
@@ -617,15 +558,7 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
         if (i > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
           __syncwarp();
           tc::tc_fence_after();
-#pragma unroll 1
-          for (int x = 0; x < DP / 16; ++x) {  // (small pieces: the scores are still in registers)
-            uint32_t o[16];
-            tc::tmem_ld16(o_addr + 16 * x, o);
-            tc::tmem_ld_wait();
-#pragma unroll
-            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-            tc::tmem_st16(o_addr + 16 * x, o);
-          }
+          rescale_row(o_addr, DP, f);
         }
         const float off = m == -INFINITY ? 0.0f : kBias - m;
         const F2 sl2 = f2(a.sl, a.sl), off2 = f2(off, off);
@@ -662,9 +595,7 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
         tc::tc_fence_after();
       }
       const bool none = m == -INFINITY && l == l;             // no key seen (a NaN score is one)
-      // Rows leave through shared memory, 64 bytes of each at a time: a warp's
-      // store then covers 8 row pieces of 64 bytes (a thread's own row would
-      // be 32 scattered pieces of 16).
+      // rows leave through shared memory, 64 bytes of each at a time
       const int at = mine ? (w.q0 + tok) * a.Hq + j.head * a.G + g : -1;
       const float inv = 1.0f / l;
       const bool partial = a.splits > 1;
@@ -705,18 +636,14 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
         for (int half = 0; half < 2; ++half) {
           if (half == 1 && !partial) break;
           __syncwarp();
-          // piece c of row r lies at c ^ (r / 2 % 4): eight rows hit distinct banks
 #pragma unroll
           for (int x = 0; x < 4; ++x)
-            *reinterpret_cast<uint4*>(stage + lane * 64 + ((x ^ ((lane >> 1) & 3)) << 4)) =
+            *stage_row(stage, lane, x) =
                 make_uint4(o[16 * half + 4 * x], o[16 * half + 4 * x + 1], o[16 * half + 4 * x + 2], o[16 * half + 4 * x + 3]);
           __syncwarp();
           uint4 v[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int r = 8 * x + (lane >> 2);
-            v[x] = *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
-          }
+          for (int x = 0; x < 4; ++x) v[x] = *stage_piece(stage, lane, x);
           const int col = x0 + cols * half;
           const bool inside = (col * item + (lane & 3) * 16) < a.D * item;
 #pragma unroll
