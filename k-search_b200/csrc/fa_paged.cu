@@ -29,7 +29,7 @@ constexpr int kMaxNB = 8;
 // and the table) are cut into units of 16 at multiples of 16 (so that 8 rows
 // of a unit are neighbours in one page); a KV head's units of all sequences
 // in a row are divided evenly among C workers, whatever the lengths are.
-// Worker c takes units U c / C .. U (c + 1) / C; the part of it inside
+// Worker c takes U / C units in order, the first U % C one more; the part inside
 // sequence b is one segment with its own softmax state, stored at index c + b
 // (unique: c and b only grow along the row).
 constexpr int kUnit = 16;
@@ -48,7 +48,16 @@ struct Split {
   __device__ __forceinline__ int active(int U) const { return max(1, min(workers, U / kMinUnits)); }
   static constexpr int kMinUnits = 2;
 };
-__device__ __forceinline__ int unit_begin(int U, int C, int c) { return (int)((long long)U * c / C); }
+struct Shares {
+  int base, rem;
+  __device__ __forceinline__ Shares(int U, int C) : base(U / C), rem(U % C) {}
+  __device__ __forceinline__ int begin(int c) const { return c * base + min(c, rem); }
+  // the worker that has unit u (base > 0 where there is more than one worker)
+  __device__ __forceinline__ int worker(int u) const {
+    const int head = rem * (base + 1);
+    return u < head ? u / (base + 1) : rem + (u - head) / max(base, 1);
+  }
+};
 
 // Prefix sums of the units of B sequences, T contiguous runs of them (one per
 // thread): scan[i] = units before run i, scan[T] = all.
@@ -227,7 +236,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1) fa_paged_stream_kernel(cons
   int u = 0, ue = 0;
   Cursor f{};  // the worker's first tile
   if (wk < C) {
-    u = unit_begin(U, C, wk), ue = unit_begin(U, C, wk + 1);
+    const Shares shares(U, C);
+    u = shares.begin(wk), ue = shares.begin(wk + 1);
     if (u < ue) {
       int lo = 0, hi = kStreamThreads;
       while (hi - lo > 1) {
@@ -561,7 +571,7 @@ constexpr int kTile = 128;
 constexpr int kPrefixThreads = 640;
 constexpr int kMmaWarp = 8, kDeqWarp = 9, kDeqWarps = 8;
 constexpr float kBias = 7.0f, kLazy = 8.0f;
-constexpr int kRaw = 6, kOps = 4;      // raw and operand stages (K and V alternate)
+constexpr int kRaw = 3, kOps = 2;      // blocks of raw rows and of operands in flight (K and V each)
 constexpr int kMasks = 16;             // blocks whose row masks are kept (more than are in flight)
 
 template <int NB, bool LO>
@@ -570,11 +580,11 @@ struct PrefixTraits {
   static constexpr int PANELS = DP / 64;
   static constexpr int PANEL = kBlk * 128;
   static constexpr int PART = PANELS * PANEL;       // the high (or low) parts of a block
-  static constexpr int OP = PART * (LO ? 2 : 1);
-  static constexpr int RAW = kBlk * Row<NB>::PITCH;
-  static constexpr int OFF_RAW = kOps * OP;
-  static constexpr int OFF_STAGE = OFF_RAW + kRaw * RAW;  // 2 KB per softmax warp
-  static constexpr int OFF_BAR = OFF_STAGE + 8 * 2048;
+  static constexpr int OP = PART * (LO ? 2 : 1);    // K or V of a block
+  static constexpr int RAW = 2 * kBlk * Row<NB>::PITCH;  // raw rows of a block, K and V
+  static constexpr int OFF_RAW = kOps * 2 * OP;
+  static constexpr int OFF_STAGE = OFF_RAW + kRaw * RAW;  // 4 KB per softmax warp
+  static constexpr int OFF_BAR = OFF_STAGE + 8 * 4096;
   static constexpr int SMEM = OFF_BAR + 512 + 1024;
   static_assert(SMEM <= 232448, "shared memory budget");
   static_assert(OFF_RAW % 1024 == 0 && OFF_BAR % 16 == 0, "alignment");
@@ -615,16 +625,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
   constexpr int DP = R::DP;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* op_full = reinterpret_cast<uint64_t*>(smem + R::OFF_BAR);
-  uint64_t* op_empty = op_full + kOps;
-  uint64_t* s_full = op_empty + kOps;  // S of a tile is there (and its earlier P V is done)
+  uint64_t* op_full = reinterpret_cast<uint64_t*>(smem + R::OFF_BAR);  // K at 2 (j % kOps), V behind it
+  uint64_t* op_empty = op_full + 2 * kOps;
+  uint64_t* s_full = op_empty + 2 * kOps;  // S of a tile is there (and its earlier P V is done)
   uint64_t* p_full = s_full + 2;       // P of a tile is there, its S is read
   uint64_t* o_full = p_full + 2;       // the tile's last P V is done
   uint64_t* q_full = o_full + 2;       // the tiles' queries are in TMEM
   uint64_t* drained = q_full + 1;      // all of the MMA warp's products and arrivals are done
   uint64_t* row_mask = drained + 1;    // rows present in block j, at j % kMasks
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(row_mask + kMasks);
-  static_assert((2 * kOps + 8 + kMasks) * 8 + 4 <= 512, "barrier area");
+  static_assert((4 * kOps + 8 + kMasks) * 8 + 4 <= 512, "barrier area");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
 
@@ -635,7 +645,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
   const int j0 = (int)((long long)blocks * chunk / a.chunks), n = (int)((long long)blocks * (chunk + 1) / a.chunks) - j0;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kOps; ++i) {
+    for (int i = 0; i < 2 * kOps; ++i) {
       mbar_init(&op_full[i], kDeqWarps);
       mbar_init(&op_empty[i], 1);
     }
@@ -648,127 +658,117 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
     mbar_init(drained, 1);
     fence_mbar_init();
   }
-  if (warp == kMmaWarp) tc::tmem_alloc(tmem_slot, 512);
-  tc::tc_fence_before();
-  __syncthreads();
-  tc::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const long long row_bytes = (long long)a.Hkv * Row<NB>::BYTES;
-  const int head_off = h * Row<NB>::BYTES, row15 = (int)(row_bytes & 15);
+  // The set-up's barrier, which every role meets with its first loads out.
+  auto set_up = [&]() {
+    tc::tc_fence_before();
+    named_bar_sync(0, kPrefixThreads);
+    tc::tc_fence_after();
+  };
   bool dead = false;
 
   if (warp >= 2 * 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp >= kDeqWarp + kDeqWarps) {
-    // idle
+    set_up();
   } else if (warp >= kDeqWarp) {
-    // ---- one block of 32 values per thread: token 8 w + lane % 8, block lane / 8
-    const int dw = warp - kDeqWarp, tok = dw * 8 + (lane & 7), blk = lane >> 3;
+    // ---- one block of 32 values per thread: token 8 w + lane % 8, block lane / 8.
+    // 8 tokens of a block lie in one page (pages hold a multiple of 8): page
+    // `col` of the table, from row `off0` on.
+    const long long row_bytes = (long long)a.Hkv * Row<NB>::BYTES;
+    const int head_off = h * Row<NB>::BYTES, row15 = (int)(row_bytes & 15);
+    const int dw = warp - kDeqWarp;
+    uint8_t* ring = smem + R::OFF_RAW + dw * kRaw * 16 * Row<NB>::PITCH;  // per block: 8 K rows, 8 V rows
+    const Pieces<NB> pieces(lane, row_bytes, head_off);
+    const int last_col = (a.prefix_len - 1) / a.ps;
+    int col = (j0 * kBlk + dw * 8) / a.ps, off0 = (j0 * kBlk + dw * 8) % a.ps;
+    int page = a.table[min(col, last_col)];
+    set_up();
+    // copies of block j, one group; the next page id is loaded, not looked at
+    auto issue = [&](int j) -> uint32_t {
+      const int left = a.prefix_len - ((j0 + j) * kBlk + dw * 8);
+      uint32_t present = 0;
+      if (page >= 0 && page < a.num_pages && j < n && left > 0) {
+        present = left >= 8 ? 0xffu : (1u << left) - 1u;
+        const long long at = ((long long)page * a.ps + off0) * row_bytes;
+        const uint32_t to = smem_u32(ring) + (j % kRaw) * 16 * Row<NB>::PITCH;
+        pieces.copy(to, a.k + at);
+        pieces.copy(to + 8 * Row<NB>::PITCH, a.v + at);
+      }
+      copy_commit();
+      for (off0 += kBlk; off0 >= a.ps; off0 -= a.ps) ++col;
+      page = a.table[min(col, last_col)];
+      return present;
+    };
+    uint32_t rows_at[kRaw];  // rows of the blocks in flight, oldest first
+#pragma unroll
+    for (int i = 0; i < kRaw; ++i) rows_at[i] = 0;
+#pragma unroll
+    for (int i = 0; i < kRaw - 1; ++i) rows_at[i] = issue(i);
+    const int tok = dw * 8 + (lane & 7), blk = lane >> 3;
     const int off = (((lane & 7) * row15 + head_off) & 15) + blk * kQ8;
     const uint32_t sh = (uint32_t)(off & 2) * 8;
     const bool used = blk * 32 < DP, real = blk < NB;
     uint8_t* dst = smem + (blk >> 1) * R::PANEL;
-    uint8_t* ring = smem + R::OFF_RAW + dw * kRaw * 8 * Row<NB>::PITCH;
-    const uint32_t ring32 = smem_u32(ring);
-    const Pieces<NB> pieces(lane, row_bytes, head_off);
-    // 8 tokens of a block lie in one page (pages hold a multiple of 8)
-    auto page_of = [&](int j) {
-      const int t = (j0 + j) * kBlk + dw * 8;
-      return j < n && t < a.prefix_len ? a.table[t / a.ps] : -1;
-    };
-    auto rows_of = [&](int j, int page) {
-      const int left = a.prefix_len - ((j0 + j) * kBlk + dw * 8);
-      return page >= 0 && page < a.num_pages ? (left >= 8 ? 0xffu : (1u << max(left, 0)) - 1u) : 0u;
-    };
-    int page = page_of(0);
-    uint32_t rows_at[kRaw / 2];  // rows of the blocks in flight, oldest first
-    // copies of block j: K into ring stage (2 j) % kRaw, V into the next
-    auto issue = [&](int j) -> uint32_t {
-      const uint32_t present = j < n ? rows_of(j, page) : 0u;
-      if (present) {
-        const int t = (j0 + j) * kBlk + dw * 8;
-        const long long at = ((long long)page * a.ps + t % a.ps) * row_bytes;
-        const uint32_t to = ring32 + (2 * j % kRaw) * 8 * Row<NB>::PITCH;
-        pieces.copy(to, a.k + at);
-        copy_commit();
-        pieces.copy(to + 8 * Row<NB>::PITCH, a.v + at);
-        copy_commit();
-      } else {
-        copy_commit();
-        copy_commit();
-      }
-      page = page_of(j + 1);
-      return present;
-    };
-#pragma unroll
-    for (int i = 0; i < kRaw / 2; ++i) rows_at[i] = 0;
-#pragma unroll
-    for (int i = 0; i < kRaw / 2 - 1; ++i) rows_at[i] = issue(i);
-    // the words of item i (K or V of block i / 2), once its copies are there:
-    // 9 that cover the thread's block of 34 bytes; 0 for an absent row, since
-    // whatever its slot holds must not meet P = 0
-    auto load = [&](int i, uint32_t (&w)[9]) {
-      const int rs = i % kRaw, j = i >> 1;
-      if ((i & 1) == 0) {
-        if (i > 0) {
-#pragma unroll
-          for (int x = 0; x + 1 < kRaw / 2; ++x) rows_at[x] = rows_at[x + 1];
-        }
-        rows_at[kRaw / 2 - 1] = issue(j + kRaw / 2 - 1);
-        if (lane == 0) reinterpret_cast<uint8_t*>(&row_mask[j % kMasks])[dw] = (uint8_t)rows_at[0];
-        copy_wait<kRaw - 1>();  // later groups: V of this block, and kRaw / 2 - 1 blocks
-      } else {
-        copy_wait<kRaw - 2>();
-      }
-      __syncwarp();
-      const bool present = real && (rows_at[0] >> (lane & 7) & 1);
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(ring + (rs * 8 + (lane & 7)) * Row<NB>::PITCH + (off & ~3));
+    // The 9 words that cover this thread's block of 34 bytes; 0 for an absent
+    // row, since whatever its slot holds must not meet P = 0.
+    auto words = [&](const uint8_t* row, bool present, uint32_t (&w)[9]) {
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(row + (off & ~3));
 #pragma unroll
       for (int x = 0; x < 8; ++x) w[x] = present ? src[x] : 0u;
       w[8] = !present ? 0u : sh ? src[8] : *reinterpret_cast<const uint16_t*>(src + 8);
-      __syncwarp();
     };
-    uint32_t next[9];
-    if (n > 0) load(0, next);
-    for (int i = 0; i < 2 * n; ++i) {
-      const int os = i % kOps;
-      uint32_t w[9];
+    auto convert = [&](const uint32_t (&w)[9], uint8_t* op) {
+      const uint32_t d = (w[0] >> sh) & 0xffffu, d2 = d | d << 16;
 #pragma unroll
-      for (int x = 0; x < 9; ++x) w[x] = next[x];
-      if (i + 1 < 2 * n) load(i + 1, next);
-      if (i >= kOps) mbar_wait_or_poison(&op_empty[os], ((i / kOps) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
-      if (used) {
-        const uint32_t d = (w[0] >> sh) & 0xffffu, d2 = d | d << 16;
+      for (int x = 0; x < 4; ++x) {
+        uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint32_t hi[4], lo[4];
+        for (int y = 0; y < 2; ++y) {
+          uint32_t c[2];
+          codes_h2(__funnelshift_rc(w[2 * x + y], w[2 * x + y + 1], sh + 16), c[0], c[1]);
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            uint32_t c[2];
-            codes_h2(__funnelshift_rc(w[2 * x + y], w[2 * x + y + 1], sh + 16), c[0], c[1]);
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              hi[2 * y + z] = hmul2(c[z], d2);
-              if (LO) lo[2 * y + z] = hfma2(c[z], d2, hi[2 * y + z] ^ 0x80008000u);
-            }
+          for (int z = 0; z < 2; ++z) {
+            hi[2 * y + z] = hmul2(c[z], d2);
+            if (LO) lo[2 * y + z] = hfma2(c[z], d2, hi[2 * y + z] ^ 0x80008000u);
           }
-          uint8_t* o = dst + os * R::OP + tc::sw128_off(tok, (blk & 1) * 4 + x);
-          *reinterpret_cast<uint4*>(o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if (LO) *reinterpret_cast<uint4*>(o + R::PART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
+        uint8_t* o = op + tc::sw128_off(tok, (blk & 1) * 4 + x);
+        *reinterpret_cast<uint4*>(o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (LO) *reinterpret_cast<uint4*>(o + R::PART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
-      fence_proxy_async_smem();
+    };
+    for (int j = 0; j < n; ++j) {
+      const int os = j % kOps;
+      rows_at[kRaw - 1] = issue(j + kRaw - 1);
+      if (lane == 0) reinterpret_cast<uint8_t*>(&row_mask[j % kMasks])[dw] = (uint8_t)rows_at[0];
+      copy_wait<kRaw - 1>();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&op_full[os]);
+      const bool present = real && (rows_at[0] >> (lane & 7) & 1);
+      const uint8_t* row = ring + ((j % kRaw) * 16 + (lane & 7)) * Row<NB>::PITCH;
+      uint32_t wk[9], wv[9];
+      words(row, present, wk);
+      words(row + 8 * Row<NB>::PITCH, present, wv);
+      // K is free again once its scores are there, V a block later
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        if (j >= kOps) mbar_wait_or_poison(&op_empty[2 * os + kv], ((j / kOps) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
+        if (used) convert(kv ? wv : wk, dst + (os * 2 + kv) * R::OP);
+        fence_proxy_async_smem();
+        __syncwarp();  // also: the ring's rows are read
+        if (lane == 0) mbar_arrive(&op_full[2 * os + kv]);
+      }
+#pragma unroll
+      for (int x = 0; x + 1 < kRaw; ++x) rows_at[x] = rows_at[x + 1];
     }
   } else if (warp == kMmaWarp) {
     constexpr uint32_t idesc_s = idesc_h(kBlk, false), idesc_o = idesc_h(DP, true);
-    const uint32_t base = smem_u32(smem), go = tc::elect_one();
+    tc::tmem_alloc(tmem_slot, 512);
+    set_up();
+    const uint32_t tmem = *tmem_slot, base = smem_u32(smem), go = tc::elect_one();
     const int tiles = two ? 2 : 1;
     auto score = [&](int t, int j) {
-      const int st = 2 * j % kOps;
-      mbar_wait_or_poison(&op_full[st], (2 * j / kOps) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+      mbar_wait_or_poison(&op_full[2 * (j % kOps)], (j / kOps) & 1, a.err, DEV_TIMEOUT_FULL, dead);
       tc::tc_fence_after();
-      const uint64_t kd = tc::sw128_desc(base + st * R::OP);
+      const uint64_t kd = tc::sw128_desc(base + j % kOps * 2 * R::OP);
 #pragma unroll
       for (int part = 0; part < (LO ? 2 : 1); ++part)
 #pragma unroll
@@ -778,25 +778,24 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
                         (part > 0 || k > 0) ? 1u : 0u, go);
       tc::mma_commit_go(&s_full[t], go);
     };
-    // every arrival is waited for before the CTA ends: a stage is only released
-    // to an item that waits for it, and the warp drains at the end
-    auto release = [&](int item) {
-      if (item + kOps < 2 * n) tc::mma_commit_go(&op_empty[item % kOps], go);
+    // every arrival is waited for before the CTA ends: an operand is only
+    // released to one that waits for it, and the warp drains at the end
+    auto release = [&](int j, int kv) {
+      if (j + kOps < n) tc::mma_commit_go(&op_empty[2 * (j % kOps) + kv], go);
     };
     mbar_wait_or_poison(q_full, 0, a.err, DEV_TIMEOUT_FULL, dead);
     tc::tc_fence_after();
     if (n > 0) {
       for (int t = 0; t < tiles; ++t) score(t, 0);
-      release(0);
+      release(0, 0);
     }
     for (int j = 0; j < n; ++j) {
-      const int sv = (2 * j + 1) % kOps;
+      const uint64_t vd = tc::sw128_desc_mn(base + (j % kOps * 2 + 1) * R::OP, R::PANEL);  // dims across, tokens down
 #pragma unroll 1
       for (int t = 0; t < tiles; ++t) {
-        mbar_wait_or_poison(&op_full[sv], ((2 * j + 1) / kOps) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        mbar_wait_or_poison(&op_full[2 * (j % kOps) + 1], (j / kOps) & 1, a.err, DEV_TIMEOUT_FULL, dead);
         mbar_wait_or_poison(&p_full[t], j & 1, a.err, DEV_TIMEOUT_FULL, dead);
         tc::tc_fence_after();
-        const uint64_t vd = tc::sw128_desc_mn(base + sv * R::OP, R::PANEL);  // dims across, tokens down
 #pragma unroll
         for (int part = 0; part < (LO ? 2 : 1); ++part)
 #pragma unroll
@@ -805,10 +804,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
                           vd + (uint64_t)(part * (R::PART >> 4) + k * (2048 >> 4)), idesc_o,
                           (j > 0 || part > 0 || k > 0) ? 1u : 0u, go);
         if (j + 1 == n) tc::mma_commit_go(&o_full[t], go);
+        if (t + 1 == tiles) release(j, 1);
         if (j + 1 < n) score(t, j + 1);
       }
-      release(2 * j + 1);
-      if (j + 1 < n) release(2 * j + 2);
+      if (j + 1 < n) release(j + 1, 0);
     }
     tc::mma_commit_go(drained, go);
     mbar_wait_idle_or_poison(drained, 0, a.err, DEV_TIMEOUT_FULL, dead);
@@ -816,41 +815,43 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
   } else {
     // ---- softmax, a thread per row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
-    const int t = warp >> 2, r = row0 + threadIdx.x, b = r / a.G, gq = r % a.G;
+    const int t = warp >> 2;
+    const int my_row = row0 + threadIdx.x;
+    const int qrow = my_row < rows ? my_row / a.G * a.Hq + h * a.G + my_row % a.G : -1;
+    const int my_len = a.seq_lens[qrow >= 0 ? my_row / a.G : 0];
+    // the queries: pieces of 64 bytes of the rows lane / 4 + 8 x, 32 dims per j,
+    // all in flight (a row without a query reads the first one)
+    uint4 qv[NB][4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int r = max(0, __shfl_sync(0xffffffffu, qrow, 8 * x + (lane >> 2)));
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        qv[j][x] = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + (long long)r * (NB * 32) + 32 * j)[lane & 3];
+    }
+    set_up();
+    const uint32_t tmem = *tmem_slot;
     if (t == 0 || two) {
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t s_addr = tmem + lanes + kColS + t * kBlk, o_addr = tmem + lanes + kColO + t * DP;
-      const bool mine = r < rows;
-      const int keys = mine ? max(0, min(min(a.seq_lens[b], a.limit), a.prefix_len)) : 0;
-      const int qrow = mine ? b * a.Hq + h * a.G + gq : -1;
-      uint8_t* stage = smem + R::OFF_STAGE + warp * 2048;
-      int other[4];  // rows whose pieces this lane moves
-#pragma unroll
-      for (int x = 0; x < 4; ++x) other[x] = __shfl_sync(0xffffffffu, qrow, 8 * x + (lane >> 2));
+      uint8_t* stage = smem + R::OFF_STAGE + warp * 4096;
+      const int keys = qrow >= 0 ? max(0, min(min(my_len, a.limit), a.prefix_len)) : 0;
       float sl = a.sl;
       {
-        // the row's queries to TMEM (two fp16 per column), dims past D zero:
-        // all loads in flight at once, through the stage to the row's thread
-        uint4 v[NB][4];
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            v[j][x] = other[x] >= 0 ? reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
-                                                                     (long long)other[x] * (NB * 32) + 32 * j)[lane & 3]
-                                    : make_uint4(0, 0, 0, 0);
+        // the row's queries to TMEM (two fp16 per column), dims past D and rows
+        // without a query zero, through the stage to the row's thread
         uint32_t w[DP / 2];
 #pragma unroll
         for (int j = 0; j < DP / 32; ++j) {
           if (j < NB) {
             __syncwarp();
 #pragma unroll
-            for (int x = 0; x < 4; ++x) *stage_piece(stage, lane, x) = v[j < NB ? j : 0][x];
+            for (int x = 0; x < 4; ++x) *stage_piece(stage, lane, x) = qv[j < NB ? j : 0][x];
             __syncwarp();
           }
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const uint4 y = j < NB ? *stage_row(stage, lane, x) : make_uint4(0, 0, 0, 0);
+            const uint4 y = j < NB && qrow >= 0 ? *stage_row(stage, lane, x) : make_uint4(0, 0, 0, 0);
             w[16 * j + 4 * x] = y.x, w[16 * j + 4 * x + 1] = y.y, w[16 * j + 4 * x + 2] = y.z, w[16 * j + 4 * x + 3] = y.w;
           }
         }
@@ -931,44 +932,44 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
       __syncwarp();
       tc::tc_fence_after();
       const long long base = (long long)chunk * a.B * a.Hq;
-      if (mine) a.ml[base + qrow] = make_float2(m - kBias, l);
+      if (qrow >= 0) a.ml[base + qrow] = make_float2(m - kBias, l);
       const bool none = l == 0.0f;
-#pragma unroll 1
+      float* out[8];  // of the pieces this lane stores, rows lane / 8 + 4 x
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const int r = __shfl_sync(0xffffffffu, qrow, 4 * x + (lane >> 3));
+        out[x] = r >= 0 ? a.part + (base + r) * (NB * 32) + 4 * (lane & 7) : nullptr;
+      }
+#pragma unroll
       for (int x0 = 0; x0 < NB * 32; x0 += 32) {
         uint32_t o[32];
-        __syncwarp();
         tc::tmem_ld32(o_addr + x0, o);
         tc::tmem_ld_wait();
+        __syncwarp();
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          __syncwarp();
+        for (int x = 0; x < 8; ++x)
+          *stage128_row(stage, lane, x) = none ? make_uint4(0, 0, 0, 0) : make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        __syncwarp();
+        uint4 v[8];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int i = 16 * half + 4 * x;
-            *stage_row(stage, lane, x) = none ? make_uint4(0, 0, 0, 0) : make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-          }
-          __syncwarp();
-          uint4 v[4];
+        for (int x = 0; x < 8; ++x) v[x] = *stage128_piece(stage, lane, x);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) v[x] = *stage_piece(stage, lane, x);
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (other[x] >= 0)
-              *reinterpret_cast<uint4*>(a.part + (base + other[x]) * (NB * 32) + x0 + 16 * half + 4 * (lane & 3)) = v[x];
-        }
+        for (int x = 0; x < 8; ++x)
+          if (out[x]) *reinterpret_cast<uint4*>(out[x] + x0) = v[x];
       }
     }
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
+  if (warp == kMmaWarp) tc::tmem_dealloc(*tmem_slot, 512);
 }
 
 // ---- combine -------------------------------------------------------------------------
 // out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's states (the
 // prefix chunks, then its segments), M the largest m_i. WR warps share a row:
 // warp w takes states w, w + WR, ..., kAtOnce loads in flight, and the first
-// one adds the others' sums from shared memory in their order.
+// one adds the others' sums from shared memory in their order. The grid is at
+// most what is resident at once, so that the scan of the lengths is paid once.
 struct CombineArgs {
   Split split;
   const float* part;
@@ -979,114 +980,112 @@ struct CombineArgs {
   int Hq, D;
   void* out;
 };
-constexpr int kAtOnce = 4;
+constexpr int kAtOnce = 8;  // (float4 per lane)
 constexpr int kCta = 256;
+constexpr int kCombineCtas = 4;  // per SM
 
 template <typename T, int WR, int VEC>
-__global__ void __launch_bounds__(kCta, 4) fa_paged_combine_kernel(const CombineArgs a) {
+__global__ void __launch_bounds__(kCta, kCombineCtas) fa_paged_combine_kernel(const CombineArgs a) {
   __shared__ SplitScan<kCta> ss;
-  __shared__ float4 s_o[kCta / 32][VEC * 32];
+  __shared__ float4 s_o[WR > 1 ? kCta / 32 : 1][VEC * 32];
   __shared__ float2 s_ml[kCta / 32];
   scan_units(a.split, ss);
   pdl_wait();
-  constexpr int ROWS = kCta / 32 / WR;
+  constexpr int ROWS = kCta / 32 / WR, AT = kAtOnce / VEC;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp % WR;
-  const long long brows = (long long)a.split.B * a.Hq;
-  const long long row = (long long)blockIdx.x * ROWS + warp / WR;
-  const bool real = row < brows;
-  float4 o[VEC];
+  const int brows = a.split.B * a.Hq;
+  const int U = ss.scan[kCta];
+  const Shares shares(U, a.split.active(U));
+  for (int row = blockIdx.x * ROWS + warp / WR; row < brows; row += gridDim.x * ROWS) {
+    float4 o[VEC];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float M = -INFINITY, L = 0.0f;
-  if (real) {
-    const int b = (int)(row / a.Hq), h = (int)(row % a.Hq);
-    const int U = ss.scan[kCta], C = a.split.active(U);
+    for (int i = 0; i < VEC; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float M = -INFINITY, L = 0.0f;
+    const int b = row / a.Hq, h = row - b * a.Hq;
     const int u0 = units_before(a.split, ss, b), u1 = u0 + a.split.units(b);
-    // workers whose range meets [u0, u1): the last c with begin(c) <= u, for both ends
-    auto worker_of = [&](int u) {
-      int c = (int)((long long)u * C / max(U, 1));
-      while (c + 1 < C && unit_begin(U, C, c + 1) <= u) ++c;
-      while (c > 0 && unit_begin(U, C, c) > u) --c;
-      return c;
-    };
-    const int c0 = u1 > u0 ? worker_of(u0) : 0, n = u1 > u0 ? worker_of(u1 - 1) - c0 + 1 : 0;
+    const int c0 = u1 > u0 ? shares.worker(u0) : 0, n = u1 > u0 ? shares.worker(u1 - 1) - c0 + 1 : 0;
     const int total = a.chunks + n;
-    auto index = [&](int i) { return i < a.chunks ? i * brows + row : ((long long)c0 + b + i - a.chunks) * a.Hq + h; };
+    auto index = [&](int i) {
+      return i < a.chunks ? (long long)i * brows + row : ((long long)c0 + b + i - a.chunks) * a.Hq + h;
+    };
     for (int i0 = w; i0 < total; i0 += 32 * WR) {
       float2 s = make_float2(-INFINITY, 0.0f);
       const int mine = i0 + lane * WR;
       if (mine < total) s = (mine < a.chunks ? a.pml : a.ml)[index(mine)];
-      const float Mn = fmaxf(M, warp_max(s.x));
-      const float base = Mn == -INFINITY ? 0.0f : Mn;
-      const float f = ex2(M - base), wgt = ex2(s.x - base);
-      float t = wgt * s.y;
-#pragma unroll
-      for (int x = 16; x >= 1; x >>= 1) t += __shfl_xor_sync(0xffffffffu, t, x);
-      L = L * f + t;
-      M = Mn;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) o[i].x *= f, o[i].y *= f, o[i].z *= f, o[i].w *= f;
       const int cnt = min(32, (total - i0 + WR - 1) / WR);
-      for (int k0 = 0; k0 < cnt; k0 += kAtOnce) {
+      float f = 1.0f, wgt = 0.0f;
+#pragma unroll 1
+      for (int k0 = 0; k0 < cnt; k0 += AT) {
+        float4 v[VEC][AT];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          if (i * 128 >= a.D) break;
-          float4 v[kAtOnce];
+        for (int k = 0; k < AT; ++k) {
+          const int x = i0 + min(k0 + k, cnt - 1) * WR;  // the last one again past the end, with weight 0
+          const float4* p = reinterpret_cast<const float4*>((x < a.chunks ? a.ppart : a.part) + index(x) * a.D);
 #pragma unroll
-          for (int k = 0; k < kAtOnce; ++k) {
-            const int x = i0 + min(k0 + k, cnt - 1) * WR;  // the last one again past the end, with weight 0
-            const float4* p = reinterpret_cast<const float4*>((x < a.chunks ? a.ppart : a.part) + index(x) * a.D);
-            v[k] = i * 128 + lane * 4 < a.D ? p[i * 32 + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          }
+          for (int i = 0; i < VEC; ++i) v[i][k] = p[min(i * 32 + lane, a.D / 4 - 1)];
+        }
+        if (k0 == 0) {  // under the loads
+          const float Mn = fmaxf(M, warp_max(s.x));
+          const float base = Mn == -INFINITY ? 0.0f : Mn;
+          f = ex2(M - base), wgt = ex2(s.x - base);
+          float t = wgt * s.y;
 #pragma unroll
-          for (int k = 0; k < kAtOnce; ++k) {
-            const float wk = k0 + k < cnt ? __shfl_sync(0xffffffffu, wgt, min(k0 + k, 31)) : 0.0f;
-            o[i].x = fmaf(wk, v[k].x, o[i].x), o[i].y = fmaf(wk, v[k].y, o[i].y);
-            o[i].z = fmaf(wk, v[k].z, o[i].z), o[i].w = fmaf(wk, v[k].w, o[i].w);
+          for (int x = 16; x >= 1; x >>= 1) t += __shfl_xor_sync(0xffffffffu, t, x);
+          L = L * f + t;
+          M = Mn;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) o[i].x *= f, o[i].y *= f, o[i].z *= f, o[i].w *= f;
+        }
+#pragma unroll
+        for (int k = 0; k < AT; ++k) {
+          const float wk = __shfl_sync(0xffffffffu, wgt, (k0 + k) & 31);
+          if (k0 + k < cnt) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              o[i].x = fmaf(wk, v[i][k].x, o[i].x), o[i].y = fmaf(wk, v[i][k].y, o[i].y);
+              o[i].z = fmaf(wk, v[i][k].z, o[i].z), o[i].w = fmaf(wk, v[i][k].w, o[i].w);
+            }
           }
         }
       }
     }
-  }
-  if (WR > 1) {
-    if (w > 0) {
+    if (WR > 1) {
+      __syncthreads();  // the last row's sums are read
+      if (w > 0) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (i * 128 < a.D) s_o[warp][i * 32 + lane] = o[i];
-      if (lane == 0) s_ml[warp] = make_float2(M, L);
-    }
-    __syncthreads();
-    if (w > 0) return;
-    float top = M;
+        for (int i = 0; i < VEC; ++i) s_o[WR > 1 ? warp : 0][i * 32 + lane] = o[i];
+        if (lane == 0) s_ml[warp] = make_float2(M, L);
+      }
+      __syncthreads();
+      if (w > 0) continue;
+      float top = M;
 #pragma unroll
-    for (int k = 1; k < WR; ++k) top = fmaxf(top, s_ml[warp + k].x);
-    const float base = top == -INFINITY ? 0.0f : top, f = ex2(M - base);
-    L *= f;
+      for (int k = 1; k < WR; ++k) top = fmaxf(top, s_ml[warp + k].x);
+      const float base = top == -INFINITY ? 0.0f : top, f = ex2(M - base);
+      L *= f;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) o[i].x *= f, o[i].y *= f, o[i].z *= f, o[i].w *= f;
+      for (int i = 0; i < VEC; ++i) o[i].x *= f, o[i].y *= f, o[i].z *= f, o[i].w *= f;
 #pragma unroll
-    for (int k = 1; k < WR; ++k) {
-      const float2 s = s_ml[warp + k];
-      const float fk = ex2(s.x - base);
-      L = fmaf(fk, s.y, L);
+      for (int k = 1; k < WR; ++k) {
+        const float2 s = s_ml[warp + k];
+        const float fk = ex2(s.x - base);
+        L = fmaf(fk, s.y, L);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (i * 128 < a.D) {
-          const float4 v = s_o[warp + k][i * 32 + lane];
+        for (int i = 0; i < VEC; ++i) {
+          const float4 v = s_o[WR > 1 ? warp + k : 0][i * 32 + lane];
           o[i].x = fmaf(fk, v.x, o[i].x), o[i].y = fmaf(fk, v.y, o[i].y);
           o[i].z = fmaf(fk, v.z, o[i].z), o[i].w = fmaf(fk, v.w, o[i].w);
         }
+      }
     }
-  }
-  if (!real) return;
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  T* out = static_cast<T*>(a.out) + row * a.D;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    T* out = static_cast<T*>(a.out) + (long long)row * a.D;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    if (i * 128 + lane * 4 < a.D) {
-      T* p = out + i * 128 + lane * 4;
-      store_f(p, o[i].x * inv), store_f(p + 1, o[i].y * inv), store_f(p + 2, o[i].z * inv), store_f(p + 3, o[i].w * inv);
-    }
+    for (int i = 0; i < VEC; ++i)
+      if (i * 128 + lane * 4 < a.D)
+        *reinterpret_cast<uint2*>(out + i * 128 + lane * 4) =
+            make_uint2(pack2<T>(o[i].x * inv, o[i].y * inv), pack2<T>(o[i].z * inv, o[i].w * inv));
+  }
 }
 
 // ---- pages of other sizes than a multiple of 8 tokens, or a prefix that ends within 8
@@ -1241,13 +1240,14 @@ kq_status_t launch_stream_nb(const StreamArgs& a, int grid, bool pdl, cudaStream
   return a.G > 8 ? launch_stream<NB, true>(a, grid, pdl, s) : launch_stream<NB, false>(a, grid, pdl, s);
 }
 
-// Eight warps per row while that leaves the SMs room, else two.
+// Eight warps per row while that leaves the SMs room, else one.
 template <typename T, int VEC>
 kq_status_t launch_combine(const CombineArgs& a, cudaStream_t s) {
-  const long long rows = (long long)a.split.B * a.Hq;
-  if (rows <= sm_count() * 4)
+  const long long rows = (long long)a.split.B * a.Hq, most = (long long)sm_count() * kCombineCtas;
+  if (rows <= most)
     return launch_after(fa_paged_combine_kernel<T, 8, VEC>, (int)rows, kCta, 0, true, s, a, "fa_paged_combine");
-  return launch_after(fa_paged_combine_kernel<T, 2, VEC>, (int)((rows + 3) / 4), kCta, 0, true, s, a, "fa_paged_combine");
+  return launch_after(fa_paged_combine_kernel<T, 1, VEC>, (int)std::min(most, (rows + 7) / 8), kCta, 0, true, s, a,
+                      "fa_paged_combine");
 }
 template <typename T>
 kq_status_t launch_combine_d(const CombineArgs& a, cudaStream_t s) {

@@ -105,6 +105,15 @@ __device__ __forceinline__ uint4* stage_piece(uint8_t* stage, int lane, int x) {
   const int r = 8 * x + (lane >> 2);
   return reinterpret_cast<uint4*>(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
 }
+// The same with rows of 128 bytes (4 KB): 8 pieces, a lane moves piece l % 8 of
+// rows l / 8 + 4 x.
+__device__ __forceinline__ uint4* stage128_row(uint8_t* stage, int lane, int x) {
+  return reinterpret_cast<uint4*>(stage + lane * 128 + ((x ^ (lane & 7)) << 4));
+}
+__device__ __forceinline__ uint4* stage128_piece(uint8_t* stage, int lane, int x) {
+  const int r = 4 * x + (lane >> 3);
+  return reinterpret_cast<uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+}
 #endif
 
 }  // namespace attn
