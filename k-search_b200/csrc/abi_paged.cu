@@ -86,8 +86,8 @@ kq_status_t kq_page_read_q8_0(int dtype, const void* k_cache, const void* v_cach
   if (B == 0) return fail(KQ_ERR_INVALID, "page_read: rows without a sequence");
   if (!k || !v || !cu_seqlens || (max_blocks > 0 && !block_tables) || (num_pages > 0 && (!k_cache || !v_cache)))
     return fail(KQ_ERR_INVALID, "page_read: null pointer");
-  if (!aligned(k_cache, 2) || !aligned(v_cache, 2)) return fail(KQ_ERR_INVALID, "page_read: caches must be 2-byte aligned");
-  if (!aligned(k, 16) || !aligned(v, 16)) return fail(KQ_ERR_INVALID, "page_read: k and v must be 16-byte aligned");
+  if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(k, 16) || !aligned(v, 16))
+    return fail(KQ_ERR_INVALID, "page_read: caches, k and v must be 16-byte aligned");
   return launch_page_read_q8_0(dtype, k_cache, v_cache, num_pages, page_size, Hkv, D, block_tables, max_blocks,
                                cu_seqlens, B, total_rows, k, v, static_cast<cudaStream_t>(stream));
 }

@@ -111,7 +111,7 @@ __device__ __forceinline__ int units_before(const Split& sp, const SplitScan<T>&
 // one 32-bit load (a word of 4 codes) per lane.
 constexpr int kStreamWarps = 12;
 constexpr int kStreamThreads = kStreamWarps * 32;
-constexpr int kStages = 4;
+constexpr int kStages = 3;
 constexpr float kPBits = 6.0f, kPScale = 64.0f;
 
 template <int NB>

@@ -119,8 +119,8 @@ __global__ void __launch_bounds__(kPlan) page_plan_kernel(const PlanArgs a) {
       c = max(0, a.cached[b]);
       n = max(0, a.fresh[b]);
     }
-    const int have = (int)min((long long)a.W, ((long long)c + a.ps - 1) / a.ps);
-    const int need = (int)min((long long)a.W, ((long long)c + n + a.ps - 1) / a.ps);
+    const int have = min((unsigned)a.W, ((unsigned)c + a.ps - 1) / (unsigned)a.ps);
+    const int need = min((unsigned)a.W, ((unsigned)c + n + a.ps - 1) / (unsigned)a.ps);
     const int take = need - have;
     int sums[3] = {n, take, c + n};
     scan3(sums, s_warp, lane, warp);
@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(kPlan) page_plan_kernel(const PlanArgs a) {
     s_take[tid] = take;
     s_new_end[tid] = sums[0];
     s_take_end[tid] = sums[1];
+    long long placed = 0;
     if (lead && b < a.B) {
       a.seq_lens[b] = c + n;
       a.cu_new[b + 1] = base_new + sums[0];
@@ -142,7 +143,13 @@ __global__ void __launch_bounds__(kPlan) page_plan_kernel(const PlanArgs a) {
       if (c % a.ps != 0 && c / a.ps < a.W && a.table[(long long)b * a.W + c / a.ps] < 0)
         lo = min(hi, (long long)have * a.ps);
       hi = min(hi, (long long)c + a.T - (base_new + sums[0] - n));
-      if (hi > lo) atomicAdd(&s_placed, (unsigned long long)(hi - lo));  // integers: any order gives the same sum
+      placed = max(0ll, hi - lo);
+    }
+    if (lead) {
+      // one addition per warp (integers: any order gives the same sum)
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) placed += __shfl_xor_sync(0xffffffffu, placed, o);
+      if (lane == 0 && placed > 0) atomicAdd(&s_placed, (unsigned long long)placed);
     }
     __syncthreads();
     const int batch_new = s_new_end[kPlan - 1], batch_take = s_take_end[kPlan - 1];
@@ -197,55 +204,93 @@ struct WriteArgs {
   long long row_stride[2], head_stride[2];  // elements
   uint8_t* cache[2];
   const long long* slots;
-  long long blocks;        // T * Hkv * NB
-  long long num_slots;
-  int H, NB;
+  long long T, num_slots;
+  int H, NB, segs;         // segments of kSegBlocks blocks per row
 };
 
+// round_half_even(x / d) as IEEE division gives it, without the division:
+// x * (1 / d) is within 2^-21 of x / d relatively, under 1e-4 for |x / d| <=
+// 128, so the two round to different integers only that close to a half; only
+// there (one value in 5000) the division runs.
+__device__ __forceinline__ int code_of(float x, float d, float inv) {
+  const float q = x * inv;
+  const float r = rintf(q);
+  if (!(fabsf(q - r) < 0.4999f)) return max(-128, min(127, __float2int_rn(__fdiv_rn(x, d))));
+  return (int)r;
+}
+
 // The q8_0 quantiser of quantize_rows (amax / 127, IEEE division, round half
-// to even) on 16-bit rows: 8 lanes per block, 4 values each, so a warp reads
-// 256 contiguous bytes per step. blockIdx.y picks K or V.
+// to even) on 16-bit rows: a warp takes a segment of up to 32 blocks of one row
+// of K or V, 8 lanes per block and 4 values each, all loads in flight at once.
+// The bytes go through shared memory, laid out as far from a 16-byte boundary
+// as their place in the cache is, so that they leave in whole 16-byte pieces:
+// blocks of 34 bytes stored code by code leave half-written sectors behind,
+// which made 4096 rows of 8 x 128 take 24 us.
+constexpr int kSegBlocks = 32;
+constexpr int kSegRoom = (kSegBlocks * kQ8 + 16 + 15) / 16 * 16;
+
 template <typename T>
 __global__ void __launch_bounds__(256) page_write_kernel(const WriteArgs a) {
+  __shared__ __align__(16) uint8_t s_seg[8][kSegRoom];
   const unsigned full = 0xffffffffu;
-  const int lane = threadIdx.x & 31, sub = lane & 7;
-  const int which = blockIdx.y;
-  const long long per_row = (long long)a.H * a.NB;
-  const long long nwarps = (long long)gridDim.x * (blockDim.x >> 5);
-  const T* x = static_cast<const T*>(a.x[which]);
-  for (long long b0 = ((long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * 4; b0 < a.blocks;
-       b0 += nwarps * 4) {
-    const long long blk = min(b0 + (lane >> 3), a.blocks - 1);  // a repeated last block keeps all lanes in the shuffles
-    const long long t = blk / per_row;
-    const int rem = (int)(blk % per_row), h = rem / a.NB, j = rem % a.NB;
-    const T* src = x + t * a.row_stride[which] + (long long)h * a.head_stride[which] + j * 32 + sub * 4;
-    float v[4];
-    const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
-    uint2 raw;
-    if ((reinterpret_cast<uintptr_t>(src) & 7) == 0) {
-      raw = *reinterpret_cast<const uint2*>(src);
-    } else {
-      raw.x = s16[0] | ((uint32_t)s16[1] << 16);
-      raw.y = s16[2] | ((uint32_t)s16[3] << 16);
-    }
-    const float2 f0 = to_float2<T>(raw.x), f1 = to_float2<T>(raw.y);
-    v[0] = f0.x, v[1] = f0.y, v[2] = f1.x, v[3] = f1.y;
-    float amax = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-#pragma unroll
-    for (int o = 1; o <= 4; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(full, amax, o));
-    const float d = amax > 0.0f ? __fdiv_rn(amax, 127.0f) : 1.0f;
-    uint32_t code = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int q = max(-128, min(127, __float2int_rn(__fdiv_rn(v[i], d))));
-      code |= (uint32_t)(q & 0xff) << (8 * i);
-    }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 7;
+  const int per_row = a.H * a.NB;
+  const long long units = a.T * 2 * a.segs;
+  for (long long u = (long long)blockIdx.x * 8 + warp; u < units; u += (long long)gridDim.x * 8) {
+    const long long t = u / (2 * a.segs);
+    const int which = (int)(u / a.segs & 1), b0 = (int)(u % a.segs) * kSegBlocks, blocks = min(kSegBlocks, per_row - b0);
     const long long slot = a.slots[t];
-    if (slot < 0 || slot >= a.num_slots || b0 + (lane >> 3) >= a.blocks) continue;
-    uint16_t* dst = reinterpret_cast<uint16_t*>(a.cache[which] + (slot * per_row + rem) * kQ8);
-    dst[1 + 2 * sub] = (uint16_t)code;
-    dst[2 + 2 * sub] = (uint16_t)(code >> 16);
-    if (sub == 0) dst[0] = (uint16_t)float_to_half_bits(d);
+    const T* x = static_cast<const T*>(which ? a.x[1] : a.x[0]) + t * (which ? a.row_stride[1] : a.row_stride[0]);
+    const long long head_stride = which ? a.head_stride[1] : a.head_stride[0];
+    uint2 raw[kSegBlocks / 4];
+#pragma unroll
+    for (int i = 0; i < kSegBlocks / 4; ++i) {
+      const int blk = b0 + min(4 * i + (lane >> 3), blocks - 1);  // a repeated last block keeps all lanes in the shuffles
+      const int h = blk / a.NB, j = blk - h * a.NB;
+      const T* src = x + h * head_stride + j * 32 + sub * 4;
+      if ((reinterpret_cast<uintptr_t>(src) & 7) == 0) {
+        raw[i] = *reinterpret_cast<const uint2*>(src);
+      } else {
+        const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
+        raw[i] = make_uint2(s16[0] | ((uint32_t)s16[1] << 16), s16[2] | ((uint32_t)s16[3] << 16));
+      }
+    }
+    const bool keep = slot >= 0 && slot < a.num_slots;
+    uint8_t* dst = (which ? a.cache[1] : a.cache[0]) + (keep ? (slot * per_row + b0) * kQ8 : 0);
+    const int off = (int)(reinterpret_cast<uintptr_t>(dst) & 15);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kSegBlocks / 4; ++i) {
+      const float2 f0 = to_float2<T>(raw[i].x), f1 = to_float2<T>(raw[i].y);
+      const float v[4] = {f0.x, f0.y, f1.x, f1.y};
+      float amax = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+      for (int o = 1; o <= 4; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(full, amax, o));
+      const float d = amax > 0.0f ? __fdiv_rn(amax, 127.0f) : 1.0f;
+      const float inv = 1.0f / d;
+      uint32_t code = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) code |= (uint32_t)(code_of(v[k], d, inv) & 0xff) << (8 * k);
+      const int blk = 4 * i + (lane >> 3);
+      if (blk < blocks) {
+        uint16_t* o = reinterpret_cast<uint16_t*>(s_seg[warp] + off + blk * kQ8);
+        o[1 + 2 * sub] = (uint16_t)code;
+        o[2 + 2 * sub] = (uint16_t)(code >> 16);
+        if (sub == 0) o[0] = (uint16_t)float_to_half_bits(d);
+      }
+    }
+    __syncwarp();
+    if (keep) {
+      const int end = off + blocks * kQ8;
+      for (int p = lane * 16; p < end; p += 512) {
+        if (p >= off && p + 16 <= end) {
+          *reinterpret_cast<uint4*>(dst - off + p) = *reinterpret_cast<const uint4*>(s_seg[warp] + p);
+        } else {  // the segment's ragged ends
+          for (int k = max(p, off); k < min(p + 16, end); k += 2)
+            *reinterpret_cast<uint16_t*>(dst - off + k) = *reinterpret_cast<const uint16_t*>(s_seg[warp] + k);
+        }
+      }
+    }
   }
 }
 
@@ -268,46 +313,94 @@ struct ReadArgs {
   void* out[2];
   const int32_t* table;
   const int32_t* cu;
-  int B, W, ps, H, NB;
+  int B, W, ps, H, NB, segs;
   long long num_pages, rows;
 };
 
-// One warp per packed row (all heads of one token): lane l takes chunks of 8
-// codes l, l + 32, ... of the row, 16 bytes out per chunk. blockIdx.y picks K
-// or V. A row whose page id is outside the cache, and a row that no sequence
-// owns, is zero.
+// A unit is a segment of up to 32 blocks of one packed row of K or V; a warp
+// takes kReadUnits of them. Lanes look the units' cache slots up side by side,
+// the loads of all units (whole 16-byte pieces, from the boundary below) are in
+// flight at once, then each unit is laid out in shared memory and lane l
+// converts its codes 8 l, 8 l + 256, ..., 16 bytes out at a time. A row whose
+// page id is outside the cache, and a row that no sequence owns, is zero.
+// Bound by memory, 34 bytes in and 64 out per block. More units per warp put
+// more loads in flight but leave fewer warps: 22445 rows of 8 x 128 after 4096
+// written take 50.7 us with 1, 46.0 with 2, 51.4 with 4 (both calls).
+constexpr int kReadUnits = 2;
+constexpr int kUnitPieces = (kSegRoom / 16 + 31) / 32;  // of a unit, per lane
+
 template <typename T>
-__global__ void __launch_bounds__(256) page_read_kernel(const ReadArgs a) {
-  const int lane = threadIdx.x & 31, which = blockIdx.y;
-  const long long nwarps = (long long)gridDim.x * (blockDim.x >> 5);
+__global__ void __launch_bounds__(256, 4) page_read_kernel(const ReadArgs a) {
+  __shared__ __align__(16) uint8_t s_seg[8][kSegRoom];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per_row = a.H * a.NB;
-  for (long long r = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); r < a.rows; r += nwarps) {
-    int lo = 0, hi = a.B;  // last b with cu[b] <= r
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu[mid] <= r) lo = mid;
-      else hi = mid;
-    }
-    long long page = -1;
-    const long long pos = r - a.cu[lo];
-    if (pos >= 0 && r < a.cu[lo + 1] && pos / a.ps < a.W) page = a.table[(long long)lo * a.W + pos / a.ps];
-    const bool valid = page >= 0 && page < a.num_pages;
-    const uint8_t* src = a.cache[which] + (valid ? (page * a.ps + pos % a.ps) * per_row * kQ8 : 0);
-    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out[which]) + r * per_row * 32);
-    for (int c = lane; c < per_row * 4; c += 32) {
-      uint4 o = make_uint4(0, 0, 0, 0);
-      if (valid) {
-        const uint16_t* blk = reinterpret_cast<const uint16_t*>(src + (c >> 2) * kQ8);
-        const float d = half_bits_to_float(blk[0]);
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t two = blk[1 + (c & 3) * 4 + i];
-          w[i] = pack2<T>(d * (float)(int8_t)(two & 0xff), d * (float)(int8_t)(two >> 8));
-        }
-        o = make_uint4(w[0], w[1], w[2], w[3]);
+  const long long row_bytes = (long long)per_row * kQ8, cache_bytes = a.num_pages * a.ps * row_bytes;
+  uint8_t* seg = s_seg[warp];
+  const long long units = a.rows * 2 * a.segs;
+  for (long long u0 = ((long long)blockIdx.x * 8 + warp) * kReadUnits; u0 < units; u0 += (long long)gridDim.x * 8 * kReadUnits) {
+    // lane i: the place of unit i's first byte in its cache, -1 without one
+    long long at = -1;
+    if (lane < kReadUnits && u0 + lane < units) {
+      const long long r = (u0 + lane) / (2 * a.segs);
+      int lo = 0, hi = a.B;  // last b with cu[b] <= r
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu[mid] <= r) lo = mid;
+        else hi = mid;
       }
-      dst[c] = o;
+      const long long pos = r - a.cu[lo];
+      if (pos >= 0 && r < a.cu[lo + 1] && pos / a.ps < a.W) {
+        const long long page = a.table[(long long)lo * a.W + pos / a.ps];
+        if (page >= 0 && page < a.num_pages)
+          at = (page * a.ps + pos % a.ps) * row_bytes + (u0 + lane) % a.segs * (kSegBlocks * kQ8);
+      }
+    }
+    uint4 v[kReadUnits][kUnitPieces];
+    long long from[kReadUnits];
+#pragma unroll
+    for (int i = 0; i < kReadUnits; ++i) {
+      from[i] = __shfl_sync(0xffffffffu, at, i);
+      const uint8_t* cache = ((u0 + i) / a.segs & 1) ? a.cache[1] : a.cache[0];
+      const int b0 = (int)((u0 + i) % a.segs) * kSegBlocks, blocks = min(kSegBlocks, per_row - b0);
+      const long long first = from[i] & ~15ll, end = min(from[i] + blocks * kQ8, cache_bytes);
+#pragma unroll
+      for (int k = 0; k < kUnitPieces; ++k) {
+        const long long p = first + 16 * (lane + 32 * k);
+        v[i][k] = make_uint4(0, 0, 0, 0);
+        if (from[i] < 0 || p >= end) continue;
+        if (p + 16 <= cache_bytes) {
+          v[i][k] = *reinterpret_cast<const uint4*>(cache + p);
+        } else {  // the cache's last bytes
+          const int left = (int)(cache_bytes - p);
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(cache + p);
+          auto half = [&](int x) { return 2 * x < left ? (uint32_t)h[x] : 0u; };
+          v[i][k] = make_uint4(half(0) | half(1) << 16, half(2) | half(3) << 16, half(4) | half(5) << 16, half(6));
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kReadUnits; ++i) {
+      if (u0 + i >= units) break;
+      const long long r = (u0 + i) / (2 * a.segs);
+      const int which = (int)((u0 + i) / a.segs & 1), b0 = (int)((u0 + i) % a.segs) * kSegBlocks;
+      const int blocks = min(kSegBlocks, per_row - b0), off = from[i] < 0 ? 0 : (int)(from[i] & 15);
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(which ? a.out[1] : a.out[0]) + (r * per_row + b0) * 32);
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < kUnitPieces; ++k)
+        if (16 * (lane + 32 * k) < kSegRoom) *reinterpret_cast<uint4*>(seg + 16 * (lane + 32 * k)) = v[i][k];
+      __syncwarp();
+      for (int c = lane; c < blocks * 4; c += 32) {
+        const int blk = off + (c >> 2) * kQ8, x = blk + 2 + (c & 3) * 8;  // even
+        const float d = half_bits_to_float(*reinterpret_cast<const uint16_t*>(seg + blk));
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(seg + (x & ~3));
+        const uint32_t sh = (uint32_t)(x & 2) * 8, top = sh ? w[2] : 0u;
+        const uint32_t w0 = __funnelshift_r(w[0], w[1], sh), w1 = __funnelshift_r(w[1], top, sh);
+        auto value = [&](uint32_t word, int k) { return d * (float)(int8_t)(word >> (8 * k)); };
+        uint4 o = make_uint4(pack2<T>(value(w0, 0), value(w0, 1)), pack2<T>(value(w0, 2), value(w0, 3)),
+                             pack2<T>(value(w1, 0), value(w1, 1)), pack2<T>(value(w1, 2), value(w1, 3)));
+        dst[c] = from[i] < 0 ? make_uint4(0, 0, 0, 0) : o;
+      }
     }
   }
 }
@@ -324,7 +417,7 @@ kq_status_t launch_page_plan(const int32_t* cached, const int32_t* fresh, int B,
                              int32_t* cu_new, int32_t* cu_seqlens, int32_t* counts, cudaStream_t s) {
   PlanArgs a{cached, fresh, B, table, W, free_pages, F, ps, T, reinterpret_cast<long long*>(slots), seq_lens, cu_new,
              cu_seqlens, counts};
-  page_plan_kernel<<<grid_for(T, kPlan * 4, 1), kPlan, 0, s>>>(a);
+  page_plan_kernel<<<grid_for(T, kPlan, 1), kPlan, 0, s>>>(a);
   return check_launch("page_plan");
 }
 
@@ -338,9 +431,10 @@ kq_status_t launch_page_write_q8_0(int dtype, const void* k, const void* v, cons
   a.cache[0] = static_cast<uint8_t*>(k_cache), a.cache[1] = static_cast<uint8_t*>(v_cache);
   a.slots = reinterpret_cast<const long long*>(slots);
   a.H = H, a.NB = D / 32;
-  a.blocks = (long long)T * H * a.NB;
+  a.T = T;
+  a.segs = (H * a.NB + kSegBlocks - 1) / kSegBlocks;
   a.num_slots = num_slots;
-  const dim3 grid(grid_for(a.blocks, 32, 8), 2);
+  const int grid = grid_for(T * 2 * a.segs, 8, 8);
   if (dtype == KQ_F16) page_write_kernel<__half><<<grid, 256, 0, s>>>(a);
   else page_write_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
   return check_launch("page_write");
@@ -355,7 +449,8 @@ kq_status_t launch_page_read_q8_0(int dtype, const void* k_cache, const void* v_
   a.table = table, a.cu = cu;
   a.B = B, a.W = W, a.ps = ps, a.H = H, a.NB = D / 32;
   a.num_pages = num_pages, a.rows = rows;
-  const dim3 grid(grid_for(rows, 8, 8), 2);
+  a.segs = (H * a.NB + kSegBlocks - 1) / kSegBlocks;
+  const int grid = grid_for(rows * 2 * a.segs, 8 * kReadUnits, 8);
   if (dtype == KQ_F16) page_read_kernel<__half><<<grid, 256, 0, s>>>(a);
   else page_read_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
   return check_launch("page_read");
