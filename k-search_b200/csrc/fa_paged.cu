@@ -109,9 +109,8 @@ __device__ __forceinline__ int units_before(const Split& sp, const SplitScan<T>&
 //     that small scales stay in fp16's normal range. d_v up to 1023 fits.
 // The head dimension is permuted inside a block so that every operand word is
 // one 32-bit load (a word of 4 codes) per lane.
-constexpr int kStreamWarps = 12;
-constexpr int kStreamThreads = kStreamWarps * 32;
-constexpr int kStages = 3;
+constexpr int kStreamWarps = 12;  // 12 warps with 3 stages, or 8 with 6 where there is little to stream
+constexpr int kFewWarps = 8;
 constexpr float kPBits = 6.0f, kPScale = 64.0f;
 
 template <int NB>
@@ -125,9 +124,13 @@ struct Row {
   static constexpr int COPIES = (8 * CHUNKS + 31) / 32;  // per lane, for 8 rows
   static constexpr bool ALWAYS = 16 * (CHUNKS - 1) < BYTES;  // every piece holds bytes of the row wherever it starts
   static constexpr int STAGE = 2 * kUnit * PITCH;
-  // fewer stages where the rows are long
-  static constexpr int STAGES = kStreamWarps * kStages * STAGE <= 221184 ? kStages : 2;
-  static constexpr int SMEM = kStreamWarps * STAGES * STAGE;
+};
+// A warp's ring: fewer stages where the rows are long.
+template <int NB, int WARPS>
+struct Ring {
+  static constexpr int MOST = WARPS == kStreamWarps ? 3 : 6;
+  static constexpr int STAGES = std::min(MOST, 221184 / (WARPS * Row<NB>::STAGE));
+  static constexpr int SMEM = WARPS * STAGES * Row<NB>::STAGE;
 };
 
 // 16 bytes to shared memory, asynchronously (groups of them are waited for).
@@ -172,6 +175,7 @@ struct StreamArgs {
   const int32_t* table;
   int prefix_len;  // tokens below it (a multiple of 8) lie in row 0's pages
   Split split;
+  int warps;    // per CTA
   float sl;     // scale * log2(e)
   float* part;  // [segment][Hq][NB * 32] accumulators
   float2* ml;   // [segment][Hq] maximum (log2 units), sum
@@ -216,20 +220,22 @@ struct Cursor {
   int col, off;   // its page (a column of the table) and place in it
 };
 
-template <int NB, bool WIDE>
-__global__ void __launch_bounds__(kStreamThreads, 1) fa_paged_stream_kernel(const StreamArgs a) {
+template <int NB, bool WIDE, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const StreamArgs a) {
   using R = Row<NB>;
-  constexpr int kSt = R::STAGES;
+  constexpr int kSt = Ring<NB, WARPS>::STAGES, kThreads = WARPS * 32;
   constexpr int RH = WIDE ? 2 : 1;  // row halves in use: query heads lane / 4 (+ 8)
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(16) float s_scale[kStreamWarps][2][NB][kUnit];  // K and V scales of the tile at hand
-  auto& ss = *reinterpret_cast<SplitScan<kStreamThreads>*>(smem);        // before the rings are in use
+  __shared__ __align__(16) float s_scale[WARPS][2][NB][kUnit];  // K and V scales of the tile at hand
+  auto& ss = *reinterpret_cast<SplitScan<kThreads>*>(smem);        // before the rings are in use
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   pdl_launch_dependents();
   scan_units(a.split, ss);
-  const int U = ss.scan[kStreamThreads], C = a.split.active(U);
+  const int U = ss.scan[kThreads], C = a.split.active(U);
   const int per_worker = a.Hkv * a.QG;
-  const int gw = blockIdx.x * kStreamWarps + warp;
+  // few workers: over all CTAs, as many warps in each
+  const int used = (C * per_worker + gridDim.x - 1) / gridDim.x;
+  const int gw = warp < used ? blockIdx.x * used + warp : C * per_worker;
   const int wk = gw / per_worker, hw = gw % per_worker, h = hw / a.QG, qg = hw % a.QG;
   // a programmatic dependent of the prefix kernel, whose results it does not
   // read: it only may not end before it (the combine waits for this grid)
@@ -239,13 +245,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1) fa_paged_stream_kernel(cons
     const Shares shares(U, C);
     u = shares.begin(wk), ue = shares.begin(wk + 1);
     if (u < ue) {
-      int lo = 0, hi = kStreamThreads;
+      int lo = 0, hi = kThreads;
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (ss.scan[mid] <= u) lo = mid;
         else hi = mid;
       }
-      f.b = lo * run_len<kStreamThreads>(a.split);
+      f.b = lo * run_len<kThreads>(a.split);
       int before = ss.scan[lo], here;
       while (before + (here = a.split.units(f.b)) <= u) {
         before += here;
@@ -1167,13 +1173,22 @@ __global__ void __launch_bounds__(kWarps * 32) fa_paged_simple_kernel(const FaPa
 }
 
 // Workers per KV head (and group of 16 of its query heads): one CTA's warps per SM in all.
-int workers_of(const FaPagedArgs& a) {
+int workers_of(const FaPagedArgs& a, int warps) {
   const int qg = (a.Hq / a.Hkv + 15) / 16;
-  return std::max(1, sm_count() * kStreamWarps / (a.Hkv * qg));
+  return std::max(1, sm_count() * warps / (a.Hkv * qg));
 }
-// The prefix kernel's pass: head dimensions up to 128, whole groups of 8
-// tokens per page, and a batch (one sequence alone streams its prefix).
-bool use_prefix(const FaPagedArgs& a) { return a.prefix_len > 0 && a.D <= 128 && a.B > 1; }
+// The prefix kernel's pass, for head dimensions up to 128: a third launch that
+// costs 5 to 10 us, against the tokens that streaming would read once per
+// sequence. Where those are few they are streamed (us with and without it, 8
+// KV heads of 128, 300 tokens behind the prefix: 8 sequences behind 1024 18.5
+// and 17.1, behind 4096 24.0 and 32.8; 32 behind 256 19.3 and 17.2, behind 1024
+// 23.3 and 34.9). Streaming needs a prefix of whole groups of 8.
+constexpr int kPrefixUnits = 40;  // units of repeated reading per SM that it pays from
+bool use_prefix(const FaPagedArgs& a) {
+  if (a.prefix_len <= 0 || a.D > 128 || a.B <= 1) return false;
+  const long long again = (long long)(a.B - 1) * a.prefix_len * a.Hkv;
+  return a.prefix_len % 8 || again >= (long long)kPrefixUnits * kUnit * sm_count();
+}
 // Token chunks of the prefix, so that the grid fills the SMs once.
 int prefix_groups(const FaPagedArgs& a) {  // (KV head, pair of row tiles)
   const long long rows = (long long)a.B * (a.Hq / a.Hkv);
@@ -1188,7 +1203,7 @@ struct Workspace {
   size_t part, ml, ppart, pml, total;  // offsets
 };
 Workspace workspace_of(const FaPagedArgs& a) {
-  const size_t rows = ((size_t)workers_of(a) + a.B) * a.Hq, prows = (size_t)prefix_chunks(a) * a.B * a.Hq;
+  const size_t rows = ((size_t)workers_of(a, kStreamWarps) + a.B) * a.Hq, prows = (size_t)prefix_chunks(a) * a.B * a.Hq;
   Workspace w;
   w.part = 0;
   w.ppart = rows * a.D * sizeof(float);
@@ -1229,15 +1244,19 @@ kq_status_t launch_after(void (*kernel)(Params...), int grid, int threads, int s
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, arg), what);
 }
 
-template <int NB, bool WIDE>
-kq_status_t launch_stream(const StreamArgs& a, int grid, bool pdl, cudaStream_t s) {
-  auto kernel = fa_paged_stream_kernel<NB, WIDE>;
-  if (kq_status_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), Row<NB>::SMEM, "fa_paged")) return st;
-  return launch_after(kernel, grid, kStreamThreads, Row<NB>::SMEM, pdl, s, a, "fa_paged_stream");
+template <int NB, bool WIDE, int WARPS>
+kq_status_t launch_stream(const StreamArgs& a, bool pdl, cudaStream_t s) {
+  auto kernel = fa_paged_stream_kernel<NB, WIDE, WARPS>;
+  constexpr int smem = Ring<NB, WARPS>::SMEM;
+  if (kq_status_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, "fa_paged")) return st;
+  const int grid = (a.split.workers * a.Hkv * a.QG + WARPS - 1) / WARPS;
+  return launch_after(kernel, grid, WARPS * 32, smem, pdl, s, a, "fa_paged_stream");
 }
 template <int NB>
-kq_status_t launch_stream_nb(const StreamArgs& a, int grid, bool pdl, cudaStream_t s) {
-  return a.G > 8 ? launch_stream<NB, true>(a, grid, pdl, s) : launch_stream<NB, false>(a, grid, pdl, s);
+kq_status_t launch_stream_nb(const StreamArgs& a, bool pdl, cudaStream_t s) {
+  if (a.warps == kFewWarps)
+    return a.G > 8 ? launch_stream<NB, true, kFewWarps>(a, pdl, s) : launch_stream<NB, false, kFewWarps>(a, pdl, s);
+  return a.G > 8 ? launch_stream<NB, true, kStreamWarps>(a, pdl, s) : launch_stream<NB, false, kStreamWarps>(a, pdl, s);
 }
 
 // Eight warps per row while that leaves the SMs room, else one.
@@ -1279,7 +1298,13 @@ kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s) {
   p.QG = (p.G + 15) / 16;
   p.split.seq_lens = a.seq_lens, p.split.B = a.B, p.split.start = chunks ? a.prefix_len : 0;
   p.split.limit = (int)std::min<long long>(a.max_seqlen, (long long)a.W * a.ps);
-  p.split.workers = workers_of(a);
+  // Little to stream is bound by latency: fewer warps with deeper rings start
+  // sooner (3000 tokens of one sequence, 8 KV heads of 128: 11.0 us with 8
+  // warps, 13.7 with 12; 4 x 9000: 21.8 and 25.3); more is bound by issue
+  // slots (16 x 3000: 30.1 and 28.1, 16 x 16000: 112 and 102).
+  const long long units = (long long)a.B * a.Hkv * p.QG * ((p.split.limit - p.split.start) / kUnit + 1);
+  p.warps = units <= 16ll * kFewWarps * sm_count() ? kFewWarps : kStreamWarps;
+  p.split.workers = workers_of(a, p.warps);
   p.sl = a.scale * 1.44269504088896340736f;
   p.part = reinterpret_cast<float*>(ws + w.part), p.ml = reinterpret_cast<float2*>(ws + w.ml);
   kq_status_t st = KQ_OK;
@@ -1303,16 +1328,15 @@ kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s) {
     if (st) return st;
   }
   const bool pdl = chunks > 0;
-  const int grid = (p.split.workers * a.Hkv * p.QG + kStreamWarps - 1) / kStreamWarps;
   switch (a.D / 32) {
-    case 1: st = launch_stream_nb<1>(p, grid, pdl, s); break;
-    case 2: st = launch_stream_nb<2>(p, grid, pdl, s); break;
-    case 3: st = launch_stream_nb<3>(p, grid, pdl, s); break;
-    case 4: st = launch_stream_nb<4>(p, grid, pdl, s); break;
-    case 5: st = launch_stream_nb<5>(p, grid, pdl, s); break;
-    case 6: st = launch_stream_nb<6>(p, grid, pdl, s); break;
-    case 7: st = launch_stream_nb<7>(p, grid, pdl, s); break;
-    default: st = launch_stream_nb<8>(p, grid, pdl, s); break;
+    case 1: st = launch_stream_nb<1>(p, pdl, s); break;
+    case 2: st = launch_stream_nb<2>(p, pdl, s); break;
+    case 3: st = launch_stream_nb<3>(p, pdl, s); break;
+    case 4: st = launch_stream_nb<4>(p, pdl, s); break;
+    case 5: st = launch_stream_nb<5>(p, pdl, s); break;
+    case 6: st = launch_stream_nb<6>(p, pdl, s); break;
+    case 7: st = launch_stream_nb<7>(p, pdl, s); break;
+    default: st = launch_stream_nb<8>(p, pdl, s); break;
   }
   if (st) return st;
   CombineArgs ca{p.split, p.part, p.ml, reinterpret_cast<float*>(ws + w.ppart), reinterpret_cast<float2*>(ws + w.pml),

@@ -370,6 +370,10 @@ DECODES = [
     ([260 + 3 * i for i in range(40)], 256, 16, 32, 8, 128), ([2100, 2048, 2300], 2048, 128, 4, 4, 128),
     ([130, 140], 128, 16, 8, 2, 256), ([150] * 33, 96, 16, 28, 4, 64), ([200, 210], 128, 16, 128, 1, 128),
     ([35] * 300, 32, 16, 4, 2, 32), ([515, 700], 512, 16, 48, 2, 128),
+    # prefixes that many sequences share, or that end within 8 tokens: a pass of their own
+    ([640 + 3 * i for i in range(40)], 640, 16, 32, 8, 128), ([330] * 299 + [7], 320, 16, 4, 2, 32),
+    ([2048 + 40 * i for i in range(14)], 2048, 128, 28, 4, 64), ([1030] * 100 + [500, 0], 1024, 32, 8, 1, 96),
+    ([700 + i for i in range(30)], 699, 24, 15, 5, 64), ([129, 200], 127, 16, 4, 4, 32),
 ]
 
 
@@ -404,7 +408,7 @@ def test_decode_copied_last_page(cuda, D, ps, prefix):
     check_out(kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix), ref, spread, top, torch.float16)
 
 
-@pytest.mark.parametrize("prefix", [0, 128])
+@pytest.mark.parametrize("prefix", [0, 128, 131])
 @pytest.mark.parametrize("case", ["growing", "huge", "equal", "scales"])
 def test_decode_score_ranges(cuda, prefix, case):
     import kq
@@ -434,11 +438,12 @@ def test_decode_score_ranges(cuda, prefix, case):
     check_out(got, ref, spread, top, torch.float16, case)
 
 
-def test_decode_hidden_pages(cuda):
+@pytest.mark.parametrize("prefix", [64, 61])
+def test_decode_hidden_pages(cuda, prefix):
     """A page id outside the cache hides its tokens, in the prefix and behind it."""
     import kq
     g = gen(11)
-    lens, ps, prefix = [200, 170], 16, 64
+    lens, ps = [200, 170], 16
     kc, vc, table = paged_case(g, lens, prefix, ps, 2, 128)
     table[:, 1] = -1
     table[0, 7] = kc.shape[0] + 5
@@ -450,11 +455,12 @@ def test_decode_hidden_pages(cuda):
     check_out(got, ref, spread, top, torch.float16)
 
 
-def test_decode_unowned_cache_rows_do_not_matter(cuda):
+@pytest.mark.parametrize("prefix", [64, 61])
+def test_decode_unowned_cache_rows_do_not_matter(cuda, prefix):
     """NaN scales in rows behind a sequence's end, and in pages nobody owns, change nothing."""
     import kq
     g = gen(12)
-    lens, ps, prefix = [100, 70, 0, 69], 16, 64
+    lens, ps = [100, 70, 0, 69], 16
     kc, vc, table = paged_case(g, lens, prefix, ps, 4, 128)
     q = rows(g, 4, 16, 128, torch.float16)
     ref, spread, top = decode_ref(q, kc, vc, table, lens, 128 ** -0.5)
