@@ -182,11 +182,24 @@ struct StreamArgs {
 };
 
 // d = a b + (c0, c1, c2, c3)
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1, float c0, float c1, float c2, float c3) {
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1,
+                                         float c2, float c3) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+// The 8 x 8 matrix with elements (g, 2 c) and (g, 2 c + 1) in lane 4 g + c,
+// transposed: halves of the 32-bit values in two 16-bit transpositions.
+__device__ __forceinline__ uint32_t movm(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ void transpose8(float x0, float x1, float& y0, float& y1) {
+  const uint32_t a = __float_as_uint(x0), b = __float_as_uint(x1);
+  const uint32_t lo = movm(__byte_perm(a, b, 0x5410)), hi = movm(__byte_perm(a, b, 0x7632));
+  y0 = __uint_as_float(__byte_perm(lo, hi, 0x5410));
+  y1 = __uint_as_float(__byte_perm(lo, hi, 0x7632));
 }
 __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -381,11 +394,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
         qa[i][RH + r] = w[i].y;
       }
     }
-    float acc[NB * 4][2 * RH];
+    float acc[NB * 2][RH][4];  // O^T: dims 32 (i / 2) + 4 g + 2 (i % 2) + {0, 1} of heads 8 r + 2 c + {0, 1}
 #pragma unroll
-    for (int i = 0; i < NB * 4; ++i)
+    for (int i = 0; i < NB * 2; ++i)
 #pragma unroll
-      for (int r = 0; r < 2 * RH; ++r) acc[i][r] = 0.0f;
+      for (int r = 0; r < RH; ++r)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[i][r][x] = 0.0f;
     float m[RH], l[RH];
 #pragma unroll
     for (int r = 0; r < RH; ++r) m[r] = -INFINITY, l[r] = 0.0f;
@@ -431,31 +446,39 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
       __syncwarp();
       auto scales = [&](int kv, int j, int i) { return *reinterpret_cast<const float2*>(&s_scale[warp][kv][j][i]); };
 
-      float s[2][2 * RH];
+      // S^T: tokens g and g + 8 of heads 8 r + 2 c + {0, 1}
+      float st4[RH][4];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint8_t* kr = stage + at_k + t * 8 * R::PITCH;
+      for (int r = 0; r < RH; ++r)
 #pragma unroll
-        for (int r = 0; r < 2 * RH; ++r) s[t][r] = 0.0f;
+        for (int x = 0; x < 4; ++x) st4[r][x] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          float d[4];
-          uint32_t b0, b1;
-          const uint32_t* q = qa[2 * j];
-          codes_h2(word_at<NB>(kr, j * kQ8 + 2), b0, b1);
-          mma16816(d, q[0], WIDE ? q[1] : 0u, q[RH], WIDE ? q[2 * RH - 1] : 0u, b0, b1, 0.0f, 0.0f, 0.0f, 0.0f);
-          q = qa[2 * j + 1];
-          codes_h2(word_at<NB>(kr, j * kQ8 + 18), b0, b1);
-          mma16816(d, q[0], WIDE ? q[1] : 0u, q[RH], WIDE ? q[2 * RH - 1] : 0u, b0, b1, d[0], d[1], WIDE ? d[2] : 0.0f,
-                   WIDE ? d[3] : 0.0f);
-          const float2 dk = scales(0, j, 8 * t + 2 * c);
+      for (int j = 0; j < NB; ++j) {
+        float d[RH][4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t k4[4];
+          codes_h2(word_at<NB>(stage + at_k, j * kQ8 + 2 + 16 * half), k4[0], k4[2]);
+          codes_h2(word_at<NB>(stage + at_k + 8 * R::PITCH, j * kQ8 + 2 + 16 * half), k4[1], k4[3]);
 #pragma unroll
           for (int r = 0; r < RH; ++r) {
-            s[t][2 * r] = fmaf(d[2 * r], dk.x, s[t][2 * r]);
-            s[t][2 * r + 1] = fmaf(d[2 * r + 1], dk.y, s[t][2 * r + 1]);
+            const uint32_t* q = qa[2 * j + half];
+            if (half == 0) mma16816(d[r], k4, q[r], q[RH + r], 0.0f, 0.0f, 0.0f, 0.0f);
+            else mma16816(d[r], k4, q[r], q[RH + r], d[r][0], d[r][1], d[r][2], d[r][3]);
           }
         }
+        const float dk0 = s_scale[warp][0][j][g], dk1 = s_scale[warp][0][j][g + 8];
+#pragma unroll
+        for (int r = 0; r < RH; ++r)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) st4[r][x] = fmaf(d[r][x], x < 2 ? dk0 : dk1, st4[r][x]);
       }
+      // transposed: head g (+ 8) of tokens 8 t + 2 c + {0, 1}, as P is needed
+      float s[2][2 * RH];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < RH; ++r) transpose8(st4[r][2 * t], st4[r][2 * t + 1], s[t][2 * r], s[t][2 * r + 1]);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -494,9 +517,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
       }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-        for (int i = 0; i < NB * 4; ++i)
+        for (int r = 0; r < RH; ++r) {
+          const float f0 = __shfl_sync(0xffffffffu, f_[r], 8 * c), f1 = __shfl_sync(0xffffffffu, f_[r], 8 * c + 4);
 #pragma unroll
-          for (int r = 0; r < 2 * RH; ++r) acc[i][r] *= f_[r >> 1];
+          for (int i = 0; i < NB * 2; ++i) acc[i][r][0] *= f0, acc[i][r][1] *= f1, acc[i][r][2] *= f0, acc[i][r][3] *= f1;
+        }
       }
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
@@ -515,16 +540,17 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
         const uint32_t x01 = __byte_perm(w[0], w[1], 0x5140), x23 = __byte_perm(w[0], w[1], 0x7362);
         const uint32_t y01 = __byte_perm(w[2], w[3], 0x5140), y23 = __byte_perm(w[2], w[3], 0x7362);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t sel = (i & 1) ? 0x4342u : 0x4140u;
-          const uint32_t b0 = hsub2(__byte_perm(i < 2 ? x01 : x23, 0x64646464u, sel), 0x64806480u);
-          const uint32_t b1 = hsub2(__byte_perm(i < 2 ? y01 : y23, 0x64646464u, sel), 0x64806480u);
-          float* d = acc[4 * j + i];
-          float t4[4];
-          mma16816(t4, pa[0], WIDE ? pa[1] : 0u, pa[RH], WIDE ? pa[2 * RH - 1] : 0u, b0, b1, d[0], d[1],
-                   WIDE ? d[2 * RH - 2] : 0.0f, WIDE ? d[2 * RH - 1] : 0.0f);
-          d[0] = t4[0], d[1] = t4[1];
-          if (WIDE) d[2 * RH - 2] = t4[2], d[2 * RH - 1] = t4[3];
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t x = i ? x23 : x01, y = i ? y23 : y01;
+          const uint32_t v4[4] = {hsub2(__byte_perm(x, 0x64646464u, 0x4140), 0x64806480u),
+                                  hsub2(__byte_perm(x, 0x64646464u, 0x4342), 0x64806480u),
+                                  hsub2(__byte_perm(y, 0x64646464u, 0x4140), 0x64806480u),
+                                  hsub2(__byte_perm(y, 0x64646464u, 0x4342), 0x64806480u)};
+#pragma unroll
+          for (int r = 0; r < RH; ++r) {
+            float(&o)[4] = acc[2 * j + i][r];
+            mma16816(o, v4, pa[r], pa[RH + r], o[0], o[1], o[2], o[3]);
+          }
         }
       }
       __syncwarp();  // the stage may be refilled
@@ -540,14 +566,17 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
       const int hl = qg * 16 + g + 8 * r;
       if (hl < a.G) {
         const long long row = seg * a.Hq + h * a.G + hl;
-        float4* o = reinterpret_cast<float4*>(a.part + row * (NB * 32));
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          o[8 * j + 2 * c] = make_float4(acc[4 * j][2 * r], acc[4 * j + 1][2 * r], acc[4 * j + 2][2 * r], acc[4 * j + 3][2 * r]);
-          o[8 * j + 2 * c + 1] = make_float4(acc[4 * j][2 * r + 1], acc[4 * j + 1][2 * r + 1], acc[4 * j + 2][2 * r + 1],
-                                             acc[4 * j + 3][2 * r + 1]);
-        }
         if (c == 0) a.ml[row] = make_float2(m[r] - kPBits, sum * kPScale);  // the sums carry 2^kPBits: as if m were lower
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int ho = qg * 16 + 8 * r + 2 * c + x;
+        if (ho < a.G) {
+          float4* o = reinterpret_cast<float4*>(a.part + (seg * a.Hq + h * a.G + ho) * (NB * 32)) + g;
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+            o[8 * j] = make_float4(acc[2 * j][r][x], acc[2 * j][r][2 + x], acc[2 * j + 1][r][x], acc[2 * j + 1][r][2 + x]);
+        }
       }
     }
   }
