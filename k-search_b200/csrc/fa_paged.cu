@@ -162,7 +162,7 @@ struct Pieces {
   __device__ __forceinline__ void copy(uint32_t to, const uint8_t* from) const {
 #pragma unroll
     for (int i = 0; i < R::COPIES; ++i)
-      if (src[i] >= 0) copy16(to + dst[i], from + src[i]);
+      if (src[i] >= 0) copy16(to + dst[i], from + (uint32_t)src[i]);
   }
 };
 
@@ -241,7 +241,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(16) float s_scale[WARPS][2][NB][kUnit];  // K and V scales of the tile at hand
   auto& ss = *reinterpret_cast<SplitScan<kThreads>*>(smem);        // before the rings are in use
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  // broadcasts of what is the same in a warp anyway: the row of units and the
+  // copies' bases then run on uniform registers (16 x 16000 tokens 89 -> 84 us)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   pdl_launch_dependents();
   scan_units(a.split, ss);
   const int U = ss.scan[kThreads], C = a.split.active(U);
@@ -320,7 +322,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
     uint32_t mask = 0;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int page = half ? p.y : p.x, tok = x.tok + 8 * half;
+      const int page = __shfl_sync(0xffffffffu, half ? p.y : p.x, 0), tok = x.tok + 8 * half;
       if (page >= 0 && page < a.num_pages) {
         const int off = x.off + 8 * half;
         const long long at = ((long long)page * a.ps + (off >= a.ps ? off - a.ps : off)) * row_bytes;
