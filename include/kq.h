@@ -353,14 +353,15 @@ kq_status_t kq_page_plan(const int32_t* cached_lens, const int32_t* new_lens, in
  * elements, last dimension contiguous) quantised to q8_0 into the cache rows
  * slots[t] (int64; below 0 or >= num_slots: the row is skipped). The bytes
  * are those of kq_quantize_rows on the same values. Slots of one call must
- * differ. */
+ * differ. Rows and caches are 2-byte aligned. */
 kq_status_t kq_page_write_q8_0(int dtype, const void* k, const void* v, int64_t k_row_stride, int64_t k_head_stride,
                                int64_t v_row_stride, int64_t v_head_stride, const int64_t* slots, int64_t T, int Hkv,
                                int D, void* k_cache, void* v_cache, int64_t num_slots, kq_stream_t stream);
 
 /* The sequences' cache rows in packed order: row cu_seqlens[b] + i of k and v
  * [total_rows, Hkv, D] is token i of sequence b, d * code rounded to dtype.
- * Rows of pages outside the cache, and rows past cu_seqlens[B], are zero. */
+ * Rows of pages outside the cache, and rows past cu_seqlens[B], are zero. The
+ * caches, k and v are 16-byte aligned. */
 kq_status_t kq_page_read_q8_0(int dtype, const void* k_cache, const void* v_cache, int64_t num_pages, int page_size,
                               int Hkv, int D, const int32_t* block_tables, int max_blocks, const int32_t* cu_seqlens,
                               int B, int64_t total_rows, void* k, void* v, kq_stream_t stream);
@@ -370,7 +371,12 @@ kq_status_t kq_page_read_q8_0(int dtype, const void* k_cache, const void* v_cach
  * contiguous, all of dtype. Sequence b owns q rows cu_seqlens_q[b] ..
  * cu_seqlens_q[b+1]-1 and k / v rows cu_seqlens_k[b] .. (int32 [B+1],
  * device); query head h reads KV head h / (Hq / Hkv); causal: row i sees keys
- * j <= i + (len_k - len_q). A row without keys is zero. D % 8 == 0, D <= 256.
+ * j <= i + (len_k - len_q). A row without keys is zero; rows of out past
+ * cu_seqlens_q[B] are not specified. Rows of other sequences never reach a
+ * sequence's output, whatever they hold; an infinity or NaN in v at a key that
+ * only the causal mask hides may reach rows up to 127 keys before it. q, k
+ * and v are 2-byte and out 16-byte aligned (the tensor-core kernel runs where
+ * bases and strides are multiples of 16 bytes and D <= 128). D % 8 == 0, D <= 256.
  * workspace: kq_fa_prompt_workspace() bytes of device memory, 16-byte
  * aligned, used by this call only until it has run. */
 size_t kq_fa_prompt_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int D);
@@ -383,11 +389,13 @@ kq_status_t kq_fa_prompt(int dtype, const void* q, const void* k, const void* v,
 /* Decode over the paged q8_0 cache, one query token per sequence: q and out
  * [B, Hq, D] contiguous, of dtype; seq_lens int32 [B] (device), 0 for a
  * padding row (its output is zero). The first prefix_len tokens are the same
- * pages for every sequence: they are read once for the whole batch, through
- * row 0 of block_tables; a sequence shorter than that sees its first
- * seq_lens[b] of them. max_seqlen bounds the lengths (it
- * sizes the work split; longer sequences are cut to it). Tokens in pages
- * outside the cache are hidden. D % 32 == 0, D <= 256. workspace as above. */
+ * pages for every sequence: they are read through row 0 of block_tables (once
+ * for the whole batch where that pays); a sequence shorter than that sees its
+ * first seq_lens[b] of them. max_seqlen bounds the lengths (it sizes the work
+ * split; longer sequences are cut to it). Tokens in pages outside the cache
+ * are hidden. Block scales d are up to 515 (values up to 65405, as fp16 rows
+ * hold): past that the fp16 operands overflow. q, out and the caches are
+ * 16-byte aligned. D % 32 == 0, D <= 256. workspace as above. */
 size_t kq_fa_decode_paged_workspace(int B, int Hq, int Hkv, int D, int prefix_len, int max_seqlen);
 kq_status_t kq_fa_decode_paged(int dtype, const void* q, const void* k_cache, const void* v_cache, int64_t num_pages,
                                int page_size, const int32_t* block_tables, int max_blocks, const int32_t* seq_lens,

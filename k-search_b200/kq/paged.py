@@ -201,7 +201,8 @@ def flash_prompt_ragged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_se
     head dimension has to be contiguous); cu_seqlens_q, cu_seqlens_k int32
     [B+1] on the device (cu_seqlens_k defaults to cu_seqlens_q). causal: row i
     of a sequence sees keys up to i + (len_k - len_q), so a chunk sees the
-    context before it; a row without keys is zero."""
+    context before it; a row without keys is zero, rows past cu_seqlens_q[B]
+    are not specified."""
     dt = _float16(q, "q")
     Tq, Hq, D = _rows(q, "q", q.dtype)
     dev = q.device
@@ -236,9 +237,10 @@ def flash_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     [B, Hq, D]. q fp16 or bf16 [B, Hq, D]; block_tables int32 [B, max_blocks];
     seq_lens int32 [B] (device; 0: a padding row, zeros out). The first
     prefix_len tokens are the same pages for every sequence: they are read
-    once for the whole batch, through row 0 of block_tables. max_seqlen (host)
-    bounds seq_lens, longer sequences are cut to it; it defaults to the
-    tables' width."""
+    through row 0 of block_tables, once for the whole batch where that pays.
+    max_seqlen (host) bounds seq_lens, longer sequences are cut to it; it
+    defaults to the tables' width, and a bound close to the true lengths gives
+    the better work split."""
     dt = _float16(q, "q")
     B, Hq, D = _rows(q, "q", q.dtype)
     dev = q.device
