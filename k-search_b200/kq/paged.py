@@ -38,16 +38,23 @@ def _tensor(t, name: str, dtype, device=None) -> torch.Tensor:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if device is not None and t.device != device:
+    if device is not None and t.get_device() != device.index:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
     return t
 
 
-def _vector(t, name: str, dtype, device, n: int) -> torch.Tensor:
+def _vector(t, name: str, dtype, device, n: int) -> None:
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device.index and t.numel() == n \
+            and t.dim() == 1 and t.is_contiguous():
+        return
     _tensor(t, name, dtype, device)
-    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous [{n}], got {list(t.shape)}")
-    return t
+    raise ValueError(f"{name} must be contiguous [{n}], got {list(t.shape)}")
+
+
+def _numel(t, name: str) -> int:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return t.numel()
 
 
 def _table(t, device, B: int | None) -> torch.Size:
@@ -79,11 +86,11 @@ def _caches(k_cache, v_cache, device) -> torch.Size:
     """[num_pages, page_size, Hkv, D/32, 34] of a checked cache pair."""
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         _tensor(t, name, torch.uint8, device)
-        shape = t.shape
-        if len(shape) != 5 or shape[4] != 34 or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous uint8 [num_pages, page_size, Hkv, D/32, 34], got {list(shape)}")
-    if k_cache.shape != shape:
-        raise ValueError(f"k_cache {list(k_cache.shape)} and v_cache {list(shape)} differ")
+        if t.dim() != 5 or t.size(4) != 34 or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous uint8 [num_pages, page_size, Hkv, D/32, 34], got {list(t.shape)}")
+    shape = k_cache.shape
+    if shape != v_cache.shape:
+        raise ValueError(f"k_cache {list(shape)} and v_cache {list(v_cache.shape)} differ")
     return shape
 
 
@@ -113,12 +120,11 @@ def page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
     map's length, sum(new_lens) where nothing pads it. counts[0] > F: the list
     was too short (the missing entries are -1); counts[1] > 0: that many new
     tokens got no slot. ``out``: an earlier plan whose tensors are reused."""
-    dev = _tensor(cached_lens, "cached_lens", torch.int32).device
-    B = cached_lens.numel()
+    B, F = _numel(cached_lens, "cached_lens"), _numel(free_pages, "free_pages")
+    dev = cached_lens.device
     _vector(cached_lens, "cached_lens", torch.int32, dev, B)
     _vector(new_lens, "new_lens", torch.int32, dev, B)
     W = _table(block_tables, dev, B)[1]
-    F = _tensor(free_pages, "free_pages", torch.int32, dev).numel()
     _vector(free_pages, "free_pages", torch.int32, dev, F)
     if out is None:
         slots = torch.empty(total_new, dtype=torch.int64, device=dev)
@@ -210,7 +216,7 @@ def flash_prompt_ragged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_se
     Tk, Hkv, Dk = kshape
     if _rows(v, "v", q.dtype, dev) != kshape or Dk != D:
         raise ValueError(f"k and v must be [Tk, Hkv, {D}], got {list(kshape)} and {list(v.shape)}")
-    B = _tensor(cu_seqlens_q, "cu_seqlens_q", torch.int32, dev).numel() - 1
+    B = _numel(cu_seqlens_q, "cu_seqlens_q") - 1
     _vector(cu_seqlens_q, "cu_seqlens_q", torch.int32, dev, max(B, 0) + 1)
     if cu_seqlens_k is not None:
         _vector(cu_seqlens_k, "cu_seqlens_k", torch.int32, dev, B + 1)
