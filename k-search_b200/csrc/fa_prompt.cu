@@ -720,10 +720,14 @@ Plan plan_of(const FaPromptArgs& a) {
   const int TQ = kTile / (a.Hq / a.Hkv);
   const long long keys = a.Tk / std::max(a.B, 1);  // per sequence, on average
   Plan p;
+  // two tiles per CTA where sequences are long (us for 8192 tokens of equal
+  // sequences, 32 heads over 8 of 128, one tile and two: 256 each 52 and 56, 768
+  // 75 and 80, 1024 95 and 96, 2048 158 and 152, 8192 521 and 480)
   p.tiles = keys >= 1024 ? 2 : 1;
   p.slots = a.Tq / (TQ * p.tiles) + a.B;
   // few CTAs against many keys: split the keys so that the SMs are full once,
-  // with at least 512 keys each
+  // with at least 512 keys each (256 rows against 24000 keys: 110 us in 4 parts,
+  // which leave 20 SMs idle; 109 in 9, 121 in 13)
   const long long ctas = ((a.Tq + (long long)TQ * p.tiles - 1) / (TQ * p.tiles)) * a.Hkv;
   const long long room = (long long)sm_count() * (p.tiles == 2 ? 1 : 2);
   p.splits = (int)std::max(1ll, std::min({room / std::max(ctas, 1ll), keys / 512, (long long)kMaxSplits}));
