@@ -94,12 +94,12 @@ def _caches(k_cache, v_cache, device) -> torch.Size:
     return shape
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _call(entry: str, device: torch.device, *args) -> None:
     """entry(*args, current stream of `device`) with that device current."""
-    before = torch.cuda.current_device()
+    before = _current_device()
     if device.index == before:
         status = getattr(lib(), entry)(*args, _raw_stream(before))
     else:
@@ -127,9 +127,9 @@ def page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
     W = _table(block_tables, dev, B)[1]
     _vector(free_pages, "free_pages", torch.int32, dev, F)
     if out is None:
-        slots = torch.empty(total_new, dtype=torch.int64, device=dev)
-        ints = torch.empty(3 * B + 4, dtype=torch.int32, device=dev)
-        seq_lens, cu_new, cu_seqlens, counts = ints.split_with_sizes((B, B + 1, B + 1, 2))
+        slots = cached_lens.new_empty(total_new, dtype=torch.int64)
+        seq_lens, cu_new, cu_seqlens, counts = torch.split_with_sizes(cached_lens.new_empty(3 * B + 4),
+                                                                      (B, B + 1, B + 1, 2))
         out = PagePlan(slots, seq_lens, cu_new, cu_seqlens, counts)
     else:
         slots, seq_lens, cu_new, cu_seqlens, counts = out
@@ -174,7 +174,7 @@ def page_read(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.
     pages, ps, hkv, nb, _ = _caches(k_cache, v_cache, dev)
     B, W = _table(block_tables, dev, None)
     _vector(cu_seqlens, "cu_seqlens", torch.int32, dev, B + 1)
-    k = torch.empty((total_rows, hkv, nb * 32), dtype=dtype, device=dev)
+    k = k_cache.new_empty((total_rows, hkv, nb * 32), dtype=dtype)
     v = torch.empty_like(k)
     _call("kq_page_read_q8_0", dev, dt, k_cache.data_ptr(), v_cache.data_ptr(), pages, ps, hkv, nb * 32,
           block_tables.data_ptr(), W, cu_seqlens.data_ptr(), B, total_rows, k.data_ptr(), v.data_ptr())
@@ -183,19 +183,19 @@ def page_read(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.
 
 def _out_like(q: torch.Tensor, out) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     _tensor(out, "out", q.dtype, q.device)
     if out.shape != q.shape or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {list(q.shape)}, got {list(out.shape)}")
     return out
 
 
-def _workspace(nbytes: int, device) -> tuple[torch.Tensor | None, int]:
+def _workspace(nbytes: int, like: torch.Tensor) -> tuple[torch.Tensor | None, int]:
     """Scratch from torch's caching allocator: ordered on the current stream, so
     calls on different streams never share it."""
     if nbytes == 0:
         return None, 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    ws = like.new_empty(nbytes, dtype=torch.uint8)
     return ws, ws.data_ptr()
 
 
@@ -228,7 +228,7 @@ def flash_prompt_ragged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_se
         scale = D ** -0.5
     out = _out_like(q, out)
     nbytes = lib().kq_fa_prompt_workspace(B, Tq, Tk, Hq, Hkv, D)
-    ws, ptr = _workspace(nbytes, dev)
+    ws, ptr = _workspace(nbytes, q)
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     _call("kq_fa_prompt", dev, dt, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
           cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), B, Tq, Tk, Hq, Hkv, D, int(causal), scale, out.data_ptr(),
@@ -262,7 +262,7 @@ def flash_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
         scale = D ** -0.5
     out = _out_like(q, out)
     nbytes = lib().kq_fa_decode_paged_workspace(B, Hq, hkv, D, prefix_len, max_seqlen)
-    ws, ptr = _workspace(nbytes, dev)
+    ws, ptr = _workspace(nbytes, q)
     _call("kq_fa_decode_paged", dev, dt, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages, ps,
           block_tables.data_ptr(), W, seq_lens.data_ptr(), B, Hq, hkv, D, prefix_len, max_seqlen, scale, out.data_ptr(),
           ptr, nbytes)
