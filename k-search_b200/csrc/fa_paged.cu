@@ -44,7 +44,8 @@ struct Split {
     const int n = len(b);
     return n > start ? (n - first() + kUnit - 1) / kUnit : 0;
   }
-  // C for U units: at least kMinUnits each
+  // C for U units: at least kMinUnits each (one sequence of up to 800 tokens: 8.9
+  // us with 2, 11.0 with 3, 12.2 with 4; 1 changes nothing)
   __device__ __forceinline__ int active(int U) const { return max(1, min(workers, U / kMinUnits)); }
   static constexpr int kMinUnits = 2;
 };
@@ -1102,13 +1103,13 @@ __global__ void __launch_bounds__(kCta, kCombineCtas) fa_paged_combine_kernel(co
       }
     }
     if (WR > 1) {
-      __syncthreads();  // the last row's sums are read
+      named_bar_sync(1 + warp / WR, WR * 32);  // the last row's sums are read
       if (w > 0) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) s_o[WR > 1 ? warp : 0][i * 32 + lane] = o[i];
         if (lane == 0) s_ml[warp] = make_float2(M, L);
       }
-      __syncthreads();
+      named_bar_sync(1 + warp / WR, WR * 32);
       if (w > 0) continue;
       float top = M;
 #pragma unroll
@@ -1305,14 +1306,23 @@ kq_status_t launch_stream_nb(const StreamArgs& a, bool pdl, cudaStream_t s) {
   return a.G > 8 ? launch_stream<NB, true, kStreamWarps>(a, pdl, s) : launch_stream<NB, false, kStreamWarps>(a, pdl, s);
 }
 
-// Eight warps per row while that leaves the SMs room, else one.
+// As many warps per row as still take all rows at once, else one (us of whole
+// calls: 32 rows of 62 states 10.3 with eight, 18.5 with one; 2048 rows of 26
+// states 59.6 with eight, 52.7 with four, 51.4 with two, 53.8 with one; 7168
+// rows of 8 states 62.2 with two, 57.8 with one).
+template <typename T, int VEC, int WR>
+kq_status_t launch_combine_wr(const CombineArgs& a, long long rows, long long most, cudaStream_t s) {
+  constexpr int per = kCta / 32 / WR;
+  return launch_after(fa_paged_combine_kernel<T, WR, VEC>, (int)std::min(most, (rows + per - 1) / per), kCta, 0, true, s, a,
+                      "fa_paged_combine");
+}
 template <typename T, int VEC>
 kq_status_t launch_combine(const CombineArgs& a, cudaStream_t s) {
   const long long rows = (long long)a.split.B * a.Hq, most = (long long)sm_count() * kCombineCtas;
-  if (rows <= most)
-    return launch_after(fa_paged_combine_kernel<T, 8, VEC>, (int)rows, kCta, 0, true, s, a, "fa_paged_combine");
-  return launch_after(fa_paged_combine_kernel<T, 1, VEC>, (int)std::min(most, (rows + 7) / 8), kCta, 0, true, s, a,
-                      "fa_paged_combine");
+  if (rows <= most) return launch_combine_wr<T, VEC, 8>(a, rows, most, s);
+  if (rows <= 2 * most) return launch_combine_wr<T, VEC, 4>(a, rows, most, s);
+  if (rows <= 4 * most) return launch_combine_wr<T, VEC, 2>(a, rows, most, s);
+  return launch_combine_wr<T, VEC, 1>(a, rows, most, s);
 }
 template <typename T>
 kq_status_t launch_combine_d(const CombineArgs& a, cudaStream_t s) {

@@ -374,6 +374,8 @@ DECODES = [
     ([640 + 3 * i for i in range(40)], 640, 16, 32, 8, 128), ([330] * 299 + [7], 320, 16, 4, 2, 32),
     ([2048 + 40 * i for i in range(14)], 2048, 128, 28, 4, 64), ([1030] * 100 + [500, 0], 1024, 32, 8, 1, 96),
     ([700 + i for i in range(30)], 699, 24, 15, 5, 64), ([129, 200], 127, 16, 4, 4, 32),
+    # rows for every number of warps that merge a row, odd counts among them
+    ([90 + i for i in range(53)], 0, 16, 15, 5, 64), ([200] * 111, 0, 16, 15, 3, 128), ([70 + i for i in range(127)], 48, 16, 21, 7, 160),
 ]
 
 
