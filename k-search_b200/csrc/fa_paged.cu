@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
 // times coarser) the high part alone is used; the queries become fp16 after
 // an exact power of two per row. d above 515 overflows the high part.
 //
-// 8192 tokens for 64 x 32 heads over 8 (144 CTAs of 7 blocks) take 22 us, 4 of
+// 8192 tokens for 64 x 32 heads over 8 (128 CTAs of 8 blocks) take 22 us, 4 of
 // them the set-up to the first scores, 3 the last stores; a block takes 3900
 // clocks (2700 without the low parts): the chain S -> P -> P V and next S of a
 // tile, of which the products are 1130 (560). Steps of 32 keys with the scores
@@ -1236,7 +1236,9 @@ bool use_prefix(const FaPagedArgs& a) {
   const long long again = (long long)(a.B - 1) * a.prefix_len * a.Hkv;
   return a.prefix_len % 8 || again >= (long long)kPrefixUnits * kUnit * sm_count();
 }
-// Token chunks of the prefix, so that the grid fills the SMs once.
+// Token chunks of the prefix, so that the grid fills the SMs once, and no more
+// of them than the longest one needs (128 blocks over 8 KV heads: 16 chunks of 8
+// instead of 18 of 7 or 8, which are two more states per row to merge).
 int prefix_groups(const FaPagedArgs& a) {  // (KV head, pair of row tiles)
   const long long rows = (long long)a.B * (a.Hq / a.Hkv);
   return (int)((rows + 2 * kTile - 1) / (2 * kTile)) * a.Hkv;
@@ -1244,7 +1246,8 @@ int prefix_groups(const FaPagedArgs& a) {  // (KV head, pair of row tiles)
 int prefix_chunks(const FaPagedArgs& a) {
   if (!use_prefix(a)) return 0;
   const int blocks = (a.prefix_len + kBlk - 1) / kBlk;
-  return std::max(1, std::min(blocks, sm_count() / prefix_groups(a)));
+  const int most = std::max(1, std::min(blocks, sm_count() / prefix_groups(a))), longest = (blocks + most - 1) / most;
+  return (blocks + longest - 1) / longest;
 }
 struct Workspace {
   size_t part, ml, ppart, pml, total;  // offsets
