@@ -218,6 +218,13 @@ def test_page_offsets_past_32_bits(cuda):
             ref, spread, top = attend(q[0, h:h + 1].double(), values(kc[-1])[:, h // 2], values(vc[-1])[:, h // 2],
                                       torch.ones((1, ps), dtype=torch.bool, device=cuda), D ** -0.5)
             check_out(out[0, h:h + 1], ref, spread, top, torch.float16, f"head {h} prefix {prefix}")
+    # two sequences in the same page, whose shared tokens go through the prefix's pass
+    out = kq.flash_decode_paged(q.repeat(2, 1, 1), kc, vc, table.repeat(2, 1), ints([ps, ps]), prefix_len=ps - 3)
+    for h in range(16):
+        ref, spread, top = attend(q[0, h:h + 1].double(), values(kc[-1])[:, h // 2], values(vc[-1])[:, h // 2],
+                                  torch.ones((1, ps), dtype=torch.bool, device=cuda), D ** -0.5)
+        for b in range(2):
+            check_out(out[b, h:h + 1], ref, spread, top, torch.float16, f"sequence {b} head {h}")
 
 
 # ---------------------------------------------------------------- prompt attention
@@ -438,6 +445,19 @@ def test_decode_score_ranges(cuda, prefix, case):
         fits = ref.abs() < 6.5e4
         got, ref, spread = got[fits], ref[fits], spread[fits]
     check_out(got, ref, spread, top, torch.float16, case)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1.7])
+@pytest.mark.parametrize("prefix", [0, 131])
+def test_decode_scales(cuda, prefix, scale):
+    import kq
+    g = gen(17)
+    lens = [400, 0, 140, 90]
+    kc, vc, table = paged_case(g, lens, prefix, 16, 2, 128)
+    q = rows(g, len(lens), 8, 128, torch.float16, 0.3)
+    ref, spread, top = decode_ref(q, kc, vc, table, lens, scale)
+    got = kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix, scale=scale)
+    check_out(got, ref, spread, top, torch.float16)
 
 
 @pytest.mark.parametrize("prefix", [64, 61])
