@@ -213,12 +213,12 @@ struct WriteArgs {
 // round_half_even(x / d) as IEEE division gives it, without the division:
 // x * (1 / d) is within 2^-21 of x / d relatively, under 1e-4 for |x / d| <=
 // 128, so the two round to different integers only that close to a half; only
-// there (one value in 5000) the division runs.
-__device__ __forceinline__ int code_of(float x, float d, float inv) {
-  const float q = x * inv;
-  const float r = rintf(q);
-  if (!(fabsf(q - r) < 0.4999f)) return max(-128, min(127, __float2int_rn(__fdiv_rn(x, d))));
-  return (int)r;
+// there (one value in 5000) the division runs. Adding 1.5 * 2^23 rounds to an
+// integer, whose low byte is the code.
+__device__ __forceinline__ uint32_t code_of(float x, float d, float inv) {
+  const float q = x * inv, t = q + 12582912.0f;
+  if (!(fabsf(q - (t - 12582912.0f)) < 0.4999f)) return (uint32_t)max(-128, min(127, __float2int_rn(__fdiv_rn(x, d)))) & 0xffu;
+  return __float_as_uint(t) & 0xffu;
 }
 
 // The q8_0 quantiser of quantize_rows (amax / 127, IEEE division, round half
@@ -227,10 +227,12 @@ __device__ __forceinline__ int code_of(float x, float d, float inv) {
 // The bytes go through shared memory, laid out as far from a 16-byte boundary
 // as their place in the cache is, so that they leave in whole 16-byte pieces:
 // blocks of 34 bytes stored code by code leave half-written sectors behind,
-// which made 4096 rows of 8 x 128 (26 MB in and out) take 24 us instead of 16.
-// Bound by the quantiser's arithmetic and the loads' latency; shorter segments
-// shorten single rows (11.6 -> 8.9 us with a read) but cost 10 us there.
+// which made 4096 rows of 8 x 128 (26 MB in and out) take 24 us instead of 16;
+// 13.8 with one division per block and no conversions. Bound by the quantiser's
+// arithmetic and the loads' latency; segments of 16 blocks gain 1 us on single
+// rows and lose 10 there.
 constexpr int kSegBlocks = 32;
+static_assert(kSegBlocks == 32, "a lane divides out the scale of one block of the segment");
 constexpr int kSegRoom = (kSegBlocks * kQ8 + 16 + 15) / 16 * 16;
 
 template <typename T>
@@ -263,18 +265,26 @@ __global__ void __launch_bounds__(256) page_write_kernel(const WriteArgs a) {
     uint8_t* dst = (which ? a.cache[1] : a.cache[0]) + (keep ? (slot * per_row + b0) * kQ8 : 0);
     const int off = (int)(reinterpret_cast<uintptr_t>(dst) & 15);
     __syncwarp();
+    // every block's maximum in its 8 lanes; lane `sub` of them then takes block
+    // 4 sub + lane / 8, so that each scale is divided out once, not by 8 lanes
+    float mine = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSegBlocks / 4; ++i) {
+      const float2 f0 = to_float2<T>(raw[i].x), f1 = to_float2<T>(raw[i].y);
+      float amax = fmaxf(fmaxf(fabsf(f0.x), fabsf(f0.y)), fmaxf(fabsf(f1.x), fabsf(f1.y)));
+#pragma unroll
+      for (int o = 1; o <= 4; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(full, amax, o));
+      if (sub == i) mine = amax;
+    }
+    const float my_d = mine > 0.0f ? __fdiv_rn(mine, 127.0f) : 1.0f, my_inv = 1.0f / my_d;
 #pragma unroll
     for (int i = 0; i < kSegBlocks / 4; ++i) {
       const float2 f0 = to_float2<T>(raw[i].x), f1 = to_float2<T>(raw[i].y);
       const float v[4] = {f0.x, f0.y, f1.x, f1.y};
-      float amax = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-#pragma unroll
-      for (int o = 1; o <= 4; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(full, amax, o));
-      const float d = amax > 0.0f ? __fdiv_rn(amax, 127.0f) : 1.0f;
-      const float inv = 1.0f / d;
+      const float d = __shfl_sync(full, my_d, (lane & 24) | i), inv = __shfl_sync(full, my_inv, (lane & 24) | i);
       uint32_t code = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) code |= (uint32_t)(code_of(v[k], d, inv) & 0xff) << (8 * k);
+      for (int k = 0; k < 4; ++k) code |= code_of(v[k], d, inv) << (8 * k);
       const int blk = 4 * i + (lane >> 3);
       if (blk < blocks) {
         uint16_t* o = reinterpret_cast<uint16_t*>(s_seg[warp] + off + blk * kQ8);
@@ -329,7 +339,8 @@ struct ReadArgs {
 // page id is outside the cache, and a row that no sequence owns, is zero.
 // Bound by memory, 34 bytes in and 64 out per block. More units per warp put
 // more loads in flight but leave fewer warps: 22445 rows of 8 x 128 after 4096
-// written take 50.7 us with 1, 46.0 with 2, 51.4 with 4 (both calls).
+// written take 50.7 us with 1, 46.0 with 2, 51.4 with 4 (both calls; 43.5 since the
+// write is faster).
 constexpr int kReadUnits = 2;
 constexpr int kUnitPieces = (kSegRoom / 16 + 31) / 32;  // of a unit, per lane
 
