@@ -342,8 +342,10 @@ kq_status_t kq_fa_decode_q8_0_ragged(const void* q_f16, const void* k, const voi
  * [B+1], prefix sums of new_lens and seq_lens; counts int32 [2]: pages the
  * step needs (more than num_free: the list was too short) and new tokens that
  * got no slot. Lengths sum to less than 2^31. A shared prefix is whole pages
- * already in the tables and counted in cached_lens. No device value is read
- * back. */
+ * already in the tables and counted in cached_lens. seq_lens may be
+ * cached_lens or new_lens itself (lengths updated in place); any other overlap
+ * of an output with an input or another output is refused. No device value is
+ * read back. */
 kq_status_t kq_page_plan(const int32_t* cached_lens, const int32_t* new_lens, int B, int32_t* block_tables,
                          int max_blocks, const int32_t* free_pages, int num_free, int page_size, int64_t total_new,
                          int64_t* slots, int32_t* seq_lens, int32_t* cu_new, int32_t* cu_seqlens, int32_t* counts,

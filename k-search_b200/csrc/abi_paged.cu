@@ -19,6 +19,15 @@ kq_status_t check_cache_shape(int Hkv, int D, const char* what) {
   return KQ_OK;
 }
 
+struct Span {
+  const void* p;
+  size_t bytes;
+};
+bool overlap(const Span& a, const Span& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return a.bytes > 0 && b.bytes > 0 && x < y + b.bytes && y < x + a.bytes;
+}
+
 FaPromptArgs prompt_args(int B, int Tq, int Tk, int Hq, int Hkv, int D) {
   FaPromptArgs a{};
   a.B = B, a.Tq = Tq, a.Tk = Tk, a.Hq = Hq, a.Hkv = Hkv, a.D = D;
@@ -54,6 +63,19 @@ kq_status_t kq_page_plan(const int32_t* cached_lens, const int32_t* new_lens, in
   if (!cu_new || !cu_seqlens || !counts || (total_new > 0 && !slots) || (num_free > 0 && !free_pages) ||
       (B > 0 && (!cached_lens || !new_lens || !seq_lens || (max_blocks > 0 && !block_tables))))
     return fail(KQ_ERR_INVALID, "page_plan: null pointer");
+  // the kernel's CTAs read the inputs while others already write: no output may
+  // lie on them, or on another output, but seq_lens exactly on the lengths it updates
+  const size_t w = sizeof(int32_t);
+  const Span in[3] = {{cached_lens, B * w}, {new_lens, B * w}, {free_pages, num_free * w}};
+  const Span out[6] = {{seq_lens, B * w},        {block_tables, (size_t)B * max_blocks * w}, {slots, total_new * sizeof(int64_t)},
+                       {cu_new, (B + (size_t)1) * w}, {cu_seqlens, (B + (size_t)1) * w},          {counts, 2 * w}};
+  for (int o = 0; o < 6; ++o) {
+    for (int i = 0; i < 3; ++i)
+      if (overlap(out[o], in[i]) && !(o == 0 && i < 2 && out[o].p == in[i].p))
+        return fail(KQ_ERR_INVALID, "page_plan: an output overlaps an input (only seq_lens may be cached_lens or new_lens)");
+    for (int i = 0; i < o; ++i)
+      if (overlap(out[o], out[i])) return fail(KQ_ERR_INVALID, "page_plan: two outputs overlap");
+  }
   return launch_page_plan(cached_lens, new_lens, B, block_tables, max_blocks, free_pages, num_free, page_size,
                           total_new, slots, seq_lens, cu_new, cu_seqlens, counts, static_cast<cudaStream_t>(stream));
 }

@@ -44,7 +44,7 @@ struct PlanArgs {
   int ps;
   long long T;
   long long* slots;
-  int32_t* seq_lens;
+  int32_t* seq_lens;  // null: written by plan_lens_kernel
   int32_t* cu_new;
   int32_t* cu_seqlens;
   int32_t* counts;
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kPlan) page_plan_kernel(const PlanArgs a) {
     s_take_end[tid] = sums[1];
     long long placed = 0;
     if (lead && b < a.B) {
-      a.seq_lens[b] = c + n;
+      if (a.seq_lens) a.seq_lens[b] = c + n;
       a.cu_new[b + 1] = base_new + sums[0];
       a.cu_seqlens[b + 1] = base_len + sums[2];
       // positions with a slot: up to the table's end, the free list's end and
@@ -187,6 +187,13 @@ __global__ void __launch_bounds__(kPlan) page_plan_kernel(const PlanArgs a) {
     a.counts[0] = base_take;
     a.counts[1] = (int)(base_new - (long long)s_placed);
   }
+}
+
+// Lengths updated in place by a plan of several CTAs, each of which reads all of
+// them: only once that launch has ended.
+__global__ void __launch_bounds__(256) plan_lens_kernel(const int32_t* cached, const int32_t* fresh, int B, int32_t* seq_lens) {
+  for (int b = blockIdx.x * 256 + threadIdx.x; b < B; b += gridDim.x * 256)
+    seq_lens[b] = max(0, cached[b]) + max(0, fresh[b]);
 }
 
 // ---- page write ----------------------------------------------------------------
@@ -430,9 +437,15 @@ int grid_for(long long items, int per_cta, int per_sm) {
 kq_status_t launch_page_plan(const int32_t* cached, const int32_t* fresh, int B, int32_t* table, int W,
                              const int32_t* free_pages, int F, int ps, int64_t T, int64_t* slots, int32_t* seq_lens,
                              int32_t* cu_new, int32_t* cu_seqlens, int32_t* counts, cudaStream_t s) {
-  PlanArgs a{cached, fresh, B, table, W, free_pages, F, ps, T, reinterpret_cast<long long*>(slots), seq_lens, cu_new,
-             cu_seqlens, counts};
-  page_plan_kernel<<<grid_for(T, kPlan, 1), kPlan, 0, s>>>(a);
+  const int grid = grid_for(T, kPlan, 1);
+  // in place, a single CTA reads a request's lengths before the same thread writes its sum
+  const bool later = grid > 1 && (seq_lens == cached || seq_lens == fresh);
+  PlanArgs a{cached, fresh, B, table, W, free_pages, F, ps, T, reinterpret_cast<long long*>(slots),
+             later ? nullptr : seq_lens, cu_new, cu_seqlens, counts};
+  page_plan_kernel<<<grid, kPlan, 0, s>>>(a);
+  if (kq_status_t st = check_launch("page_plan")) return st;
+  if (!later || B == 0) return KQ_OK;
+  plan_lens_kernel<<<grid_for(B, 256, 1), 256, 0, s>>>(cached, fresh, B, seq_lens);
   return check_launch("page_plan");
 }
 

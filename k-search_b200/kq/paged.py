@@ -119,7 +119,9 @@ def page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
     appended at column ceil(cached / page_size). total_new (host) is the slot
     map's length, sum(new_lens) where nothing pads it. counts[0] > F: the list
     was too short (the missing entries are -1); counts[1] > 0: that many new
-    tokens got no slot. ``out``: an earlier plan whose tensors are reused."""
+    tokens got no slot. ``out``: an earlier plan whose tensors are reused;
+    cached_lens may be its seq_lens, which then advance in place. Outputs that
+    overlap inputs in any other way are refused."""
     B, F = _numel(cached_lens, "cached_lens"), _numel(free_pages, "free_pages")
     dev = cached_lens.device
     _vector(cached_lens, "cached_lens", torch.int32, dev, B)

@@ -164,3 +164,29 @@ def test_paged_entry_points_refuse_before_any_cuda_call():
     assert L.kq_page_write_q8_0(0, None, None, 0, 0, 0, 0, None, 0, 2, 64, None, None, 0, None) == 0
     assert L.kq_page_read_q8_0(0, None, None, 1, 16, 2, 64, None, 1, None, 0, 5, None, None, None) == 1
     assert L.kq_page_read_q8_0(0, None, None, 1, 16, 2, 64, None, 1, None, 1, 0, None, None, None) == 0
+
+
+def test_page_plan_refuses_overlaps(libkq):
+    """Outputs on inputs or on each other are refused before anything is launched (addresses only: nothing is read)."""
+    from kq import _lib
+    L = _lib.lib()
+    B, W, F, T = 8, 4, 16, 1000
+    size = dict(cached=4 * B, new=4 * B, table=4 * B * W, free=4 * F, slots=8 * T, lens=4 * B, cu_new=4 * B + 4, cu_seq=4 * B + 4,
+                counts=8)
+    base = {n: 0x10000 * (i + 1) for i, n in enumerate(size)}
+
+    def plan(**moved):
+        p = {**base, **moved}
+        return L.kq_page_plan(p["cached"], p["new"], B, p["table"], W, p["free"], F, 16, T, p["slots"], p["lens"], p["cu_new"],
+                              p["cu_seq"], p["counts"], None)
+
+    outputs = ("table", "slots", "lens", "cu_new", "cu_seq", "counts")
+    for out in outputs:
+        for other in size:
+            if other == out:
+                continue
+            for at in (base[other] + size[other] - 4, base[other] - size[out] + 4, base[other]):
+                if out == "lens" and other in ("cached", "new") and at == base[other]:
+                    continue  # lengths updated in place
+                assert plan(**{out: at}) == 1, (out, other, hex(at))
+                assert "overlap" in _lib.last_error()
