@@ -336,7 +336,8 @@ kq_status_t kq_fa_decode_q8_0_ragged(const void* q_f16, const void* k, const voi
  * and tokens it adds now (negative counts as 0). Request b's new pages are
  * appended to its table row at column ceil(cached / page_size), taken from
  * free_pages int32 [num_free] in request order (-1 where the list is too
- * short). Outputs: slots int64 [total_new], one per new token in packed
+ * short; a negative entry, as of a padded list, is a page that is not there).
+ * Outputs: slots int64 [total_new], one per new token in packed
  * request order (-1 for a token without a page, past max_blocks, or past the
  * new tokens); seq_lens int32 [B] = cached + new; cu_new, cu_seqlens int32
  * [B+1], prefix sums of new_lens and seq_lens; counts int32 [2]: pages the

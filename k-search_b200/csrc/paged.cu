@@ -32,6 +32,7 @@ constexpr int kQ8 = 34;
 // by latency: 3.5 us for 8 requests of one token, 4.8 us for 256 prompts of
 // 65536 tokens together (16.5 with CTAs of 128 threads).
 constexpr int kPlan = 512;
+constexpr int kFreeAtOnce = 8;  // entries of the free list that a thread looks at side by side
 
 struct PlanArgs {
   const int32_t* cached;
@@ -161,6 +162,27 @@ __global__ void __launch_bounds__(kPlan) page_plan_kernel(const PlanArgs a) {
       const int at = i - (s_take_end[r] - s_take[r]);
       const int idx = base_take + i;
       a.table[(long long)(b0 + r) * a.W + s_have[r] + at] = idx < a.F ? a.free_pages[idx] : -1;
+    }
+    // new pages whose entry of the free list is negative (a list of fixed size,
+    // padded): their tokens got no slot either
+    if (lead) {
+      for (int i0 = tid; i0 < batch_take; i0 += kFreeAtOnce * kPlan) {
+        int page[kFreeAtOnce];
+#pragma unroll
+        for (int k = 0; k < kFreeAtOnce; ++k) {
+          const int i = i0 + k * kPlan;
+          page[k] = i < batch_take && base_take + i < a.F ? a.free_pages[base_take + i] : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < kFreeAtOnce; ++k) {
+          if (page[k] >= 0) continue;
+          const int i = i0 + k * kPlan, r = find_row(s_take_end, rows, i);
+          const long long first = ((long long)s_have[r] + i - (s_take_end[r] - s_take[r])) * a.ps;
+          const long long stop = s_cached[r] + min((long long)s_new[r], a.T - (base_new + s_new_end[r] - s_new[r]));
+          const long long lost = min(first + a.ps, stop) - first;
+          if (lost > 0) atomicAdd(&s_placed, (unsigned long long)-lost);
+        }
+      }
     }
     const long long end = min((long long)batch_new, a.T - base_new);
     for (long long i = (long long)blockIdx.x * kPlan + tid; i < end; i += step) {

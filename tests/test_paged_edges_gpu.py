@@ -41,3 +41,20 @@ def test_plan_updates_lengths_in_place(cuda, B, top, ps, W, extra, which):
         other = [rng.randint(0, top) for _ in range(B)]
         if which == "new":  # the sums are the next step's new tokens: start over behind nothing
             other = [0] * B
+
+
+@pytest.mark.parametrize("B,top,ps,W", [(1, 40, 16, 4), (7, 300, 16, 20), (40, 900, 32, 30), (600, 40, 16, 4)])
+def test_plan_counts_tokens_of_absent_free_pages(cuda, B, top, ps, W):
+    """A free list of fixed size whose unused entries are -1: the tokens of those pages count as not placed."""
+    import kq
+    rng = random.Random(B)
+    cached, new = [rng.randint(0, top) for _ in range(B)], [rng.randint(0, top) for _ in range(B)]
+    table = [[rng.randrange(1000) for _ in range(W)] for _ in range(B)]
+    need = sum(max(0, min(-(-(c + n) // ps), W) - min(-(-c // ps), W)) for c, n in zip(cached, new))
+    free = [1000 + i if rng.random() < 0.7 else -1 for i in range(need)] + [-1] * 5
+    for total in (sum(new), sum(new) * 2 // 3, sum(new) + 9):
+        tt = ints(table)
+        plan = kq.page_plan(ints(cached), ints(new), tt, ints(free), ps, total)
+        rt, rs, used, dropped = plan_ref(cached, new, table, free, ps, total)
+        assert tt.tolist() == rt and plan.slots.tolist() == rs
+        assert plan.counts.tolist() == [used, dropped]
