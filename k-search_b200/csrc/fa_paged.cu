@@ -622,6 +622,7 @@ constexpr int kTile = 128;
 constexpr int kPrefixThreads = 640;
 constexpr int kMmaWarp = 8, kDeqWarp = 9, kDeqWarps = 8;
 constexpr float kBias = 7.0f, kLazy = 8.0f;
+constexpr float kMinScale = 1e-30f;    // of a row, its power of two included: 0 would turn a hidden key's -inf into NaN
 constexpr int kRaw = 3, kOps = 2;      // blocks of raw rows and of operands in flight (K and V each)
 constexpr int kMasks = 16;             // blocks whose row masks are kept (more than are in flight)
 
@@ -913,7 +914,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
             top = max3(top, fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u)));
           const int e = min(max((int)(__float_as_uint(top) >> 23) - 127 - 14, -100), 100);
           const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-          sl *= __uint_as_float((uint32_t)(127 + e) << 23);
+          sl = fmaxf(sl * __uint_as_float((uint32_t)(127 + e) << 23), kMinScale);
 #pragma unroll
           for (int i = 0; i < DP / 2; ++i)
             w[i] = pack2<__half>(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down);
@@ -1374,7 +1375,7 @@ kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s) {
     x.prefix_len = a.prefix_len, x.limit = p.split.limit, x.chunks = chunks;
     x.table = a.table, x.seq_lens = a.seq_lens;
     x.flip = p.sl < 0.0f ? 0x80000000u : 0u;
-    x.sl = fmaxf(fabsf(p.sl), 1e-30f);  // a scale of 0 keeps -inf for hidden keys
+    x.sl = fmaxf(fabsf(p.sl), kMinScale);
     x.part = reinterpret_cast<float*>(ws + w.ppart), x.ml = reinterpret_cast<float2*>(ws + w.pml);
     x.err = device_error_word();
     const int pgrid = prefix_groups(a) * chunks;

@@ -6,7 +6,7 @@ import random
 import pytest
 import torch
 
-from test_paged_gpu import ints, plan_ref, prefix_sums
+from test_paged_gpu import check_out, decode_ref, gen, ints, paged_case, plan_ref, prefix_sums, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +58,22 @@ def test_plan_counts_tokens_of_absent_free_pages(cuda, B, top, ps, W):
         rt, rs, used, dropped = plan_ref(cached, new, table, free, ps, total)
         assert tt.tolist() == rt and plan.slots.tolist() == rs
         assert plan.counts.tolist() == [used, dropped]
+
+
+# ---------------------------------------------------------------- decode: scales and scores
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-38, -0.2])
+@pytest.mark.parametrize("prefix", [0, 125, 128])
+def test_decode_zero_queries(cuda, dtype, scale, prefix):
+    """Zero and tiny query rows with a scale of 0 beside ordinary ones: hidden tokens stay hidden."""
+    import kq
+    g = gen(31)
+    lens = [prefix + 60, 90, 0, prefix + 3]
+    kc, vc, table = paged_case(g, lens, prefix, 16, 2, 128)
+    q = rows(g, len(lens), 8, 128, dtype)
+    q[:, ::3] = 0
+    q[1:, 1] *= 2.0 ** -12
+    if dtype == torch.bfloat16:
+        q[0, 1] *= 2.0 ** -100
+    ref, spread, top = decode_ref(q, kc, vc, table, lens, scale)
+    check_out(kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix, scale=scale), ref, spread, top, dtype)
