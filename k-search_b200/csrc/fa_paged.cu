@@ -600,12 +600,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
 //   S = Q K^T (tcgen05, Q from TMEM), P = 2^(S sl - m + kBias) (a thread per
 //   row), O += P V (tcgen05, P from TMEM)
 // as in the prompt kernel (lazy maximum, two tiles alternating).
-// Operands are fp16. K = d * code has up to 19 significant bits: with fp16
-// queries it enters as an fp16 high part plus the exact remainder (two
-// products into the same accumulator), likewise V, so that P is the only
-// rounded factor. With bf16 queries and outputs (whose own rounding is 8
-// times coarser) the high part alone is used; the queries become fp16 after
-// an exact power of two per row. d above 515 overflows the high part.
+// Operands are fp16. K = d * code has up to 19 significant bits: it enters as
+// an fp16 high part plus the exact remainder (two products into the same
+// accumulator), so that the scores carry fp32's error only: an error of K grows
+// with the score and is exponentiated (scores of 100 from a rounded K put the
+// output 1 % off). V does the same for fp16 outputs (LO), where P then is the only
+// rounded factor; for bf16 outputs, whose own rounding is 8 times coarser, the
+// high part alone is used (with both, 256 samples behind 4096 tokens take 62.8 us instead of 61.5).
+// bf16 queries become fp16 after an exact power of two per row. d above 515
+// overflows the high part.
 //
 // 8192 tokens for 64 x 32 heads over 8 (128 CTAs of 8 blocks) take 22 us, 4 of
 // them the set-up to the first scores, 3 the last stores; a block takes 3900
@@ -626,15 +629,15 @@ constexpr float kMinScale = 1e-30f;    // of a row, its power of two included: 0
 constexpr int kRaw = 3, kOps = 2;      // blocks of raw rows and of operands in flight (K and V each)
 constexpr int kMasks = 16;             // blocks whose row masks are kept (more than are in flight)
 
-template <int NB, bool LO>
+template <int NB, bool LO>  // LO: V's low part too
 struct PrefixTraits {
   static constexpr int DP = NB <= 2 ? 64 : 128;
   static constexpr int PANELS = DP / 64;
   static constexpr int PANEL = kBlk * 128;
   static constexpr int PART = PANELS * PANEL;       // the high (or low) parts of a block
-  static constexpr int OP = PART * (LO ? 2 : 1);    // K or V of a block
+  static constexpr int OP_K = 2 * PART, OP = OP_K + PART * (LO ? 2 : 1);  // K of a block; K and V
   static constexpr int RAW = 2 * kBlk * Row<NB>::PITCH;  // raw rows of a block, K and V
-  static constexpr int OFF_RAW = kOps * 2 * OP;
+  static constexpr int OFF_RAW = kOps * OP;
   static constexpr int OFF_STAGE = OFF_RAW + kRaw * RAW;  // 4 KB per softmax warp
   static constexpr int OFF_BAR = OFF_STAGE + 8 * 4096;
   static constexpr int SMEM = OFF_BAR + 512 + 1024;
@@ -768,7 +771,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
       for (int x = 0; x < 8; ++x) w[x] = present ? src[x] : 0u;
       w[8] = !present ? 0u : sh ? src[8] : *reinterpret_cast<const uint16_t*>(src + 8);
     };
-    auto convert = [&](const uint32_t (&w)[9], uint8_t* op) {
+    auto convert = [&](const uint32_t (&w)[9], uint8_t* op, bool low) {
       const uint32_t d = (w[0] >> sh) & 0xffffu, d2 = d | d << 16;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -780,12 +783,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
 #pragma unroll
           for (int z = 0; z < 2; ++z) {
             hi[2 * y + z] = hmul2(c[z], d2);
-            if (LO) lo[2 * y + z] = hfma2(c[z], d2, hi[2 * y + z] ^ 0x80008000u);
+            if (low) lo[2 * y + z] = hfma2(c[z], d2, hi[2 * y + z] ^ 0x80008000u);
           }
         }
         uint8_t* o = op + tc::sw128_off(tok, (blk & 1) * 4 + x);
         *reinterpret_cast<uint4*>(o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (LO) *reinterpret_cast<uint4*>(o + R::PART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (low) *reinterpret_cast<uint4*>(o + R::PART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     };
     for (int j = 0; j < n; ++j) {
@@ -803,7 +806,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
         if (j >= kOps) mbar_wait_or_poison(&op_empty[2 * os + kv], ((j / kOps) - 1) & 1, a.err, DEV_TIMEOUT_EMPTY, dead);
-        if (used) convert(kv ? wv : wk, dst + (os * 2 + kv) * R::OP);
+        if (used) convert(kv ? wv : wk, dst + os * R::OP + kv * R::OP_K, LO || kv == 0);
         fence_proxy_async_smem();
         __syncwarp();  // also: the ring's rows are read
         if (lane == 0) mbar_arrive(&op_full[2 * os + kv]);
@@ -820,9 +823,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
     auto score = [&](int t, int j) {
       mbar_wait_or_poison(&op_full[2 * (j % kOps)], (j / kOps) & 1, a.err, DEV_TIMEOUT_FULL, dead);
       tc::tc_fence_after();
-      const uint64_t kd = tc::sw128_desc(base + j % kOps * 2 * R::OP);
+      const uint64_t kd = tc::sw128_desc(base + j % kOps * R::OP);
 #pragma unroll
-      for (int part = 0; part < (LO ? 2 : 1); ++part)
+      for (int part = 0; part < 2; ++part)
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
           tc::mma_ts_go(tmem + kColS + t * kBlk, tmem + kColQ + t * 64 + 8 * k,
@@ -842,7 +845,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
       release(0, 0);
     }
     for (int j = 0; j < n; ++j) {
-      const uint64_t vd = tc::sw128_desc_mn(base + (j % kOps * 2 + 1) * R::OP, R::PANEL);  // dims across, tokens down
+      const uint64_t vd = tc::sw128_desc_mn(base + j % kOps * R::OP + R::OP_K, R::PANEL);  // dims across, tokens down
 #pragma unroll 1
       for (int t = 0; t < tiles; ++t) {
         mbar_wait_or_poison(&op_full[2 * (j % kOps) + 1], (j / kOps) & 1, a.err, DEV_TIMEOUT_FULL, dead);

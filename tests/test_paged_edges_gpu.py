@@ -6,9 +6,13 @@ import random
 import pytest
 import torch
 
-from test_paged_gpu import check_out, decode_ref, gen, ints, paged_case, plan_ref, prefix_sums, rows
+from test_paged_gpu import U, check_out, decode_ref, gen, ints, paged_case, plan_ref, prefix_sums, rows
 
 pytestmark = pytest.mark.gpu
+
+
+def half_bytes(value):
+    return torch.tensor([value], dtype=torch.float16, device="cuda").view(torch.uint8)
 
 
 # ---------------------------------------------------------------- page_plan
@@ -77,3 +81,57 @@ def test_decode_zero_queries(cuda, dtype, scale, prefix):
         q[0, 1] *= 2.0 ** -100
     ref, spread, top = decode_ref(q, kc, vc, table, lens, scale)
     check_out(kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix, scale=scale), ref, spread, top, dtype)
+
+
+4
+def check_decode(got, ref, spread, top, dtype, what=""):
+    """Decode rounds a weight times its block scale to fp16 (and V's operand, of half the output's precision at
+    most, once more), scores stay in fp32, the output is rounded to the type: u |ref| + 3 2^-11 A + the scores' part."""
+    tol = U[dtype] * ref.abs() + 3 * 2.0 ** -11 * spread + 2e-5 * (4 + top) * spread + (2.0 ** -24 if dtype == torch.float16 else 0)
+    err = (got.double() - ref).abs()
+    assert torch.isfinite(got).all(), f"{what}: not finite"
+    assert (err <= tol).all(), f"{what}: {int((err > tol).sum())} of {err.numel()} off, worst {float((err / tol.clamp(min=1e-30)).max()):.2f} x bound"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("strength", [8.0, 16.0, 31.0])
+@pytest.mark.parametrize("prefix", [0, 2045])
+def test_decode_outlier_channel(cuda, dtype, strength, prefix):
+    """One large channel of Q and K, as projections have it: scores of 30 to 120 that differ by little."""
+    import kq
+    g = gen(41)
+    lens, ps, Hq, Hkv, D = [2100, 2300, 2045], 16, 8, 2, 128
+    kc, vc, table = paged_case(g, lens, prefix, ps, Hkv, D)
+    n = kc.shape[0] * ps
+    k = torch.randn((n, Hkv, D), generator=g, device="cuda")
+    k[..., 5] = 40.0 + 2.0 * torch.randn((n, Hkv), generator=g, device="cuda")
+    kq.page_write(k.to(dtype), k.to(dtype), torch.arange(n, device="cuda"), kc, kc.clone())
+    q = torch.randn((3, Hq, D), generator=g, device="cuda")
+    q[..., 5] = strength
+    q = q.to(dtype)
+    ref, spread, top = decode_ref(q, kc, vc, table, lens, D ** -0.5)
+    got = kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix)
+    check_decode(got, ref, spread, top, dtype)
+
+
+@pytest.mark.parametrize("prefix", [0, 128, 131])
+@pytest.mark.parametrize("case", ["growing", "huge", "equal"])
+def test_decode_score_ranges_bf16(cuda, prefix, case):
+    import kq
+    g = gen(43)
+    lens, ps, Hq, Hkv, D = [900, 300, 640], 16, 8, 2, 128
+    kc, vc, table = paged_case(g, lens, prefix, ps, Hkv, D)
+    q = rows(g, 3, Hq, D, torch.bfloat16)
+    if case == "growing":
+        q = q.abs()
+        kc[..., 2:] &= 127
+        for b, n in enumerate(lens):
+            for j in range(-(-n // ps)):
+                kc[table[b, j].item(), ..., :2] = half_bytes(0.0005 * (j + 1))
+    elif case == "huge":
+        q = (q.float() * 20).to(torch.bfloat16)
+    else:
+        q = torch.zeros_like(q)
+    ref, spread, top = decode_ref(q, kc, vc, table, lens, D ** -0.5)
+    got = kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix)
+    check_decode(got, ref, spread, top, torch.bfloat16, case)
