@@ -107,8 +107,11 @@ __device__ __forceinline__ int units_before(const Split& sp, const SplitScan<T>&
 //   S^T[t, h] = sum_j d_k(t, j) (codes_j . q_j): exact fp16 codes per 32-dim
 //     block j, rescaled in fp32, then transposed between the lanes;
 //   O^T[:, h] += sum_t codes (p d_v(t, j)): the value block's scale folded into
-//     p in fp32, rounded to fp16 once (the codes are exact), times 2^kPBits so
-//     that small scales stay in fp16's normal range. d_v up to 1023 fits.
+//     p in fp32, rounded to fp16 once (the codes are exact). Like the output's
+//     own rounding that is 2^-11 of each weight, and the weights' errors average
+//     out. p carries 2^e with e from the segment's largest d_v so far, so that p d_v
+//     stays below 2^15 for every fp16 d_v and the light weights of small values
+//     stay in fp16's normal range (down to 2^-29 of the largest possible p d_v).
 // With the heads as rows half of every product was empty: 16 conversations of
 // 16000 tokens (8 KV heads of 128) took 101 us instead of 89. The head dimension
 // is permuted inside a block so that every operand word is one 32-bit load (a
@@ -119,7 +122,7 @@ __device__ __forceinline__ int units_before(const Split& sp, const SplitScan<T>&
 // take 81 and 84 us there, but 1 and 2 us more where sequences are short.
 constexpr int kStreamWarps = 12;  // 12 warps with 3 stages, or 8 with 6 where there is little to stream
 constexpr int kFewWarps = 8;
-constexpr float kPBits = 6.0f, kPScale = 64.0f;
+constexpr float kMaxExp = 40.0f;   // e of a segment without a value scale so far (2^-24 alone needs 38)
 
 template <int NB>
 struct Row {
@@ -411,7 +414,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
       for (int r = 0; r < RH; ++r)
 #pragma unroll
         for (int x = 0; x < 4; ++x) acc[i][r][x] = 0.0f;
-    float m[RH], l[RH];
+    float m[RH], l[RH], e = kMaxExp;  // p is 2^(s - m + e)
 #pragma unroll
     for (int r = 0; r < RH; ++r) m[r] = -INFINITY, l[r] = 0.0f;
 
@@ -443,16 +446,22 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
       copy_wait<kSt - 1>();
       __syncwarp();
       const uint8_t* stage = ring + st * R::STAGE;
+      uint32_t top = 0;  // bits of the tile's largest |d_v|
       {
         // a row per lane: its scales in fp32. An absent row may hold anything:
         // its weight is 0, not 0 x scale
         const uint8_t* row = stage + at_s;
         const bool there = mask >> (lane & 15) & 1;
-        const float unit = lane < 16 ? 1.0f : kPScale;
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
-          s_scale[warp][lane >> 4][j][lane & 15] = there ? __half2float(*reinterpret_cast<const __half*>(row + j * kQ8)) * unit : 0.0f;
+        for (int j = 0; j < NB; ++j) {
+          const float d = there ? __half2float(*reinterpret_cast<const __half*>(row + j * kQ8)) : 0.0f;
+          s_scale[warp][lane >> 4][j][lane & 15] = d;
+          top = max(top, __float_as_uint(d) & 0x7fffffffu);
+        }
+        top = __reduce_max_sync(0xffffffffu, lane < 16 ? 0u : top);
       }
+      // 2^e d_v < 2^15; an infinity or NaN among the scales keeps e for the others
+      const float en = fminf(e, fmaxf(-1.0f, 141.0f - (float)(top >> 23)));
       __syncwarp();
       auto scales = [&](int kv, int j, int i) { return *reinterpret_cast<const float2*>(&s_scale[warp][kv][j][i]); };
 
@@ -501,7 +510,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
             if (!(mask >> (8 * t + 2 * c + (r & 1)) & 1u)) s[t][r] = -INFINITY;
       }
       float p[2][2 * RH], f_[RH];
-      bool moved = false;
+      bool moved = en != e;
 #pragma unroll
       for (int r = 0; r < RH; ++r) {
         float mx = m[r];
@@ -511,8 +520,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
           for (int x = 0; x < 2; ++x) mx = fmaxf(mx, s[t][2 * r + x]);
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float base = mx == -INFINITY ? 0.0f : mx;
-        f_[r] = ex2(m[r] - base);
+        const float base = mx == -INFINITY ? 0.0f : mx - en;
+        f_[r] = ex2((m[r] - e) - base);
         moved |= mx != m[r];
         m[r] = mx;
         float sum = 0.0f;
@@ -525,6 +534,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
           }
         l[r] = fmaf(l[r], f_[r], sum);
       }
+      e = en;
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int r = 0; r < RH; ++r) {
@@ -576,7 +586,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
       const int hl = qg * 16 + g + 8 * r;
       if (hl < a.G) {
         const long long row = seg * a.Hq + h * a.G + hl;
-        if (c == 0) a.ml[row] = make_float2(m[r] - kPBits, sum * kPScale);  // the sums carry 2^kPBits: as if m were lower
+        if (c == 0) a.ml[row] = make_float2(m[r] - e, sum);  // the sums carry 2^e: as if m were lower
       }
 #pragma unroll
       for (int x = 0; x < 2; ++x) {

@@ -135,3 +135,30 @@ def test_decode_score_ranges_bf16(cuda, prefix, case):
     ref, spread, top = decode_ref(q, kc, vc, table, lens, D ** -0.5)
     got = kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix)
     check_decode(got, ref, spread, top, torch.bfloat16, case)
+
+
+5
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,G,prefix", [(128, 4, 0), (128, 4, 61), (256, 2, 0), (96, 9, 0), (32, 16, 0)])
+@pytest.mark.parametrize("d,gap", [(5e-4, 12.0), (2e-3, 11.0), (3e-2, 10.0), (1e-6, 3.0), (6e-8, 0.0), (1e-6, -1.0)])
+def test_decode_small_value_scales(cuda, dtype, D, G, prefix, d, gap):
+    """Small values behind one token that takes nearly all the weight and whose value is zero; the others share
+    one score and one scale, so that a weight's rounding error would not average out. gap -1: random scores."""
+    import kq
+    g = gen(51)
+    lens, ps, Hkv = [900, 333], 16, 2
+    kc, vc, table = paged_case(g, lens, prefix, ps, Hkv, D)
+    q = torch.ones((2, G * Hkv, D), dtype=dtype, device=cuda)
+    vc[..., :2] = half_bytes(d)
+    if gap >= 0:
+        kc[..., 2:] = 0
+        for b in range(2):
+            first = kc[table[b, 0].item(), 0]
+            first[..., 2:] = 100
+            first[..., :2] = half_bytes(gap / (D ** 0.5 * 100))
+            vc[table[b, 0].item(), 0, ..., 2:] = 0
+    else:
+        q = rows(g, 2, G * Hkv, D, dtype)
+    ref, spread, top = decode_ref(q, kc, vc, table, lens, D ** -0.5)
+    got = kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix)
+    check_decode(got, ref, spread, top, dtype)
