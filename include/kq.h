@@ -396,9 +396,9 @@ kq_status_t kq_fa_prompt(int dtype, const void* q, const void* k, const void* v,
  * for the whole batch where that pays); a sequence shorter than that sees its
  * first seq_lens[b] of them. max_seqlen bounds the lengths (it sizes the work
  * split; longer sequences are cut to it). Tokens in pages outside the cache
- * are hidden. Block scales d are up to 515 (values up to 65405, as fp16 rows
- * hold): past that the fp16 operands overflow. q, out and the caches are
- * 16-byte aligned. D % 32 == 0, D <= 256. workspace as above. */
+ * are hidden, whatever they hold. Block scales are any fp16 numbers (one of
+ * 512 or more, an infinity or a NaN in a shared prefix sends the rows around it
+ * down a slow path). q, out and the caches are 16-byte aligned. D % 32 == 0, D <= 256. workspace as above. */
 size_t kq_fa_decode_paged_workspace(int B, int Hq, int Hkv, int D, int prefix_len, int max_seqlen);
 kq_status_t kq_fa_decode_paged(int dtype, const void* q, const void* k_cache, const void* v_cache, int64_t num_pages,
                                int page_size, const int32_t* block_tables, int max_blocks, const int32_t* seq_lens,

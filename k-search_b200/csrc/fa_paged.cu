@@ -603,6 +603,77 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
   pdl_wait();
 }
 
+// ---- one row in fp32 on scalar instructions ----------------------------------------------
+// 32 tokens per step: a lane per token for q . k, then a lane per dimension for
+// p . v. For the pages and rows that the other kernels do not take.
+struct Tokens {
+  const uint8_t *k, *v;
+  const int32_t *shared, *own;  // pages of tokens below prefix_len, and of the others
+  long long num_pages, row_bytes, head_off;
+  int ps, prefix_len;
+};
+// The softmax state (natural units) of tokens j0 .. j1 - 1 for the scaled query
+// s_q; s_p and s_row hold 32 values each. A warp together. U: how far the loops
+// are unrolled, 1 where the code should be short.
+template <int U, int NB>
+__device__ __forceinline__ void attend_tokens(const Tokens& a, int nb, int j0, int j1, const float* s_q, float* s_p,
+                                              long long* s_row, float& m, float& l, float (&acc)[NB]) {
+  const unsigned full = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int t = 0; t < NB; ++t) acc[t] = 0.0f;
+  for (; j0 < j1; j0 += 32) {
+    const int j = j0 + lane;
+    float s = -INFINITY;
+    long long off = -1;
+    if (j < j1) {
+      const long long page = (j < a.prefix_len ? a.shared : a.own)[j / a.ps];
+      if (page >= 0 && page < a.num_pages) {
+        off = (page * a.ps + j % a.ps) * a.row_bytes + a.head_off;
+        const uint8_t* k = a.k + off;
+        s = 0.0f;
+#pragma unroll 1
+        for (int t = 0; t < nb; ++t) {
+          const float d = half_bits_to_float(*reinterpret_cast<const uint16_t*>(k + t * kQ8));
+          float dot = 0.0f;
+#pragma unroll U
+          for (int e = 0; e < 32; ++e) dot = fmaf(s_q[t * 32 + e], (float)(int8_t)k[t * kQ8 + 2 + e], dot);
+          s = fmaf(d, dot, s);
+        }
+      }
+    }
+    const float mn = fmaxf(m, warp_max(s));
+    const float base = mn == -INFINITY ? 0.0f : mn;
+    const float p = off < 0 ? 0.0f : __expf(s - base);
+    const float c = __expf(m - base);
+    float ps = p;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) ps += __shfl_xor_sync(full, ps, o);
+    l = l * c + ps;
+    m = mn;
+    s_p[lane] = p;
+    s_row[lane] = off;
+    __syncwarp();
+#pragma unroll
+    for (int t = 0; t < NB; ++t) acc[t] *= c;
+    const int n = min(32, j1 - j0);
+#pragma unroll (U > 4 ? 4 : U)
+    for (int jj = 0; jj < n; ++jj) {
+      if (s_row[jj] < 0) continue;
+      const float pj = s_p[jj];
+      const uint8_t* v = a.v + s_row[jj];
+#pragma unroll
+      for (int t = 0; t < NB; ++t)
+        if (t < nb) {
+          const float d = half_bits_to_float(*reinterpret_cast<const uint16_t*>(v + t * kQ8));
+          acc[t] = fmaf(pj * d, (float)(int8_t)v[t * kQ8 + 2 + lane], acc[t]);
+        }
+    }
+    __syncwarp();
+  }
+}
+
 // ---- shared prefix: one pass of the tensor cores over it for the whole batch -----------
 // The B * G query heads of a KV head are the rows of 128-row tiles; a CTA
 // takes two tiles and a range of 64-token blocks of the prefix, so each block
@@ -617,8 +688,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) fa_paged_stream_kernel(const St
 // output 1 % off). V does the same for fp16 outputs (LO), where P then is the only
 // rounded factor; for bf16 outputs, whose own rounding is 8 times coarser, the
 // high part alone is used (with both, 256 samples behind 4096 tokens take 62.8 us instead of 61.5).
-// bf16 queries become fp16 after an exact power of two per row. d above 515
-// overflows the high part.
+// bf16 queries become fp16 after an exact power of two per row.
+// d of 512 and more (values past fp16's largest number) overflows the high part,
+// and a token that a row does not see enters P V with weight 0, which an infinite
+// or NaN scale turns into NaN. Where a CTA meets such a scale, its rows are done
+// again in fp32, each from its own tokens, by the warps that dequantise (which
+// have nothing else to do by then). Watching the scales and that code cost every
+// call 0.3 (bf16) to 1 us (fp16); a look at the sums and the code in the combine
+// cost 1 to 2.
 //
 // 8192 tokens for 64 x 32 heads over 8 (128 CTAs of 8 blocks) take 22 us, 4 of
 // them the set-up to the first scores, 3 the last stores; a block takes 3900
@@ -650,6 +727,7 @@ struct PrefixTraits {
   static constexpr int OFF_RAW = kOps * OP;
   static constexpr int OFF_STAGE = OFF_RAW + kRaw * RAW;  // 4 KB per softmax warp
   static constexpr int OFF_BAR = OFF_STAGE + 8 * 4096;
+  static constexpr int OFF_BIG = OFF_BAR + 508;
   static constexpr int SMEM = OFF_BAR + 512 + 1024;
   static_assert(SMEM <= 232448, "shared memory budget");
   static_assert(OFF_RAW % 1024 == 0 && OFF_BAR % 16 == 0, "alignment");
@@ -663,7 +741,7 @@ struct PrefixArgs {
   long long num_pages;
   int ps, B, Hq, Hkv, G, prefix_len, limit, chunks;
   const int32_t *table, *seq_lens;  // the table's row 0
-  float sl;
+  float scale, sl;
   uint32_t flip;
   float* part;  // [chunk][B * Hq][NB * 32]
   float2* ml;
@@ -684,6 +762,50 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
 __host__ __device__ constexpr uint32_t idesc_h(int n, bool b_mn) {
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
+// What a CTA of the prefix kernel works on.
+struct PrefixJob {
+  int chunk, h, row0, j0, n;  // chunk, KV head, first of its rows, its first block and blocks
+  __device__ __forceinline__ PrefixJob(const PrefixArgs& a, int cta) {
+    const int hp = cta / a.chunks, blocks = (a.prefix_len + kBlk - 1) / kBlk;
+    chunk = cta % a.chunks, h = hp % a.Hkv, row0 = hp / a.Hkv * 2 * kTile;
+    j0 = (int)((long long)blocks * chunk / a.chunks), n = (int)((long long)blocks * (chunk + 1) / a.chunks) - j0;
+  }
+};
+// Where the CTA met a scale past the operands' range: each dequantising warp does
+// 32 of its rows once more in fp32. Everything is derived anew, so that nothing of
+// it is kept in registers before.
+template <int NB, bool LO>
+__device__ __forceinline__ void redo_rows(const PrefixArgs& a, uint8_t* smem) {
+  using R = PrefixTraits<NB, LO>;
+  int cta = blockIdx.x, tid = threadIdx.x;
+  asm volatile("" : "+r"(cta), "+r"(tid), "+l"(smem));
+  smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem) + 1023) & ~(uintptr_t)1023);
+  if (!*reinterpret_cast<const uint32_t*>(smem + R::OFF_BIG)) return;
+  const int lane = tid & 31, dw = (tid >> 5) - kDeqWarp;
+  float* scratch = reinterpret_cast<float*>(smem + R::OFF_RAW + dw * kRaw * 16 * Row<NB>::PITCH);
+  const PrefixJob job(a, cta);
+#pragma unroll 1
+  for (int row = job.row0 + dw * 32, end = min(row + 32, a.B * a.G); row < end; ++row) {
+    const int b = row / a.G, qrow = b * a.Hq + job.h * a.G + row % a.G;
+    const int keys = max(0, min(min(a.seq_lens[b], a.limit), a.prefix_len));
+    const Tokens tokens{a.k, a.v, a.table, a.table, a.num_pages, (long long)a.Hkv * Row<NB>::BYTES, job.h * Row<NB>::BYTES,
+                        a.ps, a.prefix_len};
+    __syncwarp();
+    for (int x = lane; x < NB * 32; x += 32) {
+      const uint16_t v = static_cast<const uint16_t*>(a.q)[(long long)qrow * (NB * 32) + x];
+      scratch[x] = (a.q_bf16 ? __uint_as_float((uint32_t)v << 16) : half_bits_to_float(v)) * a.scale;
+    }
+    __syncwarp();
+    float m, l, acc[NB];
+    attend_tokens<1>(tokens, NB, job.j0 * kBlk, min(keys, (job.j0 + job.n) * kBlk), scratch, scratch + NB * 32 + 64,
+                  reinterpret_cast<long long*>(scratch + NB * 32), m, l, acc);
+    const long long at = (long long)job.chunk * a.B * a.Hq + qrow;
+#pragma unroll
+    for (int x = 0; x < NB; ++x) a.part[at * (NB * 32) + 32 * x + lane] = acc[x];
+    if (lane == 0) a.ml[at] = make_float2(m * 1.44269504088896340736f, l);
+  }
+}
+
 template <int NB, bool LO>
 __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(const PrefixArgs a) {
   using R = PrefixTraits<NB, LO>;
@@ -699,15 +821,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
   uint64_t* drained = q_full + 1;      // all of the MMA warp's products and arrivals are done
   uint64_t* row_mask = drained + 1;    // rows present in block j, at j % kMasks
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(row_mask + kMasks);
-  static_assert((4 * kOps + 8 + kMasks) * 8 + 4 <= 512, "barrier area");
+  uint32_t* big = reinterpret_cast<uint32_t*>(smem + R::OFF_BIG);  // a scale past the operands' range was met
+  static_assert((4 * kOps + 8 + kMasks) * 8 + 4 <= 508, "barrier area");
+  static_assert(kDeqWarps == 8 && kRaw * 16 * Row<NB>::PITCH >= NB * 128 + 128 + 256, "a warp's ring holds a row's scratch");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
 
-  const int chunk = blockIdx.x % a.chunks, hp = blockIdx.x / a.chunks, h = hp % a.Hkv, row0 = hp / a.Hkv * 2 * kTile;
+  const PrefixJob job(a, blockIdx.x);
+  const int chunk = job.chunk, h = job.h, row0 = job.row0, j0 = job.j0, n = job.n;
   const int rows = a.B * a.G;
   const bool two = row0 + kTile < rows;
-  const int blocks = (a.prefix_len + kBlk - 1) / kBlk;
-  const int j0 = (int)((long long)blocks * chunk / a.chunks), n = (int)((long long)blocks * (chunk + 1) / a.chunks) - j0;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * kOps; ++i) {
@@ -721,6 +844,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
     }
     mbar_init(q_full, two ? 8 : 4);
     mbar_init(drained, 1);
+    *big = 0;
     fence_mbar_init();
   }
   // The set-up's barrier, which every role meets with its first loads out.
@@ -801,6 +925,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
         if (low) *reinterpret_cast<uint4*>(o + R::PART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     };
+    uint32_t top = 0;  // bit 14 or 30: |d| of 512 or more (both high exponent bits), infinite or NaN
     for (int j = 0; j < n; ++j) {
       const int os = j % kOps;
       rows_at[kRaw - 1] = issue(j + kRaw - 1);
@@ -812,6 +937,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
       uint32_t wk[9], wv[9];
       words(row, present, wk);
       words(row + 8 * Row<NB>::PITCH, present, wv);
+      const uint32_t d = __byte_perm(wk[0] >> sh, wv[0] >> sh, 0x5410);  // the scales of K and V
+      top |= d & (d << 1);
       // K is free again once its scores are there, V a block later
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
@@ -824,6 +951,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
 #pragma unroll
       for (int x = 0; x + 1 < kRaw; ++x) rows_at[x] = rows_at[x + 1];
     }
+    if (top & 0x40004000u) *big = 1;
+    named_bar_sync(1, (8 + kDeqWarps) * 32);  // also: the softmax warps have stored their rows
+    redo_rows<NB, LO>(a, smem_raw);
   } else if (warp == kMmaWarp) {
     constexpr uint32_t idesc_s = idesc_h(kBlk, false), idesc_o = idesc_h(DP, true);
     tc::tmem_alloc(tmem_slot, 512);
@@ -1023,6 +1153,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
           if (out[x]) *reinterpret_cast<uint4*>(out[x] + x0) = v[x];
       }
     }
+    named_bar_arrive(1, (8 + kDeqWarps) * 32);
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -1157,8 +1288,7 @@ __global__ void __launch_bounds__(kCta, kCombineCtas) fa_paged_combine_kernel(co
 
 // ---- pages of other sizes than a multiple of 8 tokens, or a prefix that ends within 8
 // tokens where the prefix kernel does not run (D > 128) ------------------------------------
-// One warp per (sequence, query head), 32 tokens per step: a lane per token
-// for q . k, then a lane per dimension for p . v.
+// One warp per (sequence, query head).
 constexpr int kWarps = 4;
 
 template <typename T>
@@ -1166,67 +1296,19 @@ __global__ void __launch_bounds__(kWarps * 32) fa_paged_simple_kernel(const FaPa
   __shared__ float s_q[kWarps][kMaxNB * 32];
   __shared__ float s_p[kWarps][32];
   __shared__ long long s_row[kWarps][32];
-  const unsigned full = 0xffffffffu;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long item = (long long)blockIdx.x * kWarps + warp;
   if (item >= (long long)a.B * a.Hq) return;
-  const int b = (int)(item / a.Hq), h = (int)(item % a.Hq), kh = h / (a.Hq / a.Hkv);
-  const int nb = a.D / 32;
-  const long long row_bytes = (long long)a.Hkv * nb * kQ8;
+  const int b = (int)(item / a.Hq), h = (int)(item % a.Hq), kh = h / (a.Hq / a.Hkv), nb = a.D / 32;
   const int len = (int)min((long long)max(0, min(a.seq_lens[b], a.max_seqlen)), (long long)a.W * a.ps);
-  const T* q = static_cast<const T*>(a.q) + ((long long)b * a.Hq + h) * a.D;
+  const T* q = static_cast<const T*>(a.q) + item * a.D;
   for (int d = lane; d < a.D; d += 32) s_q[warp][d] = to_f(q[d]) * a.scale;
   __syncwarp();
-  float m = -INFINITY, l = 0.0f, acc[kMaxNB];
-#pragma unroll
-  for (int t = 0; t < kMaxNB; ++t) acc[t] = 0.0f;
-  for (int j0 = 0; j0 < len; j0 += 32) {
-    const int j = j0 + lane;
-    float s = -INFINITY;
-    long long off = -1;
-    if (j < len) {
-      const long long page = a.table[(long long)(j < a.prefix_len ? 0 : b) * a.W + j / a.ps];
-      if (page >= 0 && page < a.num_pages) {
-        off = (page * a.ps + j % a.ps) * row_bytes + (long long)kh * nb * kQ8;
-        const uint8_t* k = a.k + off;
-        s = 0.0f;
-        for (int t = 0; t < nb; ++t) {
-          const float d = half_bits_to_float(*reinterpret_cast<const uint16_t*>(k + t * kQ8));
-          float dot = 0.0f;
-          for (int e = 0; e < 32; ++e) dot = fmaf(s_q[warp][t * 32 + e], (float)(int8_t)k[t * kQ8 + 2 + e], dot);
-          s = fmaf(d, dot, s);
-        }
-      }
-    }
-    const float mn = fmaxf(m, warp_max(s));
-    const float base = mn == -INFINITY ? 0.0f : mn;
-    const float p = off < 0 ? 0.0f : __expf(s - base);
-    const float c = __expf(m - base);
-    float ps = p;
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) ps += __shfl_xor_sync(full, ps, o);
-    l = l * c + ps;
-    m = mn;
-    s_p[warp][lane] = p;
-    s_row[warp][lane] = off;
-    __syncwarp();
-#pragma unroll
-    for (int t = 0; t < kMaxNB; ++t) acc[t] *= c;
-    const int n = min(32, len - j0);
-    for (int jj = 0; jj < n; ++jj) {
-      if (s_row[warp][jj] < 0) continue;
-      const float pj = s_p[warp][jj];
-      const uint8_t* v = a.v + s_row[warp][jj];
-#pragma unroll
-      for (int t = 0; t < kMaxNB; ++t)
-        if (t < nb) {
-          const float d = half_bits_to_float(*reinterpret_cast<const uint16_t*>(v + t * kQ8));
-          acc[t] = fmaf(pj * d, (float)(int8_t)v[t * kQ8 + 2 + lane], acc[t]);
-        }
-    }
-    __syncwarp();
-  }
-  T* out = static_cast<T*>(a.out) + ((long long)b * a.Hq + h) * a.D;
+  const Tokens tokens{a.k, a.v, a.table, a.table + (long long)b * a.W, a.num_pages, (long long)a.Hkv * nb * kQ8,
+                      (long long)kh * nb * kQ8, a.ps, a.prefix_len};
+  float m, l, acc[kMaxNB];
+  attend_tokens<32>(tokens, nb, 0, len, s_q[warp], s_p[warp], s_row[warp], m, l, acc);
+  T* out = static_cast<T*>(a.out) + item * a.D;
   const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // NaN stays NaN
 #pragma unroll
   for (int t = 0; t < kMaxNB; ++t)
@@ -1388,6 +1470,7 @@ kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s) {
     x.prefix_len = a.prefix_len, x.limit = p.split.limit, x.chunks = chunks;
     x.table = a.table, x.seq_lens = a.seq_lens;
     x.flip = p.sl < 0.0f ? 0x80000000u : 0u;
+    x.scale = a.scale;
     x.sl = fmaxf(fabsf(p.sl), kMinScale);
     x.part = reinterpret_cast<float*>(ws + w.ppart), x.ml = reinterpret_cast<float2*>(ws + w.pml);
     x.err = device_error_word();

@@ -162,3 +162,56 @@ def test_decode_small_value_scales(cuda, dtype, D, G, prefix, d, gap):
     ref, spread, top = decode_ref(q, kc, vc, table, lens, D ** -0.5)
     got = kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix)
     check_decode(got, ref, spread, top, dtype)
+
+
+6
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("which", ["k", "v", "both"])
+@pytest.mark.parametrize("prefix,D,Hkv,G", [(0, 128, 2, 4), (203, 128, 2, 4), (203, 64, 1, 15), (77, 96, 3, 1), (0, 256, 2, 9)])
+def test_decode_large_scales(cuda, dtype, which, prefix, D, Hkv, G):
+    """Block scales up to the largest fp16 number, among ordinary ones, whichever kernel reads them."""
+    import kq
+    g = gen(61)
+    lens = [300, 210, 77, 500]
+    kc, vc, table = paged_case(g, lens, prefix, 16, Hkv, D)
+    scales = torch.tensor([0.01, 0.5, 600.0, 1500.0, 30000.0, 65504.0], dtype=torch.float16, device=cuda)
+    for c, name in ((kc, "k"), (vc, "v")):
+        if which in (name, "both"):
+            pick = torch.randint(0, 6, c.shape[:-1], generator=g, device="cuda")
+            pick[torch.rand(pick.shape, generator=g, device="cuda") < 0.7] = 0
+            c[..., :2] = scales[pick].unsqueeze(-1).view(torch.uint8)
+    big = 127 * 65504.0
+    q = rows(g, len(lens), G * Hkv, D, dtype, 4.0 / big * D ** 0.5 if which != "v" else 1.0)
+    # outputs that the type holds: fp16's reach up to 65504
+    if dtype == torch.float16 and which != "k":
+        vc[..., 2:] = torch.where(vc[..., 2:].view(torch.int8) > 0, 1, -1).to(torch.int8).view(torch.uint8)
+    scale = D ** -0.5 if which == "v" else 1.0 / D
+    if which != "v" and dtype == torch.float16:  # fp16 queries this small are subnormal: exact inputs all the same
+        q = rows(g, len(lens), G * Hkv, D, dtype, 2.0 ** -18)
+        scale = 2.0 ** -5
+    ref, spread, top = decode_ref(q, kc, vc, table, lens, scale)
+    got = kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix, scale=scale)
+    if dtype == torch.float16:
+        fits = ref.abs() < 6.5e4
+        assert fits.any()
+        got, ref, spread = got[fits], ref[fits], spread[fits]
+    check_decode(got, ref, spread, top, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan"), 60000.0])
+@pytest.mark.parametrize("prefix", [200, 203])
+def test_decode_hidden_prefix_tokens(cuda, dtype, bad, prefix):
+    """Sequences that end inside the prefix do not see what its later tokens hold."""
+    import kq
+    g = gen(62)
+    lens = [prefix + 50, 70, prefix, 1, 129, 0] + [100] * 40
+    kc, vc, table = paged_case(g, lens, prefix, 16, 2, 128)
+    q = rows(g, len(lens), 8, 128, dtype)
+    ref, spread, top = decode_ref(q, kc, vc, table, lens, 128 ** -0.5)
+    at = 150
+    for c in (kc, vc):
+        c[table[0, at // 16].item(), at % 16, :, 1, :2] = half_bytes(bad)
+    got = kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix)
+    short = [b for b, n in enumerate(lens) if n <= at]
+    check_decode(got[short], ref[short], spread[short], top, dtype)
