@@ -375,11 +375,10 @@ kq_status_t kq_page_read_q8_0(int dtype, const void* k_cache, const void* v_cach
  * cu_seqlens_q[b+1]-1 and k / v rows cu_seqlens_k[b] .. (int32 [B+1],
  * device); query head h reads KV head h / (Hq / Hkv); causal: row i sees keys
  * j <= i + (len_k - len_q). A row without keys is zero; rows of out past
- * cu_seqlens_q[B] are not specified. Rows of other sequences never reach a
- * sequence's output, whatever they hold; an infinity or NaN in v at a key that
- * only the causal mask hides may reach rows up to 127 keys before it. q, k
- * and v are 2-byte and out 16-byte aligned (the tensor-core kernel runs where
- * bases and strides are multiples of 16 bytes and D <= 128). D % 8 == 0, D <= 256.
+ * cu_seqlens_q[B] are not specified. Rows of other sequences, and keys that
+ * the causal mask hides, never reach a row, whatever they hold. q, k and v are
+ * 2-byte and out 16-byte aligned (the tensor-core kernel runs where bases and
+ * strides are multiples of 16 bytes and D <= 128). D % 8 == 0, D <= 256.
  * workspace: kq_fa_prompt_workspace() bytes of device memory, 16-byte
  * aligned, used by this call only until it has run. */
 size_t kq_fa_prompt_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int D);
@@ -396,9 +395,10 @@ kq_status_t kq_fa_prompt(int dtype, const void* q, const void* k, const void* v,
  * for the whole batch where that pays); a sequence shorter than that sees its
  * first seq_lens[b] of them. max_seqlen bounds the lengths (it sizes the work
  * split; longer sequences are cut to it). Tokens in pages outside the cache
- * are hidden, whatever they hold. Block scales are any fp16 numbers (one of
- * 512 or more, an infinity or a NaN in a shared prefix sends the rows around it
- * down a slow path). q, out and the caches are 16-byte aligned. D % 32 == 0, D <= 256. workspace as above. */
+ * are hidden, and what tokens hold that a row does not see never reaches it.
+ * Block scales are any fp16 numbers (one of 512 or more, an infinity or a NaN
+ * in a shared prefix sends the rows around it down a slow path). q, out and the
+ * caches are 16-byte aligned. D % 32 == 0, D <= 256. workspace as above. */
 size_t kq_fa_decode_paged_workspace(int B, int Hq, int Hkv, int D, int prefix_len, int max_seqlen);
 kq_status_t kq_fa_decode_paged(int dtype, const void* q, const void* k_cache, const void* v_cache, int64_t num_pages,
                                int page_size, const int32_t* block_tables, int max_blocks, const int32_t* seq_lens,

@@ -33,11 +33,70 @@ __device__ __forceinline__ int find_seq(const int32_t* cu, int B, long long i) {
   return lo;
 }
 
-// ---- any shape: one warp per (row, query head) ----------------------------------
-// 32 keys per step, one per lane for q . k (q in shared memory as fp32), then
-// the lanes own output dimensions for p . v. Bound by its scalar loads and
-// FMAs; it serves the head sizes and strides that the tensor-core kernel
-// does not take.
+// ---- one row by one warp ----------------------------------------------------------
+// The softmax state (natural units) of keys j0 .. j1 - 1 for the scaled query s_q
+// in shared memory; s_p holds 32 values. 32 keys per step, one per lane for q . k,
+// then the lanes own output dimensions (lane + 32 t) for p . v. SHORT: little code
+// instead of unrolled loops.
+template <bool SHORT, int ND, typename T>
+__device__ __forceinline__ void attend_keys(const T* kb, const T* vb, long long k_row, long long v_row, int D, int j0, int j1,
+                                            const float* s_q, float* s_p, float& m, float& l, float (&acc)[ND]) {
+  const unsigned full = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int t = 0; t < ND; ++t) acc[t] = 0.0f;
+  for (; j0 < j1; j0 += 32) {
+    const int j = j0 + lane;
+    float s = -INFINITY;
+    if (j < j1) {
+      const T* k = kb + (long long)j * k_row;
+      float dot = 0.0f;
+      if constexpr (SHORT) {
+#pragma unroll 1
+        for (int d = 0; d < D; ++d) dot = fmaf(s_q[d], to_f(k[d]), dot);
+      } else {
+        for (int d = 0; d < D; ++d) dot = fmaf(s_q[d], to_f(k[d]), dot);
+      }
+      s = dot;
+    }
+    const float mn = fmaxf(m, warp_max(s));
+    // all keys so far at -inf: no weight yet (and no inf - inf)
+    const float base = mn == -INFINITY ? 0.0f : mn;
+    const float p = __expf(s - base);
+    const float c = __expf(m - base);
+    float ps = p;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) ps += __shfl_xor_sync(full, ps, o);
+    l = l * c + ps;
+    m = mn;
+    s_p[lane] = p;
+    __syncwarp();
+#pragma unroll
+    for (int t = 0; t < ND; ++t) acc[t] *= c;
+    const int n = min(32, j1 - j0);
+    auto add = [&](int jj) {
+      const float pj = s_p[jj];
+      const T* v = vb + (long long)(j0 + jj) * v_row;
+#pragma unroll
+      for (int t = 0; t < ND; ++t) {
+        const int d = lane + 32 * t;
+        if (d < D) acc[t] = fmaf(pj, to_f(v[d]), acc[t]);
+      }
+    };
+    if constexpr (SHORT) {
+#pragma unroll 1
+      for (int jj = 0; jj < n; ++jj) add(jj);
+    } else {
+      for (int jj = 0; jj < n; ++jj) add(jj);
+    }
+    __syncwarp();
+  }
+}
+
+// ---- any shape ------------------------------------------------------------------
+// One warp per (row, query head). Bound by its scalar loads and FMAs; it serves
+// the head sizes and strides that the tensor-core kernel does not take.
 constexpr int kSimpleWarps = 4;
 constexpr int kMaxD = 256;
 
@@ -45,7 +104,6 @@ template <typename T>
 __global__ void __launch_bounds__(kSimpleWarps * 32) fa_prompt_simple_kernel(const FaPromptArgs a) {
   __shared__ float s_q[kSimpleWarps][kMaxD];
   __shared__ float s_p[kSimpleWarps][32];
-  const unsigned full = 0xffffffffu;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long item = (long long)blockIdx.x * kSimpleWarps + warp;
   if (item >= (long long)a.Tq * a.Hq) return;
@@ -61,44 +119,8 @@ __global__ void __launch_bounds__(kSimpleWarps * 32) fa_prompt_simple_kernel(con
   const T* vb = static_cast<const T*>(a.v) + (long long)k0 * a.v_row + (long long)kh * a.v_head;
   for (int d = lane; d < a.D; d += 32) s_q[warp][d] = to_f(q[d]) * a.scale;
   __syncwarp();
-  float m = -INFINITY, l = 0.0f, acc[kMaxD / 32];
-#pragma unroll
-  for (int t = 0; t < kMaxD / 32; ++t) acc[t] = 0.0f;
-  for (int j0 = 0; j0 < keys; j0 += 32) {
-    const int j = j0 + lane;
-    float s = -INFINITY;
-    if (j < keys) {
-      const T* k = kb + (long long)j * a.k_row;
-      float dot = 0.0f;
-      for (int d = 0; d < a.D; ++d) dot = fmaf(s_q[warp][d], to_f(k[d]), dot);
-      s = dot;
-    }
-    const float mn = fmaxf(m, warp_max(s));
-    // all keys so far at -inf: no weight yet (and no inf - inf)
-    const float base = mn == -INFINITY ? 0.0f : mn;
-    const float p = __expf(s - base);
-    const float c = __expf(m - base);
-    float ps = p;
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) ps += __shfl_xor_sync(full, ps, o);
-    l = l * c + ps;
-    m = mn;
-    s_p[warp][lane] = p;
-    __syncwarp();
-#pragma unroll
-    for (int t = 0; t < kMaxD / 32; ++t) acc[t] *= c;
-    const int n = min(32, keys - j0);
-    for (int jj = 0; jj < n; ++jj) {
-      const float pj = s_p[warp][jj];
-      const T* v = vb + (long long)(j0 + jj) * a.v_row;
-#pragma unroll
-      for (int t = 0; t < kMaxD / 32; ++t) {
-        const int d = lane + 32 * t;
-        if (d < a.D) acc[t] = fmaf(pj, to_f(v[d]), acc[t]);
-      }
-    }
-    __syncwarp();
-  }
+  float m, l, acc[kMaxD / 32];
+  attend_keys<false>(kb, vb, a.k_row, a.v_row, a.D, 0, keys, s_q[warp], s_p[warp], m, l, acc);
   const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // NaN stays NaN
 #pragma unroll
   for (int t = 0; t < kMaxD / 32; ++t) {
@@ -140,6 +162,12 @@ __global__ void __launch_bounds__(kSimpleWarps * 32) fa_prompt_simple_kernel(con
 // Warps: 4 softmax warps per tile (warp w reaches TMEM lanes 32 (w % 4) ..),
 // one that issues MMAs, one for jobs and TMA (and two idle ones that complete
 // the warpgroup whose registers go to the softmax warps where TILES = 2).
+// A key that the causal mask hides enters P V with weight 0, which an infinity or
+// NaN in its V row turns into NaN. So the rows' sums are looked at on their way
+// out, and a row with one that is not finite is done again in fp32 from its own
+// keys, if such a V row is among those that its tile went through and it does not
+// see (24 packed prompts 67.2 -> 68.6 us; a look at the V rows instead, by the load
+// warp or in shared memory, cost 5 us and more).
 // Every arrival has a waiter before the CTA ends: with two CTAs on an SM their
 // products share one queue, and an arrival that came after the CTA's end would
 // land in the next one's shared memory.
@@ -175,6 +203,10 @@ struct TcArgs {
   float* part;          // splits > 1: [split][Tq * Hq][D] unnormalised outputs
   float2* ml;           //             [split][Tq * Hq] maximum (log2 units), sum
   int* err;
+  // for rows done again
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  float scale;
 };
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
@@ -259,6 +291,48 @@ struct Job {
   int cnt[2];              // blocks of each tile
 };
 constexpr int kJobs = 3;   // jobs in the ring
+
+// Rows (bit: row of the warp's 32 of a tile) whose sums are not finite. A row that
+// shares its tile's blocks with hidden V rows that are not finite is computed
+// from its own keys. Everything is derived anew, so that nothing of it is kept in
+// registers before. scratch: 640 bytes of the warp.
+template <typename T, int ND, int BLK>
+__device__ __forceinline__ void redo_rows(const TcArgs& a, const Job* j, uint8_t* scratch, uint32_t bits) {
+  int tid = threadIdx.x;
+  asm volatile("" : "+r"(tid), "+l"(j), "+l"(scratch));
+  const int lane = tid & 31, t = tid >> 7, first = j->w.tok + t * a.TQ;
+  const int begin = j->j0 * BLK, end = min(j->w.lk, (j->j0 + j->cnt[t]) * BLK);  // the tile's keys
+  const T* kb = static_cast<const T*>(a.k) + (long long)j->w.k0 * a.k_row + (long long)j->head * a.k_head;
+  const T* vb = static_cast<const T*>(a.v) + (long long)j->w.k0 * a.v_row + (long long)j->head * a.v_head;
+  float* s_q = reinterpret_cast<float*>(scratch);
+#pragma unroll 1
+  for (; bits; bits &= bits - 1) {
+    const int row = (tid & 96) + __ffs(bits) - 1, g = row % a.G;
+    const int tok = first + row / a.G, keys = min(end, keys_of(a, j->w, tok)), lo = max(begin, keys);
+    bool odd = false;
+#pragma unroll 1
+    for (int r = lo; r < end; ++r)
+      for (int d = lane; d < a.D; d += 32) odd |= to_f(vb[r * a.v_row + d]) * 0.0f != 0.0f;
+    if (!__any_sync(0xffffffffu, odd)) continue;
+    const T* q = static_cast<const T*>(a.q) + (long long)(j->w.q0 + tok) * a.q_row + (long long)(j->head * a.G + g) * a.q_head;
+    __syncwarp();
+    for (int d = lane; d < a.D; d += 32) s_q[d] = to_f(q[d]) * a.scale;
+    __syncwarp();
+    float m, l, acc[ND];
+    attend_keys<true>(kb, vb, a.k_row, a.v_row, a.D, begin, keys, s_q, s_q + ND * 32, m, l, acc);
+    const long long at = (long long)(j->w.q0 + tok) * a.Hq + j->head * a.G + g, rows = (long long)a.Tq * a.Hq;
+    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // NaN stays NaN
+#pragma unroll
+    for (int x = 0; x < ND; ++x) {
+      const int d = lane + 32 * x;
+      if (d >= a.D) continue;
+      if (a.splits > 1) a.part[(j->split * rows + at) * a.D + d] = acc[x];
+      else store_f(static_cast<T*>(a.out) + at * a.D + d, acc[x] * inv);
+    }
+    // the other splits' sums carry 2^kBias: as if this m were higher
+    if (a.splits > 1 && lane == 0) a.ml[j->split * rows + at] = make_float2(m * 1.44269504088896340736f + kBias, l);
+  }
+}
 
 template <typename T, int DP, int TILES>
 __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
@@ -610,6 +684,7 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
         const int r = __shfl_sync(0xffffffffu, at, 8 * x + (lane >> 2));
         dst[x] = r >= 0 ? base + (long long)r * a.D * item + (lane & 3) * 16 : nullptr;
       }
+      F2 odd[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};           // NaN after a sum that is not finite
 #pragma unroll 1
       for (int x0 = 0; x0 < a.D; x0 += 32) {
         uint32_t o[32];
@@ -627,6 +702,9 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
 #pragma unroll
           for (int x = 0; x < 32; ++x) o[x] = 0;
         }
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          odd[x & 1] = fma2(f2(__uint_as_float(o[2 * x]), __uint_as_float(o[2 * x + 1])), f2(0.0f, 0.0f), odd[x & 1]);
         if (!partial) {
 #pragma unroll
           for (int x = 0; x < 16; ++x)
@@ -651,6 +729,10 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
             if (dst[x] && inside) *reinterpret_cast<uint4*>(dst[x] + col * item) = v[x];
         }
       }
+      float odd0, odd1;
+      unpack(add2(odd[0], odd[1]), odd0, odd1);
+      const uint32_t again = __ballot_sync(0xffffffffu, mine && nt > 0 && odd0 + odd1 != 0.0f);
+      if (a.causal && again) redo_rows<T, DP / 32, BLK>(a, &j, stage, again);
       finish_job(c);
     }
   }
@@ -751,6 +833,9 @@ kq_status_t launch_tc(const FaPromptArgs& a, int dtype, const Plan& plan, cudaSt
   p.part = static_cast<float*>(a.ws);
   p.ml = reinterpret_cast<float2*>(p.part + (size_t)plan.splits * a.Tq * a.Hq * a.D);
   p.err = device_error_word();
+  p.q = a.q, p.k = a.k, p.v = a.v;
+  p.q_row = a.q_row, p.q_head = a.q_head, p.k_row = a.k_row, p.k_head = a.k_head, p.v_row = a.v_row, p.v_head = a.v_head;
+  p.scale = a.scale;
   CUtensorMap mq, mk, mv;
   if (!encode_rows(&mq, dtype, a.q, a.D, a.Hq, a.Tq, a.q_head, a.q_row, p.G, p.TQ) ||
       !encode_rows(&mk, dtype, a.k, a.D, a.Hkv, a.Tk, a.k_head, a.k_row, 1, R::BLK) ||

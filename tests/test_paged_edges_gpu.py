@@ -1,12 +1,13 @@
 """Paged-serving operators where they can go wrong: lengths updated in place, padded free lists, scales and
 scores at the ends of their ranges, infinities and NaN in masked places, prefix sums that run past the rows,
 and the paths that only large batches take. Bounds as in test_paged_gpu, unless a test derives its own."""
+import math
 import random
 
 import pytest
 import torch
 
-from test_paged_gpu import U, check_out, decode_ref, gen, ints, paged_case, plan_ref, prefix_sums, rows
+from test_paged_gpu import U, check_out, decode_ref, gen, ints, paged_case, plan_ref, prefix_sums, prompt_ref, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -215,3 +216,39 @@ def test_decode_hidden_prefix_tokens(cuda, dtype, bad, prefix):
     got = kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix)
     short = [b for b, n in enumerate(lens) if n <= at]
     check_decode(got[short], ref[short], spread[short], top, dtype)
+
+
+# ---------------------------------------------------------------- prompts
+7
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lq,lk,Hq,Hkv,D,at", [
+    ([300], None, 4, 1, 128, (299, 130, 37)), ([300], None, 2, 2, 64, (255, 1)), ([1100], [1101], 2, 2, 128, (255, 700, 1100)),
+    ([1100], [1101], 4, 2, 64, (511, 128)), ([70, 200, 33], None, 28, 4, 128, (69, 150, 302)),
+    ([40], [3000], 8, 2, 128, (2999, 2970, 2961)), ([200], [4000], 8, 8, 128, (3999, 3850)), ([90], None, 6, 2, 80, (50, 89)),
+    ([1500], None, 15, 5, 96, (1, 640, 1499)), ([64], None, 2, 1, 256, (40,)),
+])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_prompt_hidden_values(cuda, dtype, lq, lk, Hq, Hkv, D, at, bad):
+    """An infinity or NaN in K or V reaches the rows that see its key, and no row before them."""
+    import kq
+    lk = lk or lq
+    g = gen(71)
+    q, k, v = rows(g, sum(lq), Hq, D, dtype), rows(g, sum(lk), Hkv, D, dtype), rows(g, sum(lk), Hkv, D, dtype)
+    ref, spread, top = prompt_ref(q, k, v, lq, lk, True, D ** -0.5)
+    cq, ck = prefix_sums(lq), prefix_sums(lk)
+    for where in ("v", "k"):
+        bk, bv = k.clone(), v.clone()
+        hidden = torch.ones(sum(lq), dtype=torch.bool, device=cuda)
+        for j in at:
+            (bv if where == "v" else bk)[j, :, 3::7] = bad
+            b = max(i for i in range(len(lk)) if ck[i] <= j)
+            first = cq[b] + max(0, j - ck[b] - (lk[b] - lq[b]))  # the first row that sees the key
+            hidden[first:cq[b + 1]] = False
+        got = kq.flash_prompt_ragged(q, bk, bv, ints(cq), ints(ck))
+        check_out(got[hidden], ref[hidden], spread[hidden], top, dtype, where)
+        dims = got[~hidden][..., 3::7] if where == "v" else got[~hidden]
+        if where == "v" or math.isnan(bad):
+            assert not torch.isfinite(dims).any(), where
+        if where == "v":
+            rest = [d for d in range(D) if d % 7 != 3]
+            check_out(got[~hidden][..., rest], ref[~hidden][..., rest], spread[~hidden][..., rest], top, dtype, "other dims")
