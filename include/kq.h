@@ -374,8 +374,9 @@ kq_status_t kq_page_read_q8_0(int dtype, const void* k_cache, const void* v_cach
  * contiguous, all of dtype. Sequence b owns q rows cu_seqlens_q[b] ..
  * cu_seqlens_q[b+1]-1 and k / v rows cu_seqlens_k[b] .. (int32 [B+1],
  * device); query head h reads KV head h / (Hq / Hkv); causal: row i sees keys
- * j <= i + (len_k - len_q). A row without keys is zero; rows of out past
- * cu_seqlens_q[B] are not specified. Rows of other sequences, and keys that
+ * j <= i + (len_k - len_q). A row without keys is zero; rows of out that no
+ * sequence owns are not specified. Prefix sums outside 0 .. Tq or 0 .. Tk are
+ * cut to that range. Rows of other sequences, and keys that
  * the causal mask hides, never reach a row, whatever they hold. q, k and v are
  * 2-byte and out 16-byte aligned (the tensor-core kernel runs where bases and
  * strides are multiples of 16 bytes and D <= 128). D % 8 == 0, D <= 256.

@@ -21,6 +21,10 @@ namespace {
 
 using namespace attn;
 
+// An entry of the prefix sums, cut to the rows that there are: nothing outside
+// them is read or written whatever the sums say.
+__device__ __forceinline__ int cut(int x, int rows) { return max(0, min(x, rows)); }
+
 // Sequence that owns packed row i: the last b with cu[b] <= i (empty ones
 // before it share that start and come earlier).
 __device__ __forceinline__ int find_seq(const int32_t* cu, int B, long long i) {
@@ -111,7 +115,8 @@ __global__ void __launch_bounds__(kSimpleWarps * 32) fa_prompt_simple_kernel(con
   const int h = (int)(item % a.Hq), kh = h / (a.Hq / a.Hkv);
   const int b = find_seq(a.cu_q, a.B, row);
   T* out = static_cast<T*>(a.out) + (row * a.Hq + h) * a.D;
-  const int q0 = a.cu_q[b], lq = a.cu_q[b + 1] - q0, k0 = a.cu_k[b], lk = a.cu_k[b + 1] - k0;
+  const int q0 = cut(a.cu_q[b], a.Tq), lq = cut(a.cu_q[b + 1], a.Tq) - q0;
+  const int k0 = cut(a.cu_k[b], a.Tk), lk = max(0, cut(a.cu_k[b + 1], a.Tk) - k0);
   const int i = (int)(row - q0);
   const int keys = i >= lq || i < 0 ? 0 : a.causal ? max(0, min(lk, i + lk - lq + 1)) : lk;
   const T* q = static_cast<const T*>(a.q) + row * a.q_row + (long long)h * a.q_head;
@@ -196,7 +201,7 @@ struct TcTraits {
 
 struct TcArgs {
   const int32_t *cu_q, *cu_k;
-  int B, Tq, Hq, Hkv, G, TQ, D, causal, slots, splits;
+  int B, Tq, Tk, Hq, Hkv, G, TQ, D, causal, slots, splits;
   float sl;             // scale * log2(e), not negative
   uint32_t flip;        // sign bit where scale < 0: scores are negated first
   void* out;
@@ -261,17 +266,17 @@ __device__ __forceinline__ bool find_work(const TcArgs& a, int tt, int slot, Wor
   int lo = 0, n = a.B;
   while (n > 1) {
     const int step = (n + 31) / 32, mid = lo + lane * step;
-    const bool before = mid < lo + n && a.cu_q[mid] / tt + mid <= slot;
+    const bool before = mid < lo + n && cut(a.cu_q[mid], a.Tq) / tt + mid <= slot;
     const int last = 31 - __clz(__ballot_sync(0xffffffffu, before) | 1u);
     n = min(step, n - last * step);
     lo += last * step;
   }
-  w.q0 = a.cu_q[lo];
-  w.lq = min(a.cu_q[lo + 1], a.Tq) - w.q0;
-  w.k0 = a.cu_k[lo];
-  w.lk = max(0, a.cu_k[lo + 1] - w.k0);
+  w.q0 = cut(a.cu_q[lo], a.Tq);
+  w.lq = cut(a.cu_q[lo + 1], a.Tq) - w.q0;
+  w.k0 = cut(a.cu_k[lo], a.Tk);
+  w.lk = max(0, cut(a.cu_k[lo + 1], a.Tk) - w.k0);
   w.tok = (slot - (w.q0 / tt + lo)) * tt;
-  return w.tok < w.lq;
+  return w.tok >= 0 && w.tok < w.lq;  // slots in front of the first sequence are empty too
 }
 // Keys that token i of the sequence sees.
 __device__ __forceinline__ int keys_of(const TcArgs& a, const Work& w, int i) {
@@ -821,7 +826,7 @@ kq_status_t launch_tc(const FaPromptArgs& a, int dtype, const Plan& plan, cudaSt
   using R = TcTraits<DP, TILES>;
   TcArgs p{};
   p.cu_q = a.cu_q, p.cu_k = a.cu_k;
-  p.B = a.B, p.Tq = a.Tq, p.Hq = a.Hq, p.Hkv = a.Hkv, p.D = a.D, p.causal = a.causal;
+  p.B = a.B, p.Tq = a.Tq, p.Tk = a.Tk, p.Hq = a.Hq, p.Hkv = a.Hkv, p.D = a.D, p.causal = a.causal;
   p.G = a.Hq / a.Hkv;
   p.TQ = kTile / p.G;
   p.slots = plan.slots;

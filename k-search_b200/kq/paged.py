@@ -209,8 +209,8 @@ def flash_prompt_ragged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_se
     head dimension has to be contiguous); cu_seqlens_q, cu_seqlens_k int32
     [B+1] on the device (cu_seqlens_k defaults to cu_seqlens_q). causal: row i
     of a sequence sees keys up to i + (len_k - len_q), so a chunk sees the
-    context before it; a row without keys is zero, rows past cu_seqlens_q[B]
-    are not specified."""
+    context before it; a row without keys is zero, rows that no sequence owns
+    are not specified. Prefix sums are cut to the rows that there are."""
     dt = _float16(q, "q")
     Tq, Hq, D = _rows(q, "q", q.dtype)
     dev = q.device

@@ -252,3 +252,29 @@ def test_prompt_hidden_values(cuda, dtype, lq, lk, Hq, Hkv, D, at, bad):
         if where == "v":
             rest = [d for d in range(D) if d % 7 != 3]
             check_out(got[~hidden][..., rest], ref[~hidden][..., rest], spread[~hidden][..., rest], top, dtype, "other dims")
+
+
+8
+@pytest.mark.parametrize("D,offset", [(128, 0), (64, 0), (256, 0), (128, 1)])
+def test_prompt_prefix_sums_past_the_rows(cuda, D, offset):
+    """Prefix sums outside the rows given are cut to them: nothing outside is read or written."""
+    import kq
+    g = gen(81)
+    Tq, Tk, Hq, Hkv, dtype = 200, 200, 4, 2, torch.float16
+    flat = torch.randn(Tk * Hkv * D + 8, generator=g, device="cuda").to(dtype)
+    k = flat[offset:offset + Tk * Hkv * D].view(Tk, Hkv, D)
+    q, v = rows(g, Tq, Hq, D, dtype), rows(g, Tk, Hkv, D, dtype)
+    guarded = torch.full((3 * Tq, Hq, D), 7.0, dtype=dtype, device=cuda)
+    out = guarded[Tq:2 * Tq]
+    for causal in (True, False):
+        # the last sequence claims more than there is
+        got = kq.flash_prompt_ragged(q, k, v, ints([0, 90, 2 ** 31 - 1]), ints([0, 90, 2 ** 31 - 1]), causal=causal, out=out)
+        ref, spread, top = prompt_ref(q, k, v, [90, 110], [90, 110], causal, D ** -0.5)
+        check_out(got, ref, spread, top, dtype, f"causal={causal}")
+        # a first entry above zero, and one below
+        got = kq.flash_prompt_ragged(q, k, v, ints([60, 200]), ints([60, 200]), causal=causal, out=out)
+        ref, spread, top = prompt_ref(q[60:], k[60:], v[60:], [140], [140], causal, D ** -0.5)
+        check_out(got[60:], ref, spread, top, dtype, f"behind 60 rows, causal={causal}")
+        kq.flash_prompt_ragged(q, k, v, ints([-500, 100, 200]), ints([-9, 100, 2 ** 30]), causal=causal, out=out)
+    torch.cuda.synchronize()
+    assert (guarded[:Tq] == 7).all() and (guarded[2 * Tq:] == 7).all() and kq.device_error() == 0
