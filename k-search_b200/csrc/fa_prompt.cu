@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
   uint64_t* kv_empty = kv_full + STAGES;
   uint64_t* s_full = kv_empty + STAGES;      // [tile][buffer]: S is there
   uint64_t* p_full = s_full + NBUF * TILES;  // [tile][half]: 64 keys of P are there
-  uint64_t* pv_done = p_full + HALVES * TILES;  // [tile]: the product of a block with V is done
+  uint64_t* pv_done = p_full + HALVES * TILES;  // [tile]: the product of a block with V is done (one S buffer: a job's last)
   uint64_t* o_empty = pv_done + TILES;       // [tile]: O is read, the next job may overwrite it
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + TILES);
   Job* jobs = reinterpret_cast<Job*>(tmem_slot + 2);
@@ -557,7 +557,7 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
               tc::mma_ts_go(tmem + kColO + t * DP, tmem + t * 128 + (u % NBUF) * BLK + 8 * k, vd + (uint64_t)(k * (2048 >> 4)),
                             idesc_o, (i > 0 || k > 0) ? 1u : 0u, go);
           }
-          tc::mma_commit_go(&pv_done[t], go);
+          if (NBUF == 2 || i + 1 == j.cnt[t]) tc::mma_commit_go(&pv_done[t], go);
           // one buffer: the next scores take the place of the P just consumed (the products run in order)
           if (NBUF == 1 && i + 1 < j.cnt[t]) score(t, i + 1);
         }
@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + t * 128, o_addr = tmem + lanes + kColO + t * DP;
     uint8_t* stage = smem + R::OFF_OUT + warp * R::OUT;
-    int items = 0, done = 0;  // K / V blocks of earlier jobs, this tile's blocks so far
+    int items = 0, done = 0, ended = 0;  // K / V blocks of earlier jobs, this tile's blocks and jobs so far
     for (int c = 0;; ++c) {
       const Job& j = take_job(c);
       if (dead || j.n < 0) break;
@@ -630,9 +630,10 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
           l2 = mul2(l2, f2(f, f));
         }
         // Before O is touched the product of the block before must be done. With
-        // one buffer it is, as S came after it; with two, its arrival (normally
-        // long there) is taken before this block's P goes out, so that none is
-        // missed.
+        // one buffer it is, as S came after it, and pv_done arrives at a job's end
+        // only; with two, its arrival (normally long there) is taken before this
+        // block's P goes out. Either way no wait falls two arrivals behind, where
+        // the parity would let it through early.
         if (NBUF == 2 && i > 0) mbar_wait_or_poison(&pv_done[t], (u - 1) & 1, a.err, DEV_TIMEOUT_FULL, dead);
         if (i > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
           __syncwarp();
@@ -669,7 +670,8 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
       unpack(l2, l, l1);
       l += l1;
       if (nt > 0) {
-        mbar_wait_or_poison(&pv_done[t], (done - 1) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        mbar_wait_or_poison(&pv_done[t], (NBUF == 2 ? done - 1 : ended) & 1, a.err, DEV_TIMEOUT_FULL, dead);
+        ++ended;
         __syncwarp();
         tc::tc_fence_after();
       }

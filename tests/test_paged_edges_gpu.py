@@ -278,3 +278,33 @@ def test_prompt_prefix_sums_past_the_rows(cuda, D, offset):
         kq.flash_prompt_ragged(q, k, v, ints([-500, 100, 200]), ints([-9, 100, 2 ** 30]), causal=causal, out=out)
     torch.cuda.synchronize()
     assert (guarded[:Tq] == 7).all() and (guarded[2 * Tq:] == 7).all() and kq.device_error() == 0
+
+
+QUEUES = [
+    # lens q, lens k, Hq, Hkv, D: several times the CTAs that fit at once, of one tile and of two
+    ([1, 0, 400, 33, 900, 128, 1, 0, 700, 257, 64, 811, 1, 500, 90, 0, 640], None, 32, 8, 128),
+    ([0, 300, 1, 1000, 129, 77, 0, 640, 31, 2, 900, 450], None, 28, 4, 128),
+    ([700, 1, 0, 900, 600, 333, 800, 127], None, 32, 32, 64),
+    ([1024, 1, 2000, 0, 3000, 1500], None, 32, 8, 128), ([2500, 0, 1, 1800, 1300], None, 28, 7, 64),
+    ([900, 1, 0, 700, 1200], [2000, 500, 0, 700, 2900], 30, 10, 96),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lq,lk,Hq,Hkv,D", QUEUES)
+def test_prompt_queues(cuda, dtype, lq, lk, Hq, Hkv, D):
+    """Many more jobs than CTAs fit at once: each takes several, empty and one-token sequences among them."""
+    import kq
+    lk = lk or lq
+    tiles = 2 if sum(lk) // len(lk) >= 1024 else 1
+    rows_per_cta = 128 // (Hq // Hkv) * tiles
+    resident = torch.cuda.get_device_properties(0).multi_processor_count * (1 if tiles == 2 else 2)
+    assert sum(-(-n // rows_per_cta) for n in lq) * Hkv > 1.9 * resident
+    g = gen(sum(lq) + D)
+    q, k, v = rows(g, sum(lq), Hq, D, dtype, 1.5), rows(g, sum(lk), Hkv, D, dtype), rows(g, sum(lk), Hkv, D, dtype)
+    for causal in (True, False):
+        ref, spread, top = prompt_ref(q, k, v, lq, lk, causal, D ** -0.5)
+        for _ in range(3):  # which CTA takes which job differs from call to call
+            got = kq.flash_prompt_ragged(q, k, v, ints(prefix_sums(lq)), ints(prefix_sums(lk)), causal=causal)
+            check_out(got, ref, spread, top, dtype, f"causal={causal}")
+    assert kq.device_error() == 0
