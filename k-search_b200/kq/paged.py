@@ -259,7 +259,8 @@ def flash_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
         raise ValueError(f"q has head dimension {D}, the caches {nb * 32}")
     W = _table(block_tables, dev, B)[1]
     _vector(seq_lens, "seq_lens", torch.int32, dev, B)
-    max_seqlen = W * ps if max_seqlen is None else min(int(max_seqlen), W * ps)
+    most = min(W * ps, 2 ** 31 - 1)  # a 32-bit argument
+    max_seqlen = most if max_seqlen is None else min(int(max_seqlen), most)
     if scale is None:
         scale = D ** -0.5
     out = _out_like(q, out)

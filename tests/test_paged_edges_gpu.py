@@ -218,6 +218,19 @@ def test_decode_hidden_prefix_tokens(cuda, dtype, bad, prefix):
     check_decode(got[short], ref[short], spread[short], top, dtype)
 
 
+0
+def test_decode_table_wider_than_32_bits(cuda):
+    """A table whose pages could hold 2^32 tokens: the default bound on the lengths does not wrap."""
+    import kq
+    g = gen(91)
+    ps, W = 1 << 15, 1 << 17
+    kc, vc, _ = paged_case(g, [ps], 0, ps, 1, 32, spare=0)
+    table = torch.zeros((1, W), dtype=torch.int32, device=cuda)
+    q = rows(g, 1, 2, 32, torch.float16)
+    ref, spread, top = decode_ref(q, kc, vc, table[:, :1], [1000], 32 ** -0.5)
+    check_out(kq.flash_decode_paged(q, kc, vc, table, ints([1000])), ref, spread, top, torch.float16)
+
+
 # ---------------------------------------------------------------- prompts
 7
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
