@@ -1,8 +1,10 @@
 """Paged-serving operators where they can go wrong: lengths updated in place, padded free lists, scales and
 scores at the ends of their ranges, infinities and NaN in masked places, prefix sums that run past the rows,
 and the paths that only large batches take. Bounds as in test_paged_gpu, unless a test derives its own."""
+import importlib.util
 import math
 import random
+from pathlib import Path
 
 import pytest
 import torch
@@ -231,6 +233,34 @@ def test_decode_table_wider_than_32_bits(cuda):
     check_out(kq.flash_decode_paged(q, kc, vc, table, ints([1000])), ref, spread, top, torch.float16)
 
 
+LARGE = [
+    # lens, prefix, page, Hq, Hkv, D: more units than the 8-warp kernel is used for
+    ([500 + 10 * i for i in range(64)], 0, 16, 32, 8, 128), ([260 + i for i in range(300)], 0, 32, 8, 4, 64),
+    ([600 + i for i in range(64)], 0, 16, 24, 8, 96), ([600 + i for i in range(64)], 0, 24, 8, 8, 32),
+    ([640 + i for i in range(64)], 0, 16, 16, 8, 160), ([640 + i for i in range(64)], 0, 16, 8, 8, 192),
+    ([640 + i for i in range(64)], 0, 64, 16, 8, 224), ([640 + i for i in range(64)], 0, 16, 32, 8, 256),
+    ([2500] * 40 + [2600 + i for i in range(24)], 0, 16, 32, 2, 128), ([1600 + i for i in range(72)], 0, 16, 40, 1, 64),
+    ([1600] * 64 + [0, 1, 17], 0, 32, 45, 3, 96), ([2600 + i for i in range(64)], 0, 128, 18, 2, 32),
+    ([2500 + i for i in range(64)], 0, 16, 32, 2, 256), ([2500 + i for i in range(64)], 0, 16, 24, 2, 160),
+    ([1024 + 500 + 10 * i for i in range(48)] + [0, 900, 1024], 1024, 16, 32, 8, 128),
+    ([515 + 1450 + i for i in range(70)], 515, 32, 45, 3, 96), ([256 + 640 + i for i in range(64)], 256, 16, 16, 8, 160),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,prefix,ps,Hq,Hkv,D", LARGE)
+def test_decode_large_batches(cuda, dtype, lens, prefix, ps, Hq, Hkv, D):
+    """Enough to stream for the kernel with twelve warps, at every head size and with groups up to three sixteens."""
+    import kq
+    g = gen(sum(lens) + D)
+    units = len(lens) * Hkv * (-(-(Hq // Hkv) // 16)) * ((max(lens) - prefix) // 16 + 1)
+    assert units > 16 * 8 * torch.cuda.get_device_properties(0).multi_processor_count
+    kc, vc, table = paged_case(g, lens, prefix, ps, Hkv, D)
+    q = rows(g, len(lens), Hq, D, dtype)
+    ref, spread, top = decode_ref(q, kc, vc, table, lens, D ** -0.5)
+    check_out(kq.flash_decode_paged(q, kc, vc, table, ints(lens), prefix_len=prefix, max_seqlen=max(lens)), ref, spread, top, dtype)
+
+
 # ---------------------------------------------------------------- prompts
 7
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
@@ -321,3 +351,32 @@ def test_prompt_queues(cuda, dtype, lq, lk, Hq, Hkv, D):
             got = kq.flash_prompt_ragged(q, k, v, ints(prefix_sums(lq)), ints(prefix_sums(lk)), causal=causal)
             check_out(got, ref, spread, top, dtype, f"causal={causal}")
     assert kq.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype,kw", [
+    (torch.float16, dict(requests=7, system=320, prompt=90, Hq=16, Hkv=4, page_size=16)),
+    (torch.bfloat16, dict(requests=40, system=1024, prompt=90, Hq=28, Hkv=4, page_size=32)),
+])
+def test_example_prompt_outputs(cuda, dtype, kw):
+    """What the serving example's prompts and its system prompt return, against their definition."""
+    import kq
+    path = Path(__file__).resolve().parents[1] / "k-search_b200" / "examples" / "paged_serving.py"
+    spec = importlib.util.spec_from_file_location("paged_serving", path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    D, E, ps, R = 128, 256, kw["page_size"], kw["requests"]
+    g = gen(5)
+    layer = ex.Layer(E, kw["Hq"], kw["Hkv"], D, dtype, cuda)
+    new = [1 + kw["prompt"] * (b + 1) // R for b in range(R)]
+    pages = kw["system"] // ps + sum(-(-n // ps) for n in new)
+    server = ex.Server(layer, R, pages, ps, -(-(kw["system"] + max(new)) // ps), cuda)
+    x = torch.randn((kw["system"], E), generator=g, device="cuda").to(dtype)
+    got = server.system_prompt(x)
+    ref, spread, top = prompt_ref(*layer.qkv(x), [kw["system"]], [kw["system"]], True, D ** -0.5)
+    check_out(got, ref, spread, top, dtype, "system prompt")
+    x = torch.randn((sum(new), E), generator=g, device="cuda").to(dtype)
+    got = server.prompts(x, new)
+    lens = [kw["system"] + n for n in new]
+    keys, values = kq.page_read(server.k_cache, server.v_cache, server.tables, ints(prefix_sums(lens)), sum(lens), dtype)
+    ref, spread, top = prompt_ref(layer.qkv(x)[0], keys, values, new, lens, True, D ** -0.5)
+    check_out(got, ref, spread, top, dtype, "prompts")
