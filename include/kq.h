@@ -376,11 +376,13 @@ kq_status_t kq_page_read_q8_0(int dtype, const void* k_cache, const void* v_cach
  * device); query head h reads KV head h / (Hq / Hkv); causal: row i sees keys
  * j <= i + (len_k - len_q). A row without keys is zero; rows of out that no
  * sequence owns are not specified. Prefix sums outside 0 .. Tq or 0 .. Tk are
- * cut to that range. Rows of other sequences, and keys that
- * the causal mask hides, never reach a row, whatever they hold. q, k and v are
- * 2-byte and out 16-byte aligned (the tensor-core kernel runs where bases and
- * strides are multiples of 16 bytes and D <= 128). D % 8 == 0, D <= 256.
- * workspace: kq_fa_prompt_workspace() bytes of device memory, 16-byte
+ * cut to that range. Rows of other sequences, and keys that the causal mask
+ * hides, never reach a row, whatever they hold (with out on q itself, a row near
+ * an infinity or NaN in v that it does not see may be NaN; out does not overlap
+ * k or v). q, k and v are 2-byte and out 16-byte aligned. The tensor-core kernel
+ * runs where bases and strides are multiples of 16 bytes and D <= 128; anything
+ * else goes one row at a time, a hundred times slower and more. D % 8 == 0,
+ * D <= 256. workspace: kq_fa_prompt_workspace() bytes of device memory, 16-byte
  * aligned, used by this call only until it has run. */
 size_t kq_fa_prompt_workspace(int B, int Tq, int Tk, int Hq, int Hkv, int D);
 kq_status_t kq_fa_prompt(int dtype, const void* q, const void* k, const void* v, int64_t q_row_stride,

@@ -208,7 +208,7 @@ struct TcArgs {
   float* part;          // splits > 1: [split][Tq * Hq][D] unnormalised outputs
   float2* ml;           //             [split][Tq * Hq] maximum (log2 units), sum
   int* err;
-  // for rows done again
+  int redo;             // rows may be done again: causal, and their queries are not overwritten
   const void *q, *k, *v;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
   float scale;
@@ -739,7 +739,7 @@ __global__ void __launch_bounds__(TILES == 2 ? 384 : 192, TILES == 2 ? 1 : 2)
       float odd0, odd1;
       unpack(add2(odd[0], odd[1]), odd0, odd1);
       const uint32_t again = __ballot_sync(0xffffffffu, mine && nt > 0 && odd0 + odd1 != 0.0f);
-      if (a.causal && again) redo_rows<T, DP / 32, BLK>(a, &j, stage, again);
+      if (a.redo && again) redo_rows<T, DP / 32, BLK>(a, &j, stage, again);
       finish_job(c);
     }
   }
@@ -843,6 +843,9 @@ kq_status_t launch_tc(const FaPromptArgs& a, int dtype, const Plan& plan, cudaSt
   p.q = a.q, p.k = a.k, p.v = a.v;
   p.q_row = a.q_row, p.q_head = a.q_head, p.k_row = a.k_row, p.k_head = a.k_head, p.v_row = a.v_row, p.v_head = a.v_head;
   p.scale = a.scale;
+  const char *q0 = static_cast<const char*>(a.q), *o0 = static_cast<const char*>(a.out);
+  const int64_t q_bytes = 2 * ((a.Tq - 1) * (a.Tq > 1 ? a.q_row : 0) + (a.Hq - 1) * (a.Hq > 1 ? a.q_head : 0) + a.D);
+  p.redo = a.causal && (q0 + q_bytes <= o0 || o0 + 2 * (int64_t)a.Tq * a.Hq * a.D <= q0);
   CUtensorMap mq, mk, mv;
   if (!encode_rows(&mq, dtype, a.q, a.D, a.Hq, a.Tq, a.q_head, a.q_row, p.G, p.TQ) ||
       !encode_rows(&mk, dtype, a.k, a.D, a.Hkv, a.Tk, a.k_head, a.k_row, 1, R::BLK) ||

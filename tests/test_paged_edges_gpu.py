@@ -380,3 +380,22 @@ def test_example_prompt_outputs(cuda, dtype, kw):
     keys, values = kq.page_read(server.k_cache, server.v_cache, server.tables, ints(prefix_sums(lens)), sum(lens), dtype)
     ref, spread, top = prompt_ref(layer.qkv(x)[0], keys, values, new, lens, True, D ** -0.5)
     check_out(got, ref, spread, top, dtype, "prompts")
+
+
+@pytest.mark.parametrize("lq,lk,D", [([300, 70], None, 128), ([1200], None, 64), ([30], [2500], 128), ([40], None, 256)])
+def test_prompt_in_place(cuda, lq, lk, D):
+    """The output on the queries themselves: the same rows; next to a hidden NaN the true row or NaN, never another."""
+    import kq
+    lk = lk or lq
+    g = gen(101)
+    q, k, v = rows(g, sum(lq), 8, D, torch.float16), rows(g, sum(lk), 2, D, torch.float16), rows(g, sum(lk), 2, D, torch.float16)
+    cq, ck = ints(prefix_sums(lq)), ints(prefix_sums(lk))
+    ref, spread, top = prompt_ref(q, k, v, lq, lk, True, D ** -0.5)
+    x = q.clone()
+    check_out(kq.flash_prompt_ragged(x, k, v, cq, ck, out=x), ref, spread, top, torch.float16)
+    v[lk[0] - 1, :, 5] = float("nan")
+    x = q.clone()
+    got = kq.flash_prompt_ragged(x, k, v, cq, ck, out=x)
+    seen = torch.isfinite(got)
+    assert not seen[lq[0] - 1, :, 5].any()
+    check_out(got[seen], ref[seen], spread[seen], top, torch.float16)
