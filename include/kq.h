@@ -401,7 +401,9 @@ kq_status_t kq_fa_prompt(int dtype, const void* q, const void* k, const void* v,
  * are hidden, and what tokens hold that a row does not see never reaches it.
  * Block scales are any fp16 numbers (one of 512 or more, an infinity or a NaN
  * in a shared prefix sends the rows around it down a slow path). q, out and the
- * caches are 16-byte aligned. D % 32 == 0, D <= 256. workspace as above. */
+ * caches are 16-byte aligned. D % 32 == 0, D <= 256. Pages that are not a
+ * multiple of 8 tokens, and a streamed prefix that is not, go one row at a time
+ * on scalar instructions, some 50 times slower. workspace as above. */
 size_t kq_fa_decode_paged_workspace(int B, int Hq, int Hkv, int D, int prefix_len, int max_seqlen);
 kq_status_t kq_fa_decode_paged(int dtype, const void* q, const void* k_cache, const void* v_cache, int64_t num_pages,
                                int page_size, const int32_t* block_tables, int max_blocks, const int32_t* seq_lens,

@@ -116,10 +116,11 @@ __device__ __forceinline__ int units_before(const Split& sp, const SplitScan<T>&
 // 16000 tokens (8 KV heads of 128) took 101 us instead of 89. The head dimension
 // is permuted inside a block so that every operand word is one 32-bit load (a
 // word of 4 codes) per lane.
-// Those conversations are 310 MB: 84 us, 3.7 TB/s. The copies alone take 55; about
-// 600 instructions per 16 tokens and head go beside them (codes to fp16, scales,
-// addresses), at 2.0 instructions a clock and SM with 12 warps. 14 and 16 warps
-// take 81 and 84 us there, but 1 and 2 us more where sequences are short.
+// Those conversations are 310 MB: 85.6 us, 3.6 TB/s (84 with a constant 2^e). The
+// copies alone take 55; about 600 instructions per 16 tokens and head go beside
+// them (codes to fp16, scales, addresses), at 2.2 instructions a clock and SM with
+// 12 warps. 14 and 16 warps took 81 and 84 us there, but 1 and 2 us more where
+// sequences are short.
 constexpr int kStreamWarps = 12;  // 12 warps with 3 stages, or 8 with 6 where there is little to stream
 constexpr int kFewWarps = 8;
 constexpr float kMaxExp = 40.0f;   // e of a segment without a value scale so far (2^-24 alone needs 38)
@@ -697,11 +698,11 @@ __device__ __forceinline__ void attend_tokens(const Tokens& a, int nb, int j0, i
 // call 0.3 (bf16) to 1 us (fp16); a look at the sums and the code in the combine
 // cost 1 to 2.
 //
-// 8192 tokens for 64 x 32 heads over 8 (128 CTAs of 8 blocks) take 22 us, 4 of
+// 8192 tokens for 64 x 32 heads over 8 (128 CTAs of 8 blocks) take 23 us, 4 of
 // them the set-up to the first scores, 3 the last stores; a block takes 3900
-// clocks (2700 without the low parts): the chain S -> P -> P V and next S of a
-// tile, of which the products are 1130 (560). Steps of 32 keys with the scores
-// one step ahead took as long.
+// clocks (2700 without any low part): the chain S -> P -> P V and next S of a
+// tile, of which the products are 1130 (850 without V's low part, 560 without
+// either). Steps of 32 keys with the scores one step ahead took as long.
 //
 // Warps: 0-3 / 4-7 softmax of tile 0 / 1, 8 MMA issue and TMEM, 9-16 copy and
 // dequantise 8 tokens of each block (a block of 32 values per thread), each
@@ -1166,8 +1167,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) fa_paged_prefix_kernel(cons
 // warp w takes states w, w + WR, ..., kAtOnce loads in flight, and the first
 // one adds the others' sums from shared memory in their order. The grid is at
 // most what is resident at once, so that the scan of the lengths is paid once.
-// Bound by the states' bytes and the launch: 64 x 32 rows of 128 with 18 prefix
-// chunks (19 MB) and their segments take 10 us from cold caches.
+// Bound by the states' bytes and the launch: 64 x 32 rows of 128 with 16 prefix
+// chunks (17 MB) and their segments take 12 us from cold caches, 10 by themselves.
 struct CombineArgs {
   Split split;
   const float* part;
@@ -1325,7 +1326,10 @@ int workers_of(const FaPagedArgs& a, int warps) {
 // sequence. Where those are few they are streamed (us with and without it, 8
 // KV heads of 128, 300 tokens behind the prefix: 8 sequences behind 1024 18.5
 // and 17.1, behind 4096 24.0 and 32.8; 32 behind 256 19.3 and 17.2, behind 1024
-// 23.3 and 34.9). Streaming needs a prefix of whole groups of 8.
+// 23.3 and 34.9; heads of 64: 32 behind 256 20.7 and 18.7, behind 1024 20.7 and
+// 25.0; 32 KV heads: 8 behind 1024 29.1 and 33.6; one KV head: 32 behind 1024 18.6
+// and 15.1, behind 4096, where the rule is 2 us off, 24.8 and 22.4). Streaming
+// needs a prefix of whole groups of 8.
 constexpr int kPrefixUnits = 40;  // units of repeated reading per SM that it pays from
 bool use_prefix(const FaPagedArgs& a) {
   if (a.prefix_len <= 0 || a.D > 128 || a.B <= 1) return false;
@@ -1456,7 +1460,9 @@ kq_status_t launch_fa_paged(const FaPagedArgs& a, int dtype, cudaStream_t s) {
   // Little to stream is bound by latency: fewer warps with deeper rings start
   // sooner (3000 tokens of one sequence, 8 KV heads of 128: 11.0 us with 8
   // warps, 13.7 with 12; 4 x 9000: 21.8 and 25.3); more is bound by issue
-  // slots (16 x 3000: 30.1 and 28.1, 16 x 16000: 112 and 102).
+  // slots (16 x 3000: 30.1 and 28.1, 16 x 16000: 112 and 102). Heads of 64: 4 x
+  // 9000 22.8 and 23.7, 16 x 3000 29.4 and 26.9; 32 KV heads: 1 x 3000 16.6 and
+  // 18.6, 4 x 9000 88 and 84; one KV head: 16 x 9000 20.6 and 24.1.
   const long long units = (long long)a.B * a.Hkv * p.QG * ((p.split.limit - p.split.start) / kUnit + 1);
   p.warps = units <= 16ll * kFewWarps * sm_count() ? kFewWarps : kStreamWarps;
   p.split.workers = workers_of(a, p.warps);

@@ -146,6 +146,9 @@ __global__ void __launch_bounds__(kSimpleWarps * 32) fa_prompt_simple_kernel(con
 // 2^kLazy (then O is rescaled in TMEM): p stays below 2^(kBias + kLazy), inside
 // fp16, and the factor cancels in O / l. P is rounded to the inputs' type, as
 // the product with V needs both operands in it; l sums the unrounded p in fp32.
+// That is one more rounding of the output's own size, averaged over the keys
+// (relative errors 2.6e-4 in fp16 and 2.3e-3 in bf16 at most, 2.0e-4 and 1.7e-3
+// with P in fp32); a second product with P's remainder would double P V.
 //
 // TILES = 2, BLK = 128: one CTA per SM, K and V read once for 256 rows. The
 // tiles alternate: the softmax warps of one work while the tensor core runs
@@ -811,7 +814,9 @@ Plan plan_of(const FaPromptArgs& a) {
   Plan p;
   // two tiles per CTA where sequences are long (us for 8192 tokens of equal
   // sequences, 32 heads over 8 of 128, one tile and two: 256 each 52 and 56, 768
-  // 75 and 80, 1024 95 and 96, 2048 158 and 152, 8192 521 and 480)
+  // 75 and 80, 1024 95 and 96, 2048 158 and 152, 8192 521 and 480; heads of 64: 512
+  // 58 and 64, 1024 82 and 85, 2048 135 and 130; 16 ungrouped heads: 45 and 49, 60
+  // and 62, 86 and 84; 8 heads over one: 27 and 31, 38 and 41, 58 and 58)
   p.tiles = keys >= 1024 ? 2 : 1;
   p.slots = a.Tq / (TQ * p.tiles) + a.B;
   // few CTAs against many keys: split the keys so that the SMs are full once,

@@ -256,10 +256,12 @@ __device__ __forceinline__ uint32_t code_of(float x, float d, float inv) {
 // The bytes go through shared memory, laid out as far from a 16-byte boundary
 // as their place in the cache is, so that they leave in whole 16-byte pieces:
 // blocks of 34 bytes stored code by code leave half-written sectors behind,
-// which made 4096 rows of 8 x 128 (26 MB in and out) take 24 us instead of 16;
-// 13.8 with one division per block and no conversions. Bound by the quantiser's
-// arithmetic and the loads' latency; segments of 16 blocks gain 1 us on single
-// rows and lose 10 there.
+// which made 4096 rows of 8 x 128 (26 MB in and out, 3.9 us of traffic) take 24
+// us instead of 16; 13.8 with one division per block and no conversions. While
+// it runs it issues 2.7 of 4 instructions a clock, with 40% of the warps that fit:
+// 64 to 80 registers leave three or four CTAs per SM, 1.7 waves of one segment per
+// warp, so that no segment's loads run under another one's quantiser. Segments of
+// 16 blocks gain 1 us on single rows and lose 10 there.
 constexpr int kSegBlocks = 32;
 static_assert(kSegBlocks == 32, "a lane divides out the scale of one block of the segment");
 constexpr int kSegRoom = (kSegBlocks * kQ8 + 16 + 15) / 16 * 16;
@@ -366,7 +368,8 @@ struct ReadArgs {
 // flight at once, then each unit is laid out in shared memory and lane l
 // converts its codes 8 l, 8 l + 256, ..., 16 bytes out at a time. A row whose
 // page id is outside the cache, and a row that no sequence owns, is zero.
-// Bound by memory, 34 bytes in and 64 out per block. More units per warp put
+// 34 bytes in and 64 out per block, 4.8 TB/s, next to the issue slots (2.8 of 4
+// instructions a clock) and half of the conversion pipe. More units per warp put
 // more loads in flight but leave fewer warps: 22445 rows of 8 x 128 after 4096
 // written take 50.7 us with 1, 46.0 with 2, 51.4 with 4 (both calls; 43.5 since the
 // write is faster).

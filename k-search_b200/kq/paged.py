@@ -210,7 +210,9 @@ def flash_prompt_ragged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_se
     [B+1] on the device (cu_seqlens_k defaults to cu_seqlens_q). causal: row i
     of a sequence sees keys up to i + (len_k - len_q), so a chunk sees the
     context before it; a row without keys is zero, rows that no sequence owns
-    are not specified. Prefix sums are cut to the rows that there are."""
+    are not specified. Prefix sums are cut to the rows that there are. Heads
+    above 128 dims, and views whose rows do not start at multiples of 16 bytes,
+    take a scalar kernel that is a hundred times slower and more."""
     dt = _float16(q, "q")
     Tq, Hq, D = _rows(q, "q", q.dtype)
     dev = q.device
@@ -248,7 +250,8 @@ def flash_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     through row 0 of block_tables, once for the whole batch where that pays.
     max_seqlen (host) bounds seq_lens, longer sequences are cut to it; it
     defaults to the tables' width, and a bound close to the true lengths gives
-    the better work split."""
+    the better work split. Pages of a multiple of 8 tokens are the fast ones:
+    others take a scalar kernel, some 50 times slower."""
     dt = _float16(q, "q")
     B, Hq, D = _rows(q, "q", q.dtype)
     dev = q.device
