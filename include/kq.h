@@ -395,7 +395,8 @@ kq_status_t kq_fa_prompt(int dtype, const void* q, const void* k, const void* v,
  * [B, Hq, D] contiguous, of dtype; seq_lens int32 [B] (device), 0 for a
  * padding row (its output is zero). The first prefix_len tokens are the same
  * pages for every sequence: they are read through row 0 of block_tables (once
- * for the whole batch where that pays); a sequence shorter than that sees its
+ * for the whole batch where that pays), which names them even where row 0 is a
+ * padding row; a sequence shorter than that sees its
  * first seq_lens[b] of them. max_seqlen bounds the lengths (it sizes the work
  * split; longer sequences are cut to it). Tokens in pages outside the cache
  * are hidden, and what tokens hold that a row does not see never reaches it.

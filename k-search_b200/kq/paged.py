@@ -247,7 +247,8 @@ def flash_decode_paged(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     [B, Hq, D]. q fp16 or bf16 [B, Hq, D]; block_tables int32 [B, max_blocks];
     seq_lens int32 [B] (device; 0: a padding row, zeros out). The first
     prefix_len tokens are the same pages for every sequence: they are read
-    through row 0 of block_tables, once for the whole batch where that pays.
+    through row 0 of block_tables (also where row 0 is a padding row), once for
+    the whole batch where that pays.
     max_seqlen (host) bounds seq_lens, longer sequences are cut to it; it
     defaults to the tables' width, and a bound close to the true lengths gives
     the better work split. Pages of a multiple of 8 tokens are the fast ones:
